@@ -49,7 +49,9 @@ enum vnx_status {
                                  point's fixed scratch          -> ValueError   */
 };
 
-enum vnx_dtype { VNX_F32 = 0, VNX_BF16 = 1, VNX_F16 = 2 };
+/* VNX_I8 and VNX_E4M3 (OCP fp8, 4 exponent and 3 mantissa bits) are codes of the
+ * 8-bit KV cache only. */
+enum vnx_dtype { VNX_F32 = 0, VNX_BF16 = 1, VNX_F16 = 2, VNX_I8 = 3, VNX_E4M3 = 4 };
 
 /* Flags written by vnx_spec_accept, one byte per (row, position). */
 enum vnx_accept_flag {
@@ -850,6 +852,132 @@ int vnx_expert_gemm_bf16_rows(const void* x, int64_t ldx, int64_t sxb, const voi
                               int64_t N, int64_t K, int experts, int epilogue, const float* comb, int64_t ldc,
                               const int32_t* rows, const int32_t* counts, int64_t total_rows, void* y, int y_dtype,
                               int64_t ldy, int64_t syb, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * The KV cache in 8 bits.  A cache row (one token of one KV head, d values x)
+ * is d codes in the cache's type and one fp32 scale:
+ *   VNX_I8    scale = RN(max|x| / 127), code = rint(x * RN(127 / max|x|))
+ *   VNX_E4M3  scale = RN(max|x| / 448), code = e4m3(x * RN(448 / max|x|))
+ * (nearest, ties to even) and stands for code * scale.  A row whose maximum is
+ * below 2^-100 has codes and scale 0; one with an infinity or a NaN has codes 0
+ * and scale NaN.  Half the bytes of a bf16 cache, to hold and to read.  The
+ * reference has no counterpart (its ParallelKVCache, kv_cache_parallel.py:
+ * 42-286, holds fp32 / fp16 rows).  Caches (B, Hkv, cap, d) with strides {batch,
+ * head, row} in elements and unit last stride, both caches alike, rows 16-byte
+ * aligned; scales (B, Hkv, cap) fp32 with strides {batch, head} and unit last
+ * stride, both alike.
+ *
+ * vnx_kv_write: rows of q | k | v heads (H, Hkv, Hkv of d values; row b*n + i
+ * at qkv + (b*n + i)*ldq, dtype VNX_F32 / VNX_BF16 / VNX_F16) at positions
+ * lens[b] + i:
+ *   q_norm / k_norm (d fp32; NULL: none)  x = x / sqrt(mean(x^2) + eps) * w of
+ *     every query / key head;
+ *   cos_table / sin_table ((table_rows, d) fp32; NULL: none)  x = x * cos +
+ *     rotate_half(x) * sin of queries and keys
+ *     (packages/verse_nex/verse_nex/tri_sparse_attn.py:182-221);
+ *   q_out (B, H, n, d) bf16 contiguous; keys and values into cache row
+ *     lens[b] + i, cache_dtype VNX_I8, VNX_E4M3 or VNX_BF16 (the values rounded;
+ *     k_scale / v_scale not used).
+ * Positions outside [0, cap) (and the tables) are skipped, their q_out rows
+ * zero.  d in {16, 32, 64, 128, 256}; pointers 16-byte aligned, ldq and strides
+ * multiples of 16 bytes.
+ * ------------------------------------------------------------------------- */
+typedef struct vnx_kv_write_args {
+  const void* qkv;
+  int64_t ldq;
+  const int32_t* lens;
+  const float* cos_table;
+  const float* sin_table;
+  int64_t table_rows;
+  const float* q_norm;
+  const float* k_norm;
+  void* q_out;
+  void* k_cache;
+  void* v_cache;
+  float* k_scale;
+  float* v_scale;
+  int64_t cache_strides[3];
+  int64_t scale_strides[2];
+  int64_t B, cap;
+  int n, H, Hkv, d;
+  int dtype, cache_dtype;
+  float eps;
+} vnx_kv_write_args;
+
+int vnx_kv_write(const vnx_kv_write_args* args, void* stream);
+
+/* vnx_kv_read: k_out / v_out (B, Hkv, rows, d) in out_dtype (VNX_F32, VNX_BF16 or
+ * VNX_F16, strides {batch, head, row} in elements, multiples of 16 bytes) = the
+ * values that cache rows start[b] + i stand for (start NULL: 0), zeros outside
+ * [0, cap).  VNX_I8, VNX_E4M3 or VNX_BF16 caches. */
+typedef struct vnx_kv_read_args {
+  const void* k_cache;
+  const void* v_cache;
+  const float* k_scale;
+  const float* v_scale;
+  const int32_t* start;
+  void* k_out;
+  void* v_out;
+  int64_t cache_strides[3];
+  int64_t scale_strides[2];
+  int64_t out_strides[3];
+  int64_t B, cap;
+  int rows, Hkv, d;
+  int cache_dtype, out_dtype;
+} vnx_kv_read_args;
+
+int vnx_kv_read(const vnx_kv_read_args* args, void* stream);
+
+/* vnx_tree_attn_q8: attention of N new rows of every batch row over its 8-bit
+ * cache, the new rows already in it (vnx_kv_write) at rows tp_b .. tp_b + N - 1,
+ * tp_b = lens[b] clamped to [0, Tp]:
+ *   out[b,h,i,:] = g0 * sum_j softmax_j(scale * q[b,h,i,:] . k_j) v_j
+ *                + g1 * (the same over the T2 rows of k_seg2 / v_seg2)
+ * over the cache rows j that node i sees:
+ *   anc and anc_host NULL  a chain of any length: rows j <= tp_b + i;
+ *   anc (device, (B, N) ancestor-or-self words, batch stride anc_batch_stride)
+ *   or anc_host (host, N words, shared)  a token tree, N <= 64: the prefix and
+ *     the rows tp_b + j of its set bits j, node i at position tp_b +
+ *     popcount(word i) - 1;
+ *   window > 0  only rows less than window positions behind (for a tree window
+ *     >= N, else VNX_ERR_UNSUPPORTED).
+ * A node that sees no row gets zeros from the first term.  T2 > 0: a second
+ * segment of bf16 rows ((B or 1, Hkv, T2, d), batch stride 0 when shared), all
+ * seen, and gates, two fp32 on the device; T2 == 0: g0 = 1 and no second term
+ * (TriSparse's global path and gates, tri_sparse_attn.py:469-495, :585-608).
+ * Query head h reads KV head h / (H / Hkv).  q bf16 (B, H, N, d), out VNX_BF16
+ * or VNX_F16, strides {batch, head, row} multiples of 8, pointers 16-byte
+ * aligned.  d in {64, 128}.  Tp + N <= cap.  Codes of e4m3 NaN must not stand in
+ * rows below tp_b + N (vnx_kv_write makes none).  One launch, or two when the
+ * keys are split over workgroups: the workspace
+ * (vnx_tree_attn_q8_workspace(args) bytes, no initialisation) then holds the
+ * partials. */
+typedef struct vnx_attn_q8_args {
+  const void* q;
+  const void* k_cache;
+  const void* v_cache;
+  const float* k_scale;
+  const float* v_scale;
+  const int32_t* lens;
+  const uint64_t* anc;
+  const uint64_t* anc_host;
+  void* out;
+  const void* k_seg2;
+  const void* v_seg2;
+  const float* gates;
+  int64_t q_strides[3];
+  int64_t cache_strides[3];
+  int64_t scale_strides[2];
+  int64_t out_strides[3];
+  int64_t seg2_strides[3];
+  int64_t anc_batch_stride, cap;
+  int B, H, Hkv, Tp, N, d;
+  int T2, window, kv_dtype, out_dtype;
+  float scale;
+} vnx_attn_q8_args;
+
+size_t vnx_tree_attn_q8_workspace(const vnx_attn_q8_args* args);
+int vnx_tree_attn_q8(const vnx_attn_q8_args* args, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 _PKG_DIR = os.path.dirname(os.path.abspath(__file__))
@@ -25,12 +26,16 @@ VNX_EPI_NONE, VNX_EPI_SWIGLU = 0, 1
 VNX_F32 = 0
 VNX_BF16 = 1
 VNX_F16 = 2
+VNX_I8 = 3
+VNX_E4M3 = 4
 
 try:
     import torch as _torch
     DTYPE_CODES = {_torch.float32: VNX_F32, _torch.bfloat16: VNX_BF16, _torch.float16: VNX_F16}
+    KV_DTYPE_CODES = {_torch.int8: VNX_I8, _torch.float8_e4m3fn: VNX_E4M3, _torch.bfloat16: VNX_BF16}
 except Exception:  # the CPU-only ABI tests do not need torch dtypes
     DTYPE_CODES = {}
+    KV_DTYPE_CODES = {}
 
 FLAG_NEAR_TIE = 1
 FLAG_LSE_EDGE = 2
@@ -177,6 +182,64 @@ SIGNATURES.update({
     "vnx_expert_gemm_bf16": (_int, [_vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _c_i64, _c_i64, _int, _int, _vp,
                                     _c_i64, _int, _vp, _vp, _vp, _vp, _int, _c_i64, _c_i64, _vp]),
 })
+
+
+class KvWriteArgs(ctypes.Structure):
+    """vnx_kv_write_args (include/vnx.h)."""
+    _fields_ = [
+        ("qkv", _vp), ("ldq", _c_i64), ("lens", _vp), ("cos_table", _vp), ("sin_table", _vp), ("table_rows", _c_i64),
+        ("q_norm", _vp), ("k_norm", _vp), ("q_out", _vp), ("k_cache", _vp), ("v_cache", _vp), ("k_scale", _vp),
+        ("v_scale", _vp), ("cache_strides", _c_i64 * 3), ("scale_strides", _c_i64 * 2), ("B", _c_i64), ("cap", _c_i64),
+        ("n", _int), ("H", _int), ("Hkv", _int), ("d", _int), ("dtype", _int), ("cache_dtype", _int), ("eps", _f32),
+    ]
+
+
+class KvReadArgs(ctypes.Structure):
+    """vnx_kv_read_args (include/vnx.h)."""
+    _fields_ = [
+        ("k_cache", _vp), ("v_cache", _vp), ("k_scale", _vp), ("v_scale", _vp), ("start", _vp), ("k_out", _vp),
+        ("v_out", _vp), ("cache_strides", _c_i64 * 3), ("scale_strides", _c_i64 * 2), ("out_strides", _c_i64 * 3),
+        ("B", _c_i64), ("cap", _c_i64), ("rows", _int), ("Hkv", _int), ("d", _int), ("cache_dtype", _int),
+        ("out_dtype", _int),
+    ]
+
+
+class AttnQ8Args(ctypes.Structure):
+    """vnx_attn_q8_args (include/vnx.h)."""
+    _fields_ = [
+        ("q", _vp), ("k_cache", _vp), ("v_cache", _vp), ("k_scale", _vp), ("v_scale", _vp), ("lens", _vp),
+        ("anc", _vp), ("anc_host", _vp), ("out", _vp), ("k_seg2", _vp), ("v_seg2", _vp), ("gates", _vp),
+        ("q_strides", _c_i64 * 3), ("cache_strides", _c_i64 * 3), ("scale_strides", _c_i64 * 2),
+        ("out_strides", _c_i64 * 3), ("seg2_strides", _c_i64 * 3), ("anc_batch_stride", _c_i64), ("cap", _c_i64),
+        ("B", _int), ("H", _int), ("Hkv", _int), ("Tp", _int), ("N", _int), ("d", _int), ("T2", _int),
+        ("window", _int), ("kv_dtype", _int), ("out_dtype", _int), ("scale", _f32),
+    ]
+
+
+SIGNATURES.update({
+    "vnx_kv_write": (_int, [_vp, _vp]),
+    "vnx_kv_read": (_int, [_vp, _vp]),
+    "vnx_tree_attn_q8_workspace": (_c_sz, [_vp]),
+    "vnx_tree_attn_q8": (_int, [_vp, _vp, _c_sz, _vp]),
+})
+
+
+def _packer(cls):
+    """The argument block as bytes, values in field order (arrays flattened,
+    None for a NULL pointer written as 0): struct.pack fills it in one call,
+    where a ctypes.Structure takes a Python call per field."""
+    code = {_vp: "P", _c_i64: "q", _int: "i", _f32: "f"}
+    fmt = "@" + "".join(code[t] if t in code else code[t._type_] * t._length_ for _, t in cls._fields_) + "0q"
+    s = struct.Struct(fmt)
+    if s.size != ctypes.sizeof(cls):
+        raise AssertionError(f"{cls.__name__}: {s.size} bytes packed, {ctypes.sizeof(cls)} declared")
+    return s.pack
+
+
+pack_kv_write = _packer(KvWriteArgs)
+pack_kv_read = _packer(KvReadArgs)
+pack_attn_q8 = _packer(AttnQ8Args)
+
 
 def stream_handle(index: int) -> int:
     """The current PyTorch stream of GPU `index` as the void* the entries take.

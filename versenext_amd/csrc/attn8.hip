@@ -1,0 +1,808 @@
+// Attention of the new rows of every sequence over its 8-bit KV cache
+// (vnx_tree_attn_q8) on gfx950: a token tree, a chain of any length, one token.
+//
+//   S_ij = scale * sk_j * (q_i . kc_j),  P = softmax over the keys i sees,
+//   O_i = sum_j P_ij sv_j vc_j           (kc, vc codes; sk, sv their scales)
+//   out_i = g0 * O_i + g1 * (the same over the second segment, bf16 rows)
+//
+// A code is exact in bf16 (8 significant bits), so both products run on
+// v_mfma_f32_16x16x32_bf16 with the codes as operands and the scales applied
+// to scores and probabilities, one multiply each.
+//
+// A wave owns 16 CT query columns of one KV head (column c is node c / rep of
+// query head kvh * rep + c % rep, so heads that share K and V share every
+// loaded row) and walks keys 32 at a time.  No row passes through LDS: each
+// operand is loaded in the order in which the matrix core wants it.
+//   S^T[key][col]    A = K: a lane holds 16 consecutive bytes of key lane % 16
+//                    (the order of d inside a product is free, q is loaded
+//                    the same way);
+//   O^T[dim][col]    A = V^T: a lane holds D / 16 consecutive bytes of each of
+//                    8 keys, row m of dim tile t standing for dim m D/16 + t.
+//                    The 8 keys are those of its own 8 scores, so P goes from
+//                    the score registers into the B operand as it is.
+// A step's rows are loaded into registers under the previous step's math.
+// Statistics and sums are fp32; P * sv is rounded once to bf16 (at most 2^-8
+// of each term, as much as the rounding of a bf16 output, and independent from
+// key to key).
+// The running maximum of a column moves only when a score passes it by 2^8:
+// until then P stays below 2^8 in fp32 sums and bf16 operands, and the step
+// needs no exchange between lanes and no rescaling.
+#include <climits>
+
+#include "kvcache.h"
+
+namespace vnx {
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+
+constexpr int kQ8MaxN = 64;      // nodes of a tree: bits of an ancestor word
+constexpr int kQ8Split = 32;     // key splits of a launch at most
+constexpr float kQ8Jump = 8.0f;  // log2 of what P may grow to before the maximum moves
+
+struct Q8Words {
+  uint64_t w[kQ8MaxN];
+};
+
+struct Q8Params {
+  const uint16_t* q;
+  const char* kc;
+  const char* vc;
+  const float* ks;
+  const float* vs;
+  const int32_t* lens;
+  const uint64_t* anc;     // per-row words on the device (tree == 2)
+  const char* k2;          // bf16 rows of the second segment
+  const char* v2;
+  const float* gates;
+  void* out;
+  float* part_o;           // [(unit * slots + slot) * 16 CT + col][D]
+  float2* part_ml;
+  int64_t q_sb, q_sh, q_sr;
+  int64_t c_sb, c_sh, c_sr;
+  int64_t s_sb, s_sh;
+  int64_t o_sb, o_sh, o_sr;
+  int64_t s2_sb, s2_sh, s2_sr;  // bytes
+  int64_t anc_sb;
+  int B, H, Hkv, rep, N, cols, Tp, T2, window;
+  int tree;                // 0 chain, 1 words by value, 2 words on the device
+  int groups, splits, slots;
+  int f16;                 // output type: fp16, else bf16
+  float c;                 // scale * log2(e)
+};
+
+__device__ __forceinline__ float q8_ex2(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// Maximum / sum over the four lanes lane % 16 + {0, 16, 32, 48}: v_permlane
+// swaps pair the halves without LDS.
+__device__ __forceinline__ float q8_max4(float x) {
+  auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float q8_sum4(float x) {
+  auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// Where a wave's keys lie.
+struct Q8Src {
+  const char* k;
+  const char* v;
+  const float* ks;
+  const float* vs;
+  uint32_t sr;   // row pitch in bytes
+  int rows;      // rows that may be read
+};
+
+// The loaded rows of one step of 32 keys.
+template <int D, int KT>
+struct Q8Rows {
+  static constexpr int E = KT == KV_BF16 ? 2 : 1;
+  static constexpr int KW = D / 64 * E;     // 16-byte loads a key tile
+  static constexpr int VW = D / 64 * E;     // words of a key's V a lane
+  u32x4 k[2][KW];
+  uint32_t v[8][VW];
+  f32x4 sk[2], sv[2];
+
+  // Rows past the last one are read as the last one (their scores are masked).
+  template <bool TAIL>
+  __device__ __forceinline__ void load(const Q8Src& s, int k0, int lane) {
+    const int m = lane & 15, g = lane >> 4;
+    const int last = s.rows - 1 - k0;
+    const char* kb = s.k + (int64_t)k0 * s.sr;
+    const char* vb = s.v + (int64_t)k0 * s.sr;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int r = TAIL ? min(16 * t + m, last) : 16 * t + m;
+      const uint32_t o = (uint32_t)r * s.sr + (uint32_t)g * (16 * E);
+#pragma unroll
+      for (int i = 0; i < KW; ++i)
+        k[t][i] = *reinterpret_cast<const u32x4*>(kb + (o + (uint32_t)(E == 1 ? 64 * i : 128 * (i / 2) + 16 * (i % 2))));
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int rr = (j < 4 ? 0 : 16) + 4 * g + (j & 3);
+      const int r = TAIL ? min(rr, last) : rr;
+      const uint32_t o = (uint32_t)r * s.sr + (uint32_t)m * (D / 16 * E);
+      if constexpr (VW == 1) {
+        v[j][0] = *reinterpret_cast<const uint32_t*>(vb + o);
+      } else if constexpr (VW == 2) {
+        const uint2 w = *reinterpret_cast<const uint2*>(vb + o);
+        v[j][0] = w.x; v[j][1] = w.y;
+      } else {
+        const u32x4 w = *reinterpret_cast<const u32x4*>(vb + o);
+        v[j][0] = w[0]; v[j][1] = w[1]; v[j][2] = w[2]; v[j][3] = w[3];
+      }
+    }
+    if constexpr (KT != KV_BF16) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int r = 16 * t + 4 * g;
+        if constexpr (TAIL) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int rc = k0 + min(r + i, last);
+            sk[t][i] = s.ks[rc];
+            sv[t][i] = s.vs[rc];
+          }
+        } else {
+          sk[t] = *reinterpret_cast<const f32x4u*>(s.ks + k0 + r);
+          sv[t] = *reinterpret_cast<const f32x4u*>(s.vs + k0 + r);
+        }
+      }
+    }
+  }
+
+  // K operands of key tile t.
+  __device__ __forceinline__ void kfrag(int t, bf16x8 (&f)[D / 32]) const {
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s) {
+      u32x4 w;
+      if constexpr (KT == KV_BF16) {
+        w = k[t][s];
+      } else {
+        const u32x4 c = k[t][s / 2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t x = c[2 * (s % 2) + h];
+          if constexpr (KT == KV_E4M3) {
+            w[2 * h] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, false));
+            w[2 * h + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, true));
+          } else {
+            float y[4];
+            kv_f32x4<KV_I8>(x, y);
+            w[2 * h] = kv_pk_bf16(y[0], y[1]);
+            w[2 * h + 1] = kv_pk_bf16(y[2], y[3]);
+          }
+        }
+      }
+      f[s] = __builtin_bit_cast(bf16x8, w);
+    }
+  }
+
+  // V^T operands: dim tile t, keys j of this lane.
+  __device__ __forceinline__ void vfrag(bf16x8 (&f)[D / 16]) const {
+#pragma unroll
+    for (int x = 0; x < VW; ++x) {
+      constexpr int PW = KT == KV_BF16 ? 2 : 4;  // dims of a word
+      uint32_t w[PW][4];
+      if constexpr (KT == KV_BF16) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          w[0][j] = __builtin_amdgcn_perm(v[2 * j + 1][x], v[2 * j][x], 0x05040100u);
+          w[1][j] = __builtin_amdgcn_perm(v[2 * j + 1][x], v[2 * j][x], 0x07060302u);
+        }
+      } else if constexpr (KT == KV_E4M3) {
+        uint32_t c[8][2];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          c[j][0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[j][x], 1.0f, false));
+          c[j][1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[j][x], 1.0f, true));
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            w[2 * h][j] = __builtin_amdgcn_perm(c[2 * j + 1][h], c[2 * j][h], 0x05040100u);
+            w[2 * h + 1][j] = __builtin_amdgcn_perm(c[2 * j + 1][h], c[2 * j][h], 0x07060302u);
+          }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float a[4], b[4];
+          kv_f32x4<KV_I8>(v[2 * j][x], a);
+          kv_f32x4<KV_I8>(v[2 * j + 1][x], b);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[i][j] = kv_pk_bf16(a[i], b[i]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < PW; ++i) f[PW * x + i] = __builtin_bit_cast(bf16x8, u32x4{w[i][0], w[i][1], w[i][2], w[i][3]});
+    }
+  }
+};
+
+// What the columns of a wave see: keys [lo, hi) of its own, of which keys from
+// tp on only where the word has their bit (trees).  Keys [full_lo, full_hi)
+// are seen by every column.
+template <int CT>
+struct Q8Mask {
+  int lo[CT], hi[CT];
+  uint64_t word[CT];
+  int tp, full_lo, full_hi;
+  bool tree;
+};
+
+enum { Q8_SOFTMAX = 0, Q8_STATS = 1, Q8_FIXED = 2 };
+
+// Walks steps s0, s0 + ds, .. < s1 of 32 keys from key `first` on.
+//   Q8_SOFTMAX  online softmax: acc, m (the columns' maxima, the same in the
+//               four lanes of a column), l (this lane's share of the sums)
+//   Q8_STATS    m and l alone
+//   Q8_FIXED    acc += (exp2(x - m) * l) sv v: given maxima, l a weight
+template <int D, int KT, int CT, int MODE>
+__device__ __forceinline__ void q8_walk(const Q8Src& src, int first, int s0, int ds, int s1, const Q8Mask<CT>& mk,
+                                        float c, const bf16x8 (&qf)[CT][D / 32], f32x4 (&acc)[CT][D / 16],
+                                        float (&m)[CT], float (&l)[CT], int lane) {
+  if (s0 >= s1) return;
+  const int g4 = (lane >> 4) * 4;
+  Q8Rows<D, KT> rows;
+  auto fetch = [&](int s) {
+    const int k0 = first + 32 * s;
+    if (k0 + 32 <= src.rows) rows.template load<false>(src, k0, lane);
+    else rows.template load<true>(src, k0, lane);
+  };
+  fetch(s0);
+  for (int s = s0; s < s1; s += ds) {
+    const int k0 = first + 32 * s;
+    bf16x8 kf[2][D / 32], vf[D / 16];
+    rows.kfrag(0, kf[0]);
+    rows.kfrag(1, kf[1]);
+    if constexpr (MODE != Q8_STATS) rows.vfrag(vf);
+    float fk[8], sv[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      fk[e] = KT == KV_BF16 ? c : rows.sk[e / 4][e % 4] * c;
+      sv[e] = KT == KV_BF16 ? 1.0f : rows.sv[e / 4][e % 4];
+    }
+    if (s + ds < s1) fetch(s + ds);
+    const bool full = k0 >= mk.full_lo && k0 + 32 <= mk.full_hi;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      float x[8];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        f32x4 a = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[t][i], qf[ct][i], a, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[4 * t + i] = a[i] * fk[4 * t + i];
+      }
+      uint32_t hide = 0;
+      if (!full) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int key = k0 + 16 * (e / 4) + g4 + e % 4;
+          bool see = key >= mk.lo[ct] && key < mk.hi[ct];
+          if (mk.tree && key >= mk.tp) see = see && ((mk.word[ct] >> ((key - mk.tp) & 63)) & 1);
+          if (!see) {
+            x[e] = kNegInf;
+            hide |= 1u << e;
+          }
+        }
+      }
+      if constexpr (MODE != Q8_FIXED) {
+        float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+        if (__any(top > m[ct] + kQ8Jump)) {
+          const float mn = fmaxf(m[ct], q8_max4(top));
+          const float al = mn == kNegInf ? 1.0f : q8_ex2(m[ct] - mn);
+          m[ct] = mn;
+          l[ct] *= al;
+          if constexpr (MODE == Q8_SOFTMAX) {
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) acc[ct][d] *= al;
+          }
+        }
+      }
+      const float mu = m[ct] == kNegInf ? 0.0f : m[ct];
+      float pv[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float pe = q8_ex2(x[e] - mu);
+        if constexpr (MODE == Q8_FIXED) pe *= l[ct];
+        else l[ct] += pe;
+        pv[e] = pe * sv[e];
+      }
+      if constexpr (MODE != Q8_STATS) {
+        if (!full) {  // a hidden row's scale may be NaN: nothing of it is kept
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (hide & (1u << e)) pv[e] = 0.0f;
+        }
+        const u32x4 w = {kv_pk_bf16(pv[0], pv[1]), kv_pk_bf16(pv[2], pv[3]), kv_pk_bf16(pv[4], pv[5]),
+                         kv_pk_bf16(pv[6], pv[7])};
+        const bf16x8 pf = __builtin_bit_cast(bf16x8, w);
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d)
+          acc[ct][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[d], pf, acc[ct][d], 0, 0, 0);
+      }
+    }
+  }
+}
+
+// A column's node and query head.
+__device__ __forceinline__ void q8_col(const Q8Params& p, int col, int& node, int& h) {
+  node = col / p.rep;
+  h = col - node * p.rep;
+}
+
+template <int D, int CT>
+struct Q8Tile {
+  int b, kvh, col0, tp;
+  bf16x8 qf[CT][D / 32];
+  Q8Mask<CT> mask;
+  Q8Src src;
+  int first, steps;   // steps of 32 keys from key first on
+  Q8Src src2;
+
+  // E: bytes of the cache's elements
+  __device__ __forceinline__ void init(const Q8Params& p, const Q8Words& tw, int bh, int c0, int lane) {
+    const int m = lane & 15, g = lane >> 4;
+    b = bh / p.Hkv;
+    kvh = bh - b * p.Hkv;
+    col0 = c0;
+    tp = uni(min(max(p.lens[b], 0), p.Tp));
+    const int n0 = c0 / p.rep, n1 = min((c0 + 16 * CT - 1) / p.rep, p.N - 1);
+    const int W = p.window > 0 ? p.window : INT_MAX;
+    mask.tp = tp;
+    mask.tree = p.tree != 0;
+    const int rows = tp + p.N;
+    int lo_min, hi_max;
+    if (p.tree) {
+      lo_min = p.window > 0 ? max(0, tp - 1 - W + 1) : 0;             // an empty word sits at tp - 1
+      mask.full_lo = p.window > 0 ? max(0, tp + p.N - 1 - W + 1) : 0;  // depth N - 1 at most
+      hi_max = rows;
+      mask.full_hi = tp;
+    } else {
+      lo_min = p.window > 0 ? max(0, tp + n0 - W + 1) : 0;
+      mask.full_lo = p.window > 0 ? max(0, tp + n1 - W + 1) : 0;
+      hi_max = tp + n1 + 1;
+      mask.full_hi = tp + n0 + 1;
+    }
+    first = lo_min & ~15;
+    steps = (hi_max - first + 31) / 32;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      const int col = min(c0 + 16 * ct + m, p.cols - 1);
+      int node, h;
+      q8_col(p, col, node, h);
+      const uint16_t* q = p.q + b * p.q_sb + (int64_t)(kvh * p.rep + h) * p.q_sh + (int64_t)node * p.q_sr;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+        qf[ct][i] = *reinterpret_cast<const bf16x8*>(q + 64 * (i / 2) + 16 * g + 8 * (i % 2));
+      int pos = tp + node;
+      mask.word[ct] = 0;
+      mask.hi[ct] = pos + 1;
+      if (p.tree) {
+        const uint64_t w = p.tree == 1 ? tw.w[node] : p.anc[b * p.anc_sb + node];
+        mask.word[ct] = w;
+        mask.hi[ct] = rows;
+        pos = tp + __popcll(w) - 1;
+      }
+      mask.lo[ct] = p.window > 0 ? pos - W + 1 : 0;
+    }
+    const int64_t kv = b * p.c_sb + kvh * p.c_sh, ss = b * p.s_sb + kvh * p.s_sh;
+    src.k = p.kc + kv;
+    src.v = p.vc + kv;
+    src.ks = p.ks + ss;
+    src.vs = p.vs + ss;
+    src.sr = (uint32_t)p.c_sr;
+    src.rows = rows;
+    const int64_t s2 = b * p.s2_sb + kvh * p.s2_sh;
+    src2.k = p.k2 + s2;
+    src2.v = p.v2 + s2;
+    src2.ks = src2.vs = nullptr;
+    src2.sr = (uint32_t)p.s2_sr;
+    src2.rows = p.T2;
+  }
+
+  __device__ __forceinline__ Q8Mask<CT> mask2(int T2) const {
+    Q8Mask<CT> k;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) { k.lo[ct] = 0; k.hi[ct] = T2; k.word[ct] = 0; }
+    k.tp = 0; k.full_lo = 0; k.full_hi = T2; k.tree = false;
+    return k;
+  }
+};
+
+template <int NW>
+__device__ __forceinline__ void q8_store(const Q8Params& p, int64_t off, const float* v) {
+  uint32_t w[NW / 2];
+#pragma unroll
+  for (int i = 0; i < NW / 2; ++i) {
+    if (p.f16) w[i] = __builtin_bit_cast(uint32_t, f16x2{(_Float16)v[2 * i], (_Float16)v[2 * i + 1]});
+    else w[i] = kv_pk_bf16(v[2 * i], v[2 * i + 1]);
+  }
+  uint16_t* o = static_cast<uint16_t*>(p.out) + off;
+  if constexpr (NW == 4) {
+    *reinterpret_cast<uint2*>(o) = make_uint2(w[0], w[1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < NW / 8; ++i)
+      *reinterpret_cast<u32x4*>(o + 8 * i) = u32x4{w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
+  }
+}
+
+__device__ __forceinline__ int64_t q8_out_off(const Q8Params& p, int b, int kvh, int col) {
+  int node, h;
+  q8_col(p, col, node, h);
+  return b * p.o_sb + (int64_t)(kvh * p.rep + h) * p.o_sh + (int64_t)node * p.o_sr;
+}
+
+// Many columns (prompts): a wave per column tile, no exchange between waves.
+// The second segment follows the walk in two passes (its maxima and sums, then
+// its rows weighted by g1 / sum), so that it needs no accumulators of its own.
+template <int D, int KT, int CT>
+__global__ __launch_bounds__(256, D == 64 ? 2 : 1) void k_attn8_wide(Q8Params p, Q8Words tw) {
+  const int lane = threadIdx.x & 63, w = uni(threadIdx.x >> 6);
+  const int BH = p.B * p.Hkv;
+  // later tiles see the most keys and start first; the tiles of a head share an XCD where BH % 8 == 0
+  const int bh = blockIdx.x % BH, grp = p.groups - 1 - blockIdx.x / BH;
+  const int c0 = (grp * 4 + w) * 16 * CT;
+  if (c0 >= p.cols) return;
+  Q8Tile<D, CT> t;
+  t.init(p, tw, bh, c0, lane);
+  f32x4 acc[CT][D / 16];
+  float m[CT], l[CT];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    m[ct] = kNegInf;
+    l[ct] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) acc[ct][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  q8_walk<D, KT, CT, Q8_SOFTMAX>(t.src, t.first, 0, 1, t.steps, t.mask, p.c, t.qf, acc, m, l, lane);
+  const float g0 = p.T2 > 0 ? p.gates[0] : 1.0f;
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const float sum = q8_sum4(l[ct]);
+    const float inv = sum == 0.0f ? 0.0f : g0 / sum;
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) acc[ct][d] *= inv;
+    m[ct] = kNegInf;
+    l[ct] = 0.0f;
+  }
+  if (p.T2 > 0) {
+    const Q8Mask<CT> mk = t.mask2(p.T2);
+    const int s1 = (p.T2 + 31) / 32;
+    q8_walk<D, KV_BF16, CT, Q8_STATS>(t.src2, 0, 0, 1, s1, mk, p.c, t.qf, acc, m, l, lane);
+    const float g1 = p.gates[1];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) l[ct] = g1 / q8_sum4(l[ct]);
+    q8_walk<D, KV_BF16, CT, Q8_FIXED>(t.src2, 0, 0, 1, s1, mk, p.c, t.qf, acc, m, l, lane);
+  }
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const int col = c0 + 16 * ct + (lane & 15);
+    if (col < p.cols) {
+      float v[D / 4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) v[i * (D / 16) + d] = acc[ct][d][i];
+      q8_store<D / 4>(p, q8_out_off(p, t.b, t.kvh, col) + (lane >> 4) * (D / 4), v);
+    }
+  }
+}
+
+// Few columns: the keys of a column group are split over `splits` workgroups
+// and over the 4 waves of each; a fifth wave takes the second segment (in the
+// last split).  The waves' (acc, m, l) meet in LDS; with one split the result
+// is written, else the split's partial (relative to its own maxima).
+template <int D, int KT, int CT>
+__global__ __launch_bounds__(320, 1) void k_attn8_split(Q8Params p, Q8Words tw) {
+  constexpr int PD = D + 4;  // row pitch: four columns' 16-byte writes on distinct banks
+  __shared__ __attribute__((aligned(16))) float s_o[5 * 16 * PD];
+  __shared__ float s_m[5][16 * CT], s_l[5][16 * CT];
+  const int lane = threadIdx.x & 63, w = uni(threadIdx.x >> 6);
+  const int BH = p.B * p.Hkv;
+  const int bh = blockIdx.x % BH, rest = blockIdx.x / BH;
+  const int grp = rest % p.groups, split = rest / p.groups;
+  Q8Tile<D, CT> t;
+  t.init(p, tw, bh, grp * 16 * CT, lane);
+  f32x4 acc[CT][D / 16];
+  float m[CT], l[CT];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    m[ct] = kNegInf;
+    l[ct] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) acc[ct][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  const bool second = p.T2 > 0 && split == p.splits - 1;
+  if (w < 4) {
+    const int per = (t.steps + p.splits - 1) / p.splits;
+    const int s1 = min(t.steps, (split + 1) * per);
+    q8_walk<D, KT, CT, Q8_SOFTMAX>(t.src, t.first, split * per + w, 4, s1, t.mask, p.c, t.qf, acc, m, l, lane);
+  } else if (second) {
+    q8_walk<D, KV_BF16, CT, Q8_SOFTMAX>(t.src2, 0, 0, 1, (p.T2 + 31) / 32, t.mask2(p.T2), p.c, t.qf, acc, m, l, lane);
+  }
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    l[ct] = q8_sum4(l[ct]);
+    if (lane < 16) {
+      s_m[w][16 * ct + lane] = m[ct];
+      s_l[w][16 * ct + lane] = l[ct];
+    }
+  }
+  const float g0 = p.T2 > 0 ? p.gates[0] : 1.0f, g1 = p.T2 > 0 ? p.gates[1] : 0.0f;
+  const int64_t unit = (int64_t)bh * p.groups + grp;
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    float* o = s_o + (w * 16 + (lane & 15)) * PD + (lane >> 4) * (D / 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int d = 0; d < D / 16; d += 4)
+        *reinterpret_cast<f32x4*>(o + i * (D / 16) + d) =
+            f32x4{acc[ct][d][i], acc[ct][d + 1][i], acc[ct][d + 2][i], acc[ct][d + 3][i]};
+    __syncthreads();
+    const int cc = threadIdx.x / 16, dd = threadIdx.x % 16 * (D / 16);
+    const int col = t.col0 + 16 * ct + cc;
+    if (threadIdx.x < 256 && col < p.cols) {
+      float mx = kNegInf;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s_m[i][16 * ct + cc]);
+      float sum = 0.0f, v[D / 16] = {};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float mi = s_m[i][16 * ct + cc];
+        const float e = mi == kNegInf ? 0.0f : q8_ex2(mi - mx);
+        sum += s_l[i][16 * ct + cc] * e;
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) v[d] = fmaf(s_o[(i * 16 + cc) * PD + dd + d], e, v[d]);
+      }
+      if (p.splits == 1) {
+        const float inv = sum == 0.0f ? 0.0f : g0 / sum;
+        const float inv2 = second ? g1 / s_l[4][16 * ct + cc] : 0.0f;
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) {
+          v[d] *= inv;
+          if (second) v[d] = fmaf(s_o[(4 * 16 + cc) * PD + dd + d], inv2, v[d]);
+        }
+        q8_store<D / 16>(p, q8_out_off(p, t.b, t.kvh, col) + dd, v);
+      } else {
+        const int64_t r = (unit * p.slots + split) * (16 * CT) + 16 * ct + cc;
+#pragma unroll
+        for (int d = 0; d < D / 16; d += 4)
+          *reinterpret_cast<f32x4*>(p.part_o + r * D + dd + d) = f32x4{v[d], v[d + 1], v[d + 2], v[d + 3]};
+        if (dd == 0) p.part_ml[r] = make_float2(mx, sum);
+        if (second) {
+          const int64_t r2 = (unit * p.slots + p.splits) * (16 * CT) + 16 * ct + cc;
+#pragma unroll
+          for (int d = 0; d < D / 16; ++d) v[d] = s_o[(4 * 16 + cc) * PD + dd + d];
+#pragma unroll
+          for (int d = 0; d < D / 16; d += 4)
+            *reinterpret_cast<f32x4*>(p.part_o + r2 * D + dd + d) = f32x4{v[d], v[d + 1], v[d + 2], v[d + 3]};
+          if (dd == 0) p.part_ml[r2] = make_float2(s_m[4][16 * ct + cc], s_l[4][16 * ct + cc]);
+        }
+      }
+    }
+    if (ct + 1 < CT) __syncthreads();  // s_o is written again
+  }
+}
+
+// Joins the splits' partials: four dims of a column a thread.
+template <int D>
+__global__ __launch_bounds__(256) void k_attn8_join(Q8Params p, int ct16) {
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int dd = (int)(id % (D / 4)) * 4;
+  const int64_t cell = id / (D / 4);   // unit * ct16 + column of the group
+  const int64_t unit = cell / ct16;
+  if (unit >= (int64_t)p.B * p.Hkv * p.groups) return;
+  const int cc = (int)(cell - unit * ct16);
+  const int bh = (int)(unit / p.groups), grp = (int)(unit - (int64_t)bh * p.groups);
+  const int col = grp * ct16 + cc;
+  if (col >= p.cols) return;
+  const int64_t r0 = unit * p.slots * ct16 + cc;
+  float mx = kNegInf;
+  for (int s = 0; s < p.splits; ++s) mx = fmaxf(mx, p.part_ml[r0 + (int64_t)s * ct16].x);
+  float sum = 0.0f;
+  f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int s = 0; s < p.splits; ++s) {
+    const int64_t r = r0 + (int64_t)s * ct16;
+    const float2 ml = p.part_ml[r];
+    const float e = ml.x == kNegInf ? 0.0f : q8_ex2(ml.x - mx);
+    sum += ml.y * e;
+    const f32x4 o = *reinterpret_cast<const f32x4*>(p.part_o + r * D + dd);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = fmaf(o[i], e, v[i]);
+  }
+  const float g0 = p.T2 > 0 ? p.gates[0] : 1.0f;
+  v *= sum == 0.0f ? 0.0f : g0 / sum;
+  if (p.T2 > 0) {
+    const int64_t r = r0 + (int64_t)p.splits * ct16;
+    const float inv = p.gates[1] / p.part_ml[r].y;
+    const f32x4 o = *reinterpret_cast<const f32x4*>(p.part_o + r * D + dd);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = fmaf(o[i], inv, v[i]);
+  }
+  const int b = bh / p.Hkv, kvh = bh - b * p.Hkv;
+  const float t[4] = {v[0], v[1], v[2], v[3]};
+  q8_store<4>(p, q8_out_off(p, b, kvh, col) + dd, t);
+}
+
+// The launch shape: column tiles of 16 a wave, column groups, key splits.
+struct Q8Plan {
+  int ct, groups, splits;
+  bool wide;
+};
+
+Q8Plan q8_plan(const vnx_attn_q8_args* a) {
+  const int64_t cols = (int64_t)(a->H / a->Hkv) * a->N, BH = (int64_t)a->B * a->Hkv;
+  const int most = a->d == 64 ? 4 : 2;
+  const int64_t tiles = (cols + 15) / 16;
+  const int cus = device_cus();
+  Q8Plan pl{};
+  pl.ct = most;
+  pl.wide = BH * ((tiles + most - 1) / most) >= 4 * (int64_t)cus;
+  if (pl.wide) {
+    pl.groups = (int)((tiles + 4 * most - 1) / (4 * most));
+    pl.splits = 1;
+    return pl;
+  }
+  pl.groups = (int)((tiles + most - 1) / most);
+  pl.ct = (int)((tiles + pl.groups - 1) / pl.groups);
+  // keys a column group walks: about a workgroup a CU, 128 keys a split at least
+  const int64_t keys = a->window > 0 && a->window < a->Tp + a->N ? (int64_t)a->window + a->N : (int64_t)a->Tp + a->N;
+  const int64_t units = BH * pl.groups;
+  int64_t s = units >= cus ? 1 : (cus + units - 1) / units;
+  s = s < keys / 128 ? s : keys / 128;
+  pl.splits = (int)(s < 1 ? 1 : s > kQ8Split ? kQ8Split : s);
+  return pl;
+}
+
+size_t q8_ws_bytes(const vnx_attn_q8_args* a, const Q8Plan& pl, Q8Params* p, void* ws) {
+  if (pl.splits == 1) return 0;
+  const int slots = pl.splits + (a->T2 > 0);
+  const size_t rows = (size_t)a->B * a->Hkv * pl.groups * slots * 16 * pl.ct;
+  Carve c(ws);
+  float* o = c.take<float>(rows * a->d);
+  float2* ml = c.take<float2>(rows);
+  if (p) {
+    p->part_o = o;
+    p->part_ml = ml;
+    p->slots = slots;
+  }
+  return c.bytes();
+}
+
+// Everything that needs no pointer.
+int q8_check_sizes(const vnx_attn_q8_args* a) {
+  if (a->B < 0 || a->H < 1 || a->Hkv < 1 || a->H % a->Hkv || a->N < 1 || a->Tp < 0 || a->T2 < 0 || a->window < 0)
+    return VNX_ERR_INVALID_ARG;
+  if (a->d != 64 && a->d != 128) return VNX_ERR_UNSUPPORTED;
+  if (a->kv_dtype != VNX_I8 && a->kv_dtype != VNX_E4M3) return VNX_ERR_UNSUPPORTED;
+  if (a->out_dtype != VNX_BF16 && a->out_dtype != VNX_F16) return VNX_ERR_UNSUPPORTED;
+  if ((int64_t)a->Tp + a->N > a->cap) return VNX_ERR_INVALID_ARG;
+  const bool tree = a->anc || a->anc_host;
+  if (tree && (a->N > kQ8MaxN || (a->window > 0 && a->window < a->N))) return VNX_ERR_UNSUPPORTED;
+  // 32-bit row, column and workgroup numbers
+  if (a->cap > INT_MAX - 64 || (int64_t)a->Tp + a->N > INT_MAX - 64 || a->T2 > INT_MAX - 64 ||
+      (int64_t)a->H / a->Hkv * a->N > INT_MAX / 2 ||
+      (int64_t)a->B * a->Hkv * (((int64_t)a->H / a->Hkv * a->N + 15) / 16) * kQ8Split > INT_MAX)
+    return VNX_ERR_UNSUPPORTED;
+  return VNX_OK;
+}
+
+inline bool q8_strides(const int64_t* s, int n, int64_t unit) {
+  for (int i = 0; i < n; ++i)
+    if (s[i] < 0 || s[i] % unit) return false;
+  return true;
+}
+
+template <int D, int KT, int CT>
+void q8_launch(const Q8Params& p, const Q8Words& tw, const Q8Plan& pl, hipStream_t st) {
+  const unsigned bh = (unsigned)(p.B * p.Hkv);
+  if (pl.wide)
+    hipLaunchKernelGGL((k_attn8_wide<D, KT, CT>), dim3(bh * pl.groups), dim3(256), 0, st, p, tw);
+  else
+    hipLaunchKernelGGL((k_attn8_split<D, KT, CT>), dim3(bh * pl.groups * pl.splits), dim3(p.T2 > 0 ? 320 : 256), 0, st,
+                       p, tw);
+}
+
+template <int D, int KT>
+int q8_by_ct(const Q8Params& p, const Q8Words& tw, const Q8Plan& pl, hipStream_t st) {
+  if (pl.ct == 1) q8_launch<D, KT, 1>(p, tw, pl, st);
+  else if (pl.ct == 2) q8_launch<D, KT, 2>(p, tw, pl, st);
+  if constexpr (D == 64) {
+    if (pl.ct == 3) q8_launch<D, KT, 3>(p, tw, pl, st);
+    else if (pl.ct == 4) q8_launch<D, KT, 4>(p, tw, pl, st);
+  }
+  VNX_LAUNCH_CHECK();
+  if (pl.splits > 1) {
+    const int64_t work = (int64_t)p.B * p.Hkv * p.groups * 16 * pl.ct * (D / 4);
+    hipLaunchKernelGGL((k_attn8_join<D>), dim3((unsigned)((work + 255) / 256)), dim3(256), 0, st, p, 16 * pl.ct);
+    VNX_LAUNCH_CHECK();
+  }
+  return VNX_OK;
+}
+
+}  // namespace
+}  // namespace vnx
+
+using namespace vnx;
+
+extern "C" {
+
+size_t vnx_tree_attn_q8_workspace(const vnx_attn_q8_args* a) {
+  if (!a || q8_check_sizes(a) != VNX_OK || a->B == 0) return 256;
+  const size_t n = q8_ws_bytes(a, q8_plan(a), nullptr, nullptr);
+  return n < 256 ? 256 : n;
+}
+
+int vnx_tree_attn_q8(const vnx_attn_q8_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!a) return VNX_ERR_INVALID_ARG;
+  const int bad = q8_check_sizes(a);
+  if (bad != VNX_OK) return bad;
+  if (a->B == 0) return VNX_OK;
+  if (!a->q || !a->k_cache || !a->v_cache || !a->k_scale || !a->v_scale || !a->lens || !a->out)
+    return VNX_ERR_INVALID_ARG;
+  if (!(a->scale > 0.0f) || !__builtin_isfinite(a->scale) || a->anc_batch_stride < 0) return VNX_ERR_INVALID_ARG;
+  if (a->cache_strides[2] < a->d || !q8_strides(a->scale_strides, 2, 1)) return VNX_ERR_INVALID_ARG;
+  if (a->T2 > 0 && (!a->k_seg2 || !a->v_seg2 || !a->gates)) return VNX_ERR_INVALID_ARG;
+  // 16-byte loads; a step's row offsets in 32 bits
+  if (!q8_strides(a->q_strides, 3, 8) || !q8_strides(a->cache_strides, 3, 16) || !q8_strides(a->out_strides, 3, 8) ||
+      (a->T2 > 0 && !q8_strides(a->seg2_strides, 3, 8)) || a->cache_strides[2] >= (1 << 25) ||
+      (a->T2 > 0 && a->seg2_strides[2] >= (1 << 24)))
+    return VNX_ERR_UNSUPPORTED;
+  if (!aligned16(a->q) || !aligned16(a->k_cache) || !aligned16(a->v_cache) || !aligned16(a->out) ||
+      (a->T2 > 0 && (!aligned16(a->k_seg2) || !aligned16(a->v_seg2) || !aligned_to(a->gates, 4))) ||
+      !aligned_to(a->k_scale, 4) || !aligned_to(a->v_scale, 4) || !aligned_to(a->lens, 4) || !aligned_to(a->anc, 8))
+    return VNX_ERR_UNSUPPORTED;
+  const Q8Plan pl = q8_plan(a);
+  Q8Params p{};
+  p.slots = 1;
+  const size_t need = q8_ws_bytes(a, pl, &p, workspace);
+  if (need && (!workspace || workspace_bytes < need)) return VNX_ERR_WORKSPACE;
+  p.q = static_cast<const uint16_t*>(a->q);
+  p.kc = static_cast<const char*>(a->k_cache); p.vc = static_cast<const char*>(a->v_cache);
+  p.ks = a->k_scale; p.vs = a->v_scale;
+  p.lens = a->lens;
+  p.out = a->out;
+  p.q_sb = a->q_strides[0]; p.q_sh = a->q_strides[1]; p.q_sr = a->q_strides[2];
+  p.c_sb = a->cache_strides[0]; p.c_sh = a->cache_strides[1]; p.c_sr = a->cache_strides[2];
+  p.s_sb = a->scale_strides[0]; p.s_sh = a->scale_strides[1];
+  p.o_sb = a->out_strides[0]; p.o_sh = a->out_strides[1]; p.o_sr = a->out_strides[2];
+  p.B = a->B; p.H = a->H; p.Hkv = a->Hkv; p.rep = a->H / a->Hkv; p.N = a->N; p.cols = p.rep * a->N;
+  p.Tp = a->Tp; p.T2 = a->T2; p.window = a->window;
+  if (a->T2 > 0) {
+    p.k2 = static_cast<const char*>(a->k_seg2); p.v2 = static_cast<const char*>(a->v_seg2);
+    p.s2_sb = 2 * a->seg2_strides[0]; p.s2_sh = 2 * a->seg2_strides[1]; p.s2_sr = 2 * a->seg2_strides[2];
+    p.gates = a->gates;
+  }
+  Q8Words tw{};
+  if (a->anc) {
+    p.tree = 2;
+    p.anc = a->anc;
+    p.anc_sb = a->anc_batch_stride;
+  } else if (a->anc_host) {
+    p.tree = 1;
+    for (int i = 0; i < a->N; ++i) tw.w[i] = a->anc_host[i];
+  }
+  p.groups = pl.groups; p.splits = pl.splits;
+  p.f16 = a->out_dtype == VNX_F16;
+  p.c = (float)((double)a->scale * 1.4426950408889634);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (a->d == 64)
+    return a->kv_dtype == VNX_I8 ? q8_by_ct<64, KV_I8>(p, tw, pl, st) : q8_by_ct<64, KV_E4M3>(p, tw, pl, st);
+  return a->kv_dtype == VNX_I8 ? q8_by_ct<128, KV_I8>(p, tw, pl, st) : q8_by_ct<128, KV_E4M3>(p, tw, pl, st);
+}
+
+}  // extern "C"

@@ -671,6 +671,185 @@ class HipBackend(DeviceBackend):
         del keep
         return out
 
+    # ---- the KV cache in 8 bits ---------------------------------------------
+    def _kv_pair(self, a, b, what: str, dtypes):
+        """Checks two tensors of one shape, dtype and strides that live on this
+        device (a cache is read and written where it is: nothing is copied)."""
+        for t in (a, b):
+            if not isinstance(t, torch.Tensor) or t.device != self._torch_device:
+                raise ValueError(f"{what} must be tensors on {self._torch_device}")
+        if a.dtype not in dtypes or a.dtype != b.dtype:
+            raise ValueError(f"{what} must share one of the types {', '.join(str(d) for d in dtypes)}, "
+                             f"got {a.dtype} and {b.dtype}")
+        if a.shape != b.shape or a.stride() != b.stride() or (a.numel() and a.stride(-1) != 1):
+            raise ValueError(f"{what} must share their shape and strides, with unit last stride")
+
+    def _kv_cache(self, k_cache, v_cache, k_scale, v_scale, dtypes):
+        """(B, Hkv, cap, d, dtype code, scale strides) of a cache."""
+        self._kv_pair(k_cache, v_cache, "k_cache and v_cache", dtypes)
+        if k_cache.dim() != 4:
+            raise ValueError(f"the caches must be (B, Hkv, cap, d), got {tuple(k_cache.shape)}")
+        B, Hkv, cap, d = k_cache.shape
+        if k_cache.dtype == torch.bfloat16:
+            if k_scale is not None or v_scale is not None:
+                raise ValueError("a bf16 cache has no scales")
+            return B, Hkv, cap, d, _lib.VNX_BF16, (0, 0)
+        self._kv_pair(k_scale, v_scale, "k_scale and v_scale", (torch.float32,))
+        if k_scale.shape != (B, Hkv, cap):
+            raise ValueError(f"scales must be ({B}, {Hkv}, {cap}), got {tuple(k_scale.shape)}")
+        return B, Hkv, cap, d, _lib.KV_DTYPE_CODES[k_cache.dtype], k_scale.stride()[:2]
+
+    def _kv_lens(self, lens, B: int, what: str = "lens") -> torch.Tensor:
+        t = _to_tensor(lens, self._torch_device, torch.int32)
+        if t.dim() != 1 or t.numel() != B:
+            raise ValueError(f"{what} must have {B} entries")
+        return t.contiguous()
+
+    def _kv_vec(self, t, shape, what: str):
+        """A contiguous fp32 tensor of `shape` on 16 bytes, or None."""
+        if t is None:
+            return None
+        t = _to_tensor(t, self._torch_device, torch.float32)
+        if t.dim() != len(shape) or any(n is not None and t.shape[i] != n for i, n in enumerate(shape)):
+            raise ValueError(f"{what} must be {tuple('rows' if n is None else n for n in shape)}, got {tuple(t.shape)}")
+        t = t.contiguous()
+        return t.clone() if t.data_ptr() % 16 else t
+
+    _KV_DTYPES = (torch.int8, torch.float8_e4m3fn, torch.bfloat16)
+
+    def kv_write(self, qkv, k_cache, v_cache, lens, k_scale=None, v_scale=None, cos=None, sin=None, q_norm=None,
+                 k_norm=None, eps: float = 1e-6) -> torch.Tensor:
+        """Writes the new rows of a projection into the cache (vnx_kv_write)
+        and returns the queries (B, H, n, d) bf16.
+
+        qkv (B, n, (H + 2 Hkv) d) fp32, bf16 or fp16: H query, Hkv key and Hkv
+        value heads a row, row (b, i) at position lens[b] + i.  k_cache /
+        v_cache (B, Hkv, cap, d) int8, float8_e4m3fn (with k_scale / v_scale
+        (B, Hkv, cap) fp32) or bfloat16, written in place.  cos / sin (rows, d)
+        rotate queries and keys; q_norm / k_norm (d,) norm every query / key
+        head before that.  Positions outside the cache (or the tables) are
+        skipped and their queries zero."""
+        B, Hkv, cap, d, code, ss = self._kv_cache(k_cache, v_cache, k_scale, v_scale, self._KV_DTYPES)
+        x = _to_tensor(qkv, self._torch_device).resolve_neg()
+        if x.dtype not in _lib.DTYPE_CODES:
+            raise ValueError(f"qkv must be float32, bfloat16 or float16, got {x.dtype}")
+        if x.dim() != 3 or x.shape[0] != B or x.shape[2] % d or x.shape[2] // d <= 2 * Hkv or x.shape[1] < 1:
+            raise ValueError(f"qkv must be ({B}, n, (H + {2 * Hkv}) * {d}), got {tuple(x.shape)}")
+        n, H = x.shape[1], x.shape[2] // d - 2 * Hkv
+        s0, ldq, s2 = x.stride()
+        if (s2 != 1 or (B > 1 and s0 != n * ldq) or ldq < x.shape[2] or ldq * x.element_size() % 16
+                or x.data_ptr() % 16):
+            x = x.clone(memory_format=torch.contiguous_format)
+            ldq = x.shape[2]
+        if (cos is None) != (sin is None):
+            raise ValueError("pass both cos and sin, or neither")
+        ct = self._kv_vec(cos, (None, d), "cos")
+        st = self._kv_vec(sin, (None, d), "sin")
+        if ct is not None and ct.shape != st.shape:
+            raise ValueError("cos and sin must have the same rows")
+        qn, kn = self._kv_vec(q_norm, (d,), "q_norm"), self._kv_vec(k_norm, (d,), "k_norm")
+        ln = self._kv_lens(lens, B)
+        q = torch.empty((B, H, n, d), dtype=torch.bfloat16, device=self._torch_device)
+        _lib.check(self._L.vnx_kv_write(_lib.pack_kv_write(
+            x.data_ptr(), ldq, ln.data_ptr(), _ptr(ct) or 0, _ptr(st) or 0, ct.shape[0] if ct is not None else 0,
+            _ptr(qn) or 0, _ptr(kn) or 0, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_scale) or 0,
+            _ptr(v_scale) or 0, *k_cache.stride()[:3], *ss, B, cap, n, H, Hkv, d, _lib.DTYPE_CODES[x.dtype], code,
+            float(eps)), self._stream()), "kv_write")
+        return q
+
+    def kv_read(self, k_cache, v_cache, k_scale=None, v_scale=None, start=None, rows: int | None = None,
+                out_dtype=torch.bfloat16):
+        """(k, v), each (B, Hkv, rows, d) in out_dtype (float32, bfloat16 or
+        float16): what rows start[b] .. start[b] + rows - 1 of a cache as
+        kv_write fills it stand for (vnx_kv_read); start None: from row 0,
+        rows None: cap of them.  Rows outside the cache are zeros."""
+        B, Hkv, cap, d, code, ss = self._kv_cache(k_cache, v_cache, k_scale, v_scale, self._KV_DTYPES)
+        if out_dtype not in _lib.DTYPE_CODES:
+            raise ValueError("out_dtype must be torch.float32, torch.bfloat16 or torch.float16")
+        rows = cap if rows is None else int(rows)
+        if rows < 0:
+            raise ValueError(f"rows must be >= 0, got {rows}")
+        st = None if start is None else self._kv_lens(start, B, "start")
+        k = torch.empty((B, Hkv, rows, d), dtype=out_dtype, device=self._torch_device)
+        v = torch.empty_like(k)
+        _lib.check(self._L.vnx_kv_read(_lib.pack_kv_read(
+            k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_scale) or 0, _ptr(v_scale) or 0, _ptr(st) or 0,
+            k.data_ptr(), v.data_ptr(), *k_cache.stride()[:3], *ss, Hkv * rows * d, rows * d, d, B, cap, rows, Hkv, d,
+            code, _lib.DTYPE_CODES[out_dtype]), self._stream()), "kv_read")
+        return k, v
+
+    def tree_attention_q8(self, q, k_cache, v_cache, k_scale, v_scale, lens, anc=None, scale: float | None = None,
+                          seg2=None, gates=None, window: int = 0, max_len: int | None = None,
+                          out_dtype=torch.bfloat16, out=None) -> torch.Tensor:
+        """Attention of N new rows of every sequence over its 8-bit cache
+        (vnx_tree_attn_q8), the new rows already written at rows lens[b] ..
+        lens[b] + N - 1 (kv_write).
+
+        q (B, H, N, d), read as bf16; lens (B,) int32; anc None: a chain of any
+        N (one token, drafts, a prompt); or (N,) / (B, N) ancestor words
+        (tree.ancestor_words) of a token tree of at most 64 nodes.  window,
+        seg2 and gates as in tree_attention (no ALiBi).  max_len: a bound of
+        lens known to the caller (cap - N by default; longer lens are cut to
+        it), from which the launch is sized.  Returns (B, H, N, d) bfloat16 or
+        float16, written into `out` (any strides with unit last stride) when
+        given."""
+        dev = self._torch_device
+        B, Hkv, cap, d, code, ss = self._kv_cache(k_cache, v_cache, k_scale, v_scale, self._KV_DTYPES[:2])
+        qt = self._heads_bf16(q, "q")
+        H, N = qt.shape[1], qt.shape[2]
+        if qt.shape[0] != B or qt.shape[3] != d or H % Hkv or N < 1:
+            raise ValueError(f"q {tuple(qt.shape)} does not match the cache {tuple(k_cache.shape)}")
+        Tp = cap - N if max_len is None else int(max_len)
+        if Tp < 0 or Tp + N > cap:
+            raise ValueError(f"{N} new rows after up to {Tp} do not fit a cache of {cap}")
+        ln = self._kv_lens(lens, B)
+        a = anc_t = None
+        if anc is not None:
+            if isinstance(anc, torch.Tensor) and anc.device == dev and anc.dtype == torch.int64:
+                a = anc_t = anc.contiguous()
+            else:
+                a = anc.detach().cpu().numpy() if isinstance(anc, torch.Tensor) else np.asarray(anc)
+                a = np.ascontiguousarray(a.astype(np.uint64) if a.dtype != np.uint64 else a)
+                if a.ndim == 2:
+                    anc_t = torch.from_numpy(a.view(np.int64)).to(dev)
+            if tuple(a.shape) not in ((N,), (B, N)):
+                raise ValueError(f"anc must be ({N},) or ({B}, {N}), got {tuple(a.shape)}")
+        if out is None:
+            if out_dtype not in (torch.bfloat16, torch.float16):
+                raise ValueError("out_dtype must be torch.bfloat16 or torch.float16")
+            out = torch.empty((B, H, N, d), dtype=out_dtype, device=dev)
+        elif tuple(out.shape) != (B, H, N, d) or out.stride(-1) != 1 or out.device != dev \
+                or out.dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError(f"out must be a ({B}, {H}, {N}, {d}) bfloat16 or float16 tensor with unit last stride")
+        k2 = v2 = g = None
+        s2 = (0, 0, 0)
+        if seg2 is not None:
+            k2, v2 = self._heads_bf16(seg2[0], "k_seg2"), self._heads_bf16(seg2[1], "v_seg2")
+            if (k2.shape != v2.shape or k2.shape[0] not in (1, B) or k2.shape[1] != Hkv or k2.shape[2] < 1
+                    or k2.shape[3] != d):
+                raise ValueError(f"second segment {tuple(k2.shape)} / {tuple(v2.shape)} does not match")
+            if k2.stride() != v2.stride():
+                k2, v2 = k2.contiguous(), v2.contiguous()
+            if gates is None:
+                raise ValueError("a second segment needs the two gates")
+            g = _to_tensor(gates, dev, torch.float32).reshape(-1).contiguous()
+            if g.numel() < 2:
+                raise ValueError("gates must hold two values")
+            s2 = (0 if k2.shape[0] == 1 else k2.stride(0), k2.stride(1), k2.stride(2))
+        args = _lib.pack_attn_q8(
+            qt.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+            ln.data_ptr(), _ptr(anc_t) or 0, a.ctypes.data if a is not None and anc_t is None else 0, out.data_ptr(),
+            _ptr(k2) or 0, _ptr(v2) or 0, _ptr(g) or 0, *qt.stride()[:3], *k_cache.stride()[:3], *ss,
+            *out.stride()[:3], *s2, N if a is not None and a.ndim == 2 else 0, cap, B, H, Hkv, Tp, N, d,
+            k2.shape[2] if k2 is not None else 0, int(window), code, _lib.DTYPE_CODES[out.dtype],
+            float(scale) if scale is not None else d ** -0.5)
+        # a workspace of this call's own: a captured graph keeps it in its pool
+        need = self._L.vnx_tree_attn_q8_workspace(args)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 256 else None
+        _lib.check(self._L.vnx_tree_attn_q8(args, _ptr(ws), need if ws is not None else 0, self._stream()),
+                   "tree_attention_q8")
+        return out
+
     def attention(self, q, k, v, mask=None):
         """DeviceBackend.attention (device.py:260-270; TorchBackend's SDPA call,
         backend_torch.py:356-379).  bf16 (B, H, Nq, d) queries over (B, Hkv, T, d)
