@@ -5,9 +5,10 @@
 //   O_i = sum_j P_ij sv_j vc_j           (kc, vc codes; sk, sv their scales)
 //   out_i = g0 * O_i + g1 * (the same over the second segment, bf16 rows)
 //
-// A code is exact in bf16 (8 significant bits), so both products run on
-// v_mfma_f32_16x16x32_bf16 with the codes as operands and the scales applied
-// to scores and probabilities, one multiply each.
+// A code is exact in bf16 and in fp16 (8 significant bits), so the products run
+// on v_mfma_f32_16x16x32_bf16 (the scores, with the bf16 queries) and _f16 (the
+// values) with the codes as operands and the scales applied to scores and
+// probabilities, one multiply each.
 //
 // A wave owns 16 CT query columns of one KV head (column c is node c / rep of
 // query head kvh * rep + c % rep, so heads that share K and V share every
@@ -21,9 +22,8 @@
 //                    The 8 keys are those of its own 8 scores, so P goes from
 //                    the score registers into the B operand as it is.
 // A step's rows are loaded into registers under the previous step's math.
-// Statistics and sums are fp32; P * sv is rounded once to bf16 (at most 2^-8
-// of each term, as much as the rounding of a bf16 output, and independent from
-// key to key).
+// Statistics and sums are fp32; P * sv is rounded once to fp16 (2^-11 of each
+// term; see q8_walk for its range).
 // The running maximum of a column moves only when a score passes it by 2^8:
 // until then P stays below 2^8 in fp32 sums and bf16 operands, and the step
 // needs no exchange between lanes and no rescaling.
@@ -35,7 +35,7 @@ namespace vnx {
 namespace {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kQ8MaxN = 64;      // nodes of a tree: bits of an ancestor word
 constexpr int kQ8Split = 32;     // key splits of a launch at most
@@ -100,67 +100,51 @@ struct Q8Src {
   int rows;      // rows that may be read
 };
 
-// The loaded rows of one step of 32 keys.
-template <int D, int KT>
-struct Q8Rows {
-  static constexpr int E = KT == KV_BF16 ? 2 : 1;
-  static constexpr int KW = D / 64 * E;     // 16-byte loads a key tile
-  static constexpr int VW = D / 64 * E;     // words of a key's V a lane
-  u32x4 k[2][KW];
-  uint32_t v[8][VW];
-  f32x4 sk[2], sv[2];
+// A buffer of the `left` rows (at most 32) from p on: what lies behind them
+// reads as zeros, dword by dword, so a step needs no test of its last rows and
+// a step behind the end (left <= 0) moves no data.
+template <int BYTES>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t q8_buffer(const void* p, uint32_t pitch, int left) {
+  const int n = min(left, 32);
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, n > 0 ? (n - 1) * (int)pitch + BYTES : 0, 0x00027000);
+}
 
-  // Rows past the last one are read as the last one (their scores are masked).
-  template <bool TAIL>
-  __device__ __forceinline__ void load(const Q8Src& s, int k0, int lane) {
+// fp32 to an fp16 pair, nearest even.
+__device__ __forceinline__ uint32_t q8_pk_f16(float a, float b) {
+  return __builtin_bit_cast(uint32_t, f16x2{(_Float16)a, (_Float16)b});
+}
+
+// The scales of this lane's 8 keys.
+__device__ __forceinline__ void q8_scales(const float* s, int k0, int left, int g, f32x4 (&o)[2]) {
+  const auto rs = q8_buffer<4>(s + k0, 4, left);
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+    o[t] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, 16 * g, 64 * t, 0));
+}
+
+// The loaded rows of one step of 32 keys from k0 on, `left` of them to be read.
+template <int D, int KT>
+struct Q8Keys {
+  static constexpr int E = KT == KV_BF16 ? 2 : 1;
+  static constexpr int W = D / 64 * E;  // 16-byte loads a key tile
+  u32x4 k[2][W];
+  f32x4 sk[2];
+
+  __device__ __forceinline__ void load(const Q8Src& s, int k0, int left, int lane) {
     const int m = lane & 15, g = lane >> 4;
-    const int last = s.rows - 1 - k0;
-    const char* kb = s.k + (int64_t)k0 * s.sr;
-    const char* vb = s.v + (int64_t)k0 * s.sr;
+    const auto rs = q8_buffer<D * E>(s.k + (int64_t)k0 * s.sr, s.sr, left);
+    const int o = m * (int)s.sr + g * (16 * E);
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int r = TAIL ? min(16 * t + m, last) : 16 * t + m;
-      const uint32_t o = (uint32_t)r * s.sr + (uint32_t)g * (16 * E);
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int i = 0; i < KW; ++i)
-        k[t][i] = *reinterpret_cast<const u32x4*>(kb + (o + (uint32_t)(E == 1 ? 64 * i : 128 * (i / 2) + 16 * (i % 2))));
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int rr = (j < 4 ? 0 : 16) + 4 * g + (j & 3);
-      const int r = TAIL ? min(rr, last) : rr;
-      const uint32_t o = (uint32_t)r * s.sr + (uint32_t)m * (D / 16 * E);
-      if constexpr (VW == 1) {
-        v[j][0] = *reinterpret_cast<const uint32_t*>(vb + o);
-      } else if constexpr (VW == 2) {
-        const uint2 w = *reinterpret_cast<const uint2*>(vb + o);
-        v[j][0] = w.x; v[j][1] = w.y;
-      } else {
-        const u32x4 w = *reinterpret_cast<const u32x4*>(vb + o);
-        v[j][0] = w[0]; v[j][1] = w[1]; v[j][2] = w[2]; v[j][3] = w[3];
-      }
-    }
-    if constexpr (KT != KV_BF16) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int r = 16 * t + 4 * g;
-        if constexpr (TAIL) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int rc = k0 + min(r + i, last);
-            sk[t][i] = s.ks[rc];
-            sv[t][i] = s.vs[rc];
-          }
-        } else {
-          sk[t] = *reinterpret_cast<const f32x4u*>(s.ks + k0 + r);
-          sv[t] = *reinterpret_cast<const f32x4u*>(s.vs + k0 + r);
-        }
-      }
-    }
+      for (int i = 0; i < W; ++i)
+        k[t][i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+            rs, o + (E == 1 ? 64 * i : 128 * (i / 2) + 16 * (i % 2)), 16 * t * (int)s.sr, 0));
+    if constexpr (KT != KV_BF16) q8_scales(s.ks, k0, left, g, sk);
   }
 
-  // K operands of key tile t.
-  __device__ __forceinline__ void kfrag(int t, bf16x8 (&f)[D / 32]) const {
+  // Operands of key tile t.
+  __device__ __forceinline__ void frag(int t, bf16x8 (&f)[D / 32]) const {
 #pragma unroll
     for (int s = 0; s < D / 32; ++s) {
       u32x4 w;
@@ -185,33 +169,61 @@ struct Q8Rows {
       f[s] = __builtin_bit_cast(bf16x8, w);
     }
   }
+};
 
-  // V^T operands: dim tile t, keys j of this lane.
-  __device__ __forceinline__ void vfrag(bf16x8 (&f)[D / 16]) const {
+template <int D, int KT>
+struct Q8Vals {
+  static constexpr int E = KT == KV_BF16 ? 2 : 1;
+  static constexpr int W = D / 64 * E;  // words of a key's values a lane
+  uint32_t v[8][W];
+  f32x4 sv[2];
+
+  __device__ __forceinline__ void load(const Q8Src& s, int k0, int left, int lane) {
+    const int m = lane & 15, g = lane >> 4;
+    const auto rs = q8_buffer<D * E>(s.v + (int64_t)k0 * s.sr, s.sr, left);
+    const int o = 4 * g * (int)s.sr + m * (D / 16 * E);
 #pragma unroll
-    for (int x = 0; x < VW; ++x) {
-      constexpr int PW = KT == KV_BF16 ? 2 : 4;  // dims of a word
-      uint32_t w[PW][4];
+    for (int j = 0; j < 8; ++j) {
+      const int so = ((j < 4 ? 0 : 16) + (j & 3)) * (int)s.sr;
+      if constexpr (W == 1) {
+        v[j][0] = __builtin_amdgcn_raw_buffer_load_b32(rs, o, so, 0);
+      } else if constexpr (W == 2) {
+        const auto w = __builtin_amdgcn_raw_buffer_load_b64(rs, o, so, 0);
+        v[j][0] = w[0]; v[j][1] = w[1];
+      } else {
+        const auto w = __builtin_amdgcn_raw_buffer_load_b128(rs, o, so, 0);
+        v[j][0] = w[0]; v[j][1] = w[1]; v[j][2] = w[2]; v[j][3] = w[3];
+      }
+    }
+    if constexpr (KT != KV_BF16) q8_scales(s.vs, k0, left, g, sv);
+  }
+
+  // Operands of dim tiles 4 x .. (codes; 2 x .. of bf16 rows) from word x: the
+  // 8 keys of this lane, fp16 (codes) or bf16 pairs.
+  __device__ __forceinline__ void frag(u32x4 (&f)[D / 16]) const {
+#pragma unroll
+    for (int x = 0; x < W; ++x) {
       if constexpr (KT == KV_BF16) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          w[0][j] = __builtin_amdgcn_perm(v[2 * j + 1][x], v[2 * j][x], 0x05040100u);
-          w[1][j] = __builtin_amdgcn_perm(v[2 * j + 1][x], v[2 * j][x], 0x07060302u);
+          f[2 * x][j] = __builtin_amdgcn_perm(v[2 * j + 1][x], v[2 * j][x], 0x05040100u);
+          f[2 * x + 1][j] = __builtin_amdgcn_perm(v[2 * j + 1][x], v[2 * j][x], 0x07060302u);
         }
       } else if constexpr (KT == KV_E4M3) {
-        uint32_t c[8][2];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          c[j][0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[j][x], 1.0f, false));
-          c[j][1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[j][x], 1.0f, true));
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < 4; ++j) {
+          uint32_t c[2][2];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            w[2 * h][j] = __builtin_amdgcn_perm(c[2 * j + 1][h], c[2 * j][h], 0x05040100u);
-            w[2 * h + 1][j] = __builtin_amdgcn_perm(c[2 * j + 1][h], c[2 * j][h], 0x07060302u);
+            c[h][0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v[2 * j + h][x], 1.0f, false));
+            c[h][1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v[2 * j + h][x], 1.0f, true));
           }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            f[4 * x + 2 * h][j] = __builtin_amdgcn_perm(c[1][h], c[0][h], 0x05040100u);
+            f[4 * x + 2 * h + 1][j] = __builtin_amdgcn_perm(c[1][h], c[0][h], 0x07060302u);
+          }
+        }
       } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -219,121 +231,232 @@ struct Q8Rows {
           kv_f32x4<KV_I8>(v[2 * j][x], a);
           kv_f32x4<KV_I8>(v[2 * j + 1][x], b);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) w[i][j] = kv_pk_bf16(a[i], b[i]);
+          for (int i = 0; i < 4; ++i)  // (exact: the rounding mode does not matter)
+            f[4 * x + i][j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a[i], b[i]));
         }
       }
-#pragma unroll
-      for (int i = 0; i < PW; ++i) f[PW * x + i] = __builtin_bit_cast(bf16x8, u32x4{w[i][0], w[i][1], w[i][2], w[i][3]});
     }
   }
 };
 
-// What the columns of a wave see: keys [lo, hi) of its own, of which keys from
-// tp on only where the word has their bit (trees).  Keys [full_lo, full_hi)
-// are seen by every column.
+// What the columns of a wave see.  Keys [full_lo, full_hi) are seen by every
+// column; elsewhere column ct of node[ct] sees key j when
+//   Q8_CHAIN  j <= tp + node and j > tp + node - window;
+//   Q8_TREE   j < tp + N, j > its position - window, and from tp on its word has
+//             the bit (words read where they are needed: few steps do);
+//   Q8_ALL    j < rows (the second segment).
+enum { Q8_CHAIN = 0, Q8_TREE = 1, Q8_ALL = 2 };
 template <int CT>
 struct Q8Mask {
-  int lo[CT], hi[CT];
-  uint64_t word[CT];
-  int tp, full_lo, full_hi;
-  bool tree;
+  int node[CT];
+  int tp, window, rows, full_lo, full_hi;
+  const uint64_t* words;
 };
+
+// Bit e set: key k0 + 16 (e / 4) + g4 + e % 4 is hidden from the column.
+template <int KIND>
+__device__ __forceinline__ uint32_t q8_hidden(int tp, int window, int rows, const uint64_t* words, int node, int k0,
+                                              int g4) {
+  int lo, hi;
+  uint64_t w = 0;
+  if constexpr (KIND == Q8_ALL) {
+    lo = 0;
+    hi = rows;
+  } else if constexpr (KIND == Q8_CHAIN) {
+    lo = tp + node - window + 1;
+    hi = tp + node + 1;
+  } else {
+    w = words[node];
+    lo = tp + __popcll(w) - window;
+    hi = rows;
+  }
+  uint32_t hide = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int key = k0 + 16 * (e / 4) + g4 + e % 4;
+    uint32_t no = (uint32_t)(key < lo) | (uint32_t)(key >= hi);
+    if constexpr (KIND == Q8_TREE) {
+      const int j = key - tp;  // (>= 64 only from hi on)
+      no |= (uint32_t)(j >= 0) & ~(uint32_t)(w >> (j & 63));
+    }
+    hide |= (no & 1u) << e;
+  }
+  return hide;
+}
 
 enum { Q8_SOFTMAX = 0, Q8_STATS = 1, Q8_FIXED = 2 };
 
-// Walks steps s0, s0 + ds, .. < s1 of 32 keys from key `first` on.
-//   Q8_SOFTMAX  online softmax: acc, m (the columns' maxima, the same in the
-//               four lanes of a column), l (this lane's share of the sums)
-//   Q8_STATS    m and l alone
-//   Q8_FIXED    acc += (exp2(x - m) * l) sv v: given maxima, l a weight
-template <int D, int KT, int CT, int MODE>
-__device__ __forceinline__ void q8_walk(const Q8Src& src, int first, int s0, int ds, int s1, const Q8Mask<CT>& mk,
-                                        float c, const bf16x8 (&qf)[CT][D / 32], f32x4 (&acc)[CT][D / 16],
-                                        float (&m)[CT], float (&l)[CT], int lane) {
-  if (s0 >= s1) return;
-  const int g4 = (lane >> 4) * 4;
-  Q8Rows<D, KT> rows;
-  auto fetch = [&](int s) {
-    const int k0 = first + 32 * s;
-    if (k0 + 32 <= src.rows) rows.template load<false>(src, k0, lane);
-    else rows.template load<true>(src, k0, lane);
-  };
-  fetch(s0);
-  for (int s = s0; s < s1; s += ds) {
-    const int k0 = first + 32 * s;
-    bf16x8 kf[2][D / 32], vf[D / 16];
-    rows.kfrag(0, kf[0]);
-    rows.kfrag(1, kf[1]);
-    if constexpr (MODE != Q8_STATS) rows.vfrag(vf);
-    float fk[8], sv[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      fk[e] = KT == KV_BF16 ? c : rows.sk[e / 4][e % 4] * c;
-      sv[e] = KT == KV_BF16 ? 1.0f : rows.sv[e / 4][e % 4];
-    }
-    if (s + ds < s1) fetch(s + ds);
-    const bool full = k0 >= mk.full_lo && k0 + 32 <= mk.full_hi;
+template <int CT, int D>
+struct Q8State {
+  f32x4 acc[CT][D / 16];
+  float m[CT];    // the columns' maxima, the same in the four lanes of a column; 0 before the first key
+  float lim[CT];  // what a score may pass m by: -inf before the first key, then kQ8Jump
+  float l[CT];    // this lane's share of the sums
+  __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-      float x[8];
+      m[ct] = 0.0f;
+      lim[ct] = kNegInf;
+      l[ct] = 0.0f;
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) acc[ct][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+  }
+  __device__ __forceinline__ void scale(float f) {
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) acc[ct][d] *= f;
+  }
+};
+
+// Walks steps s0, s0 + ds, .. < s1 of 32 keys from key `first` on.
+//   Q8_SOFTMAX  online softmax into st
+//   Q8_STATS    m and l alone
+//   Q8_FIXED    acc += (exp2(x - m) * l) sv v: given maxima, l a weight
+// Codes: P sv / R in fp16 (2^-11), R the largest sv so far times 2^-6: P <= 2^8
+// and sv / R <= 2^7 stay in range, and a term keeps its 11 bits down to 2^-21 of
+// the largest row's scale (below: 2^-32 of it).  bf16 rows: P in two bf16 parts.
+template <int D, int KT, int CT, int MODE, int KIND>
+__device__ __forceinline__ void q8_walk(const Q8Src& src, int first, int s0, int ds, int s1, const Q8Mask<CT>& mk,
+                                        float c, const bf16x8 (&qf)[CT][D / 32], Q8State<CT, D>& st, int lane) {
+  if (s0 >= s1) return;
+  const int g4 = (lane >> 4) * 4;
+  Q8Keys<D, KT> keys;
+  Q8Vals<D, KT> vals;
+  auto left = [&](int s) { return s < s1 ? src.rows - (first + 32 * s) : 0; };
+  // All scores before the values where they take fewer registers than the key
+  // operands that they replace.
+  constexpr bool EARLY = CT * 8 <= D / 4;
+  float R = 0.0f, iR = __builtin_inff();
+  keys.load(src, first + 32 * s0, left(s0), lane);
+  if constexpr (MODE != Q8_STATS) vals.load(src, first + 32 * s0, left(s0), lane);
+  for (int s = s0; s < s1; s += ds) {
+    const int k0 = first + 32 * s;
+    bf16x8 kf[2][D / 32];
+    keys.frag(0, kf[0]);
+    keys.frag(1, kf[1]);
+    float fk[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) fk[e] = KT == KV_BF16 ? c : keys.sk[e / 4][e % 4] * c;
+    keys.load(src, k0 + 32 * ds, left(s + ds), lane);
+    float x[EARLY ? CT : 1][8];
+    // scores relative to the maxima, in the exp2 domain
+    auto scores = [&](int ct, float (&y)[8]) {
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         f32x4 a = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[t][i], qf[ct][i], a, 0, 0, 0);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[4 * t + i] = a[i] * fk[4 * t + i];
+        for (int i = 0; i < 4; ++i) y[4 * t + i] = fmaf(a[i], fk[4 * t + i], -st.m[ct]);
       }
-      uint32_t hide = 0;
-      if (!full) {
+    };
+    if constexpr (EARLY) {
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) scores(ct, x[ct]);
+    }
+    u32x4 vf[D / 16];
+    float sv[8];
+    if constexpr (MODE != Q8_STATS) {
+      vals.frag(vf);
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) asm volatile("" : "+v"(vf[d]));  // converted here: the rows' registers are free
+      if constexpr (KT != KV_BF16) {
+        float top = 0.0f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const int key = k0 + 16 * (e / 4) + g4 + e % 4;
-          bool see = key >= mk.lo[ct] && key < mk.hi[ct];
-          if (mk.tree && key >= mk.tp) see = see && ((mk.word[ct] >> ((key - mk.tp) & 63)) & 1);
-          if (!see) {
-            x[e] = kNegInf;
-            hide |= 1u << e;
-          }
+          sv[e] = vals.sv[e / 4][e % 4];
+          top = fmaxf(top, fabsf(sv[e]));  // (NaN is passed over)
         }
+        if (__any(!(top * iR <= 128.0f))) {
+          top = 0x1p-110f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float a = fabsf(sv[e]);
+            top = fmaxf(top, a < __builtin_inff() ? a : 0.0f);
+          }
+          top = fmaxf(q8_max4(top) * 0x1p-6f, R);
+          iR = 1.0f / top;
+          if constexpr (MODE == Q8_SOFTMAX) st.scale(R * iR);
+          R = top;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sv[e] *= iR;
       }
+      vals.load(src, k0 + 32 * ds, left(s + ds), lane);
+    }
+    const bool full = k0 >= mk.full_lo && k0 + 32 <= mk.full_hi;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      float(&xx)[8] = x[EARLY ? ct : 0];
+      if constexpr (!EARLY) scores(ct, xx);
+      uint32_t hide = 0;
+      if (!full) {
+        hide = q8_hidden<KIND>(mk.tp, mk.window, mk.rows, mk.words, mk.node[ct], k0, g4);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) xx[e] = hide & (1u << e) ? kNegInf : xx[e];
+      }
+      float& l = st.l[ct];
       if constexpr (MODE != Q8_FIXED) {
-        float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-        if (__any(top > m[ct] + kQ8Jump)) {
-          const float mn = fmaxf(m[ct], q8_max4(top));
-          const float al = mn == kNegInf ? 1.0f : q8_ex2(m[ct] - mn);
-          m[ct] = mn;
-          l[ct] *= al;
+        float top = xx[0];
+#pragma unroll
+        for (int e = 1; e < 8; ++e) top = fmaxf(top, xx[e]);
+        if (__any(top > st.lim[ct])) {
+          const bool none = st.lim[ct] == kNegInf;
+          top = q8_max4(top);
+          const float up = top > (none ? kNegInf : 0.0f) ? top : 0.0f;
+          const float al = none ? 0.0f : q8_ex2(-up);
+          st.m[ct] += up;
+          if (top > kNegInf) st.lim[ct] = kQ8Jump;
+          l *= al;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) xx[e] -= up;
           if constexpr (MODE == Q8_SOFTMAX) {
 #pragma unroll
-            for (int d = 0; d < D / 16; ++d) acc[ct][d] *= al;
+            for (int d = 0; d < D / 16; ++d) st.acc[ct][d] *= al;
           }
         }
       }
-      const float mu = m[ct] == kNegInf ? 0.0f : m[ct];
-      float pv[8];
+      float p[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        float pe = q8_ex2(x[e] - mu);
-        if constexpr (MODE == Q8_FIXED) pe *= l[ct];
-        else l[ct] += pe;
-        pv[e] = pe * sv[e];
+        p[e] = q8_ex2(xx[e]);
+        if constexpr (MODE == Q8_FIXED) p[e] *= l;
+        else l += p[e];
       }
       if constexpr (MODE != Q8_STATS) {
-        if (!full) {  // a hidden row's scale may be NaN: nothing of it is kept
+        if constexpr (KT != KV_BF16) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (hide & (1u << e)) pv[e] = 0.0f;
+          for (int e = 0; e < 8; ++e) p[e] *= sv[e];
+          if (!full) {  // a hidden row's scale may be NaN: nothing of it is kept
+#pragma unroll
+            for (int e = 0; e < 8; ++e) p[e] = hide & (1u << e) ? 0.0f : p[e];
+          }
+          const u32x4 w = {q8_pk_f16(p[0], p[1]), q8_pk_f16(p[2], p[3]), q8_pk_f16(p[4], p[5]), q8_pk_f16(p[6], p[7])};
+#pragma unroll
+          for (int d = 0; d < D / 16; ++d)
+            st.acc[ct][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, vf[d]),
+                                                                  __builtin_bit_cast(f16x8, w), st.acc[ct][d], 0, 0, 0);
+        } else {
+          u32x4 hi, lo;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t h = kv_pk_bf16(p[2 * e], p[2 * e + 1]);
+            hi[e] = h;
+            lo[e] = kv_pk_bf16(p[2 * e] - __uint_as_float(h << 16), p[2 * e + 1] - __uint_as_float(h & 0xFFFF0000u));
+          }
+#pragma unroll
+          for (int d = 0; d < D / 16; ++d) {
+            const bf16x8 v = __builtin_bit_cast(bf16x8, vf[d]);
+            st.acc[ct][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, __builtin_bit_cast(bf16x8, hi), st.acc[ct][d], 0, 0, 0);
+            st.acc[ct][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, __builtin_bit_cast(bf16x8, lo), st.acc[ct][d], 0, 0, 0);
+          }
         }
-        const u32x4 w = {kv_pk_bf16(pv[0], pv[1]), kv_pk_bf16(pv[2], pv[3]), kv_pk_bf16(pv[4], pv[5]),
-                         kv_pk_bf16(pv[6], pv[7])};
-        const bf16x8 pf = __builtin_bit_cast(bf16x8, w);
-#pragma unroll
-        for (int d = 0; d < D / 16; ++d)
-          acc[ct][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[d], pf, acc[ct][d], 0, 0, 0);
       }
     }
   }
+  if constexpr (KT != KV_BF16 && MODE == Q8_SOFTMAX) st.scale(R);
 }
 
 // A column's node and query head.
@@ -359,10 +482,12 @@ struct Q8Tile {
     col0 = c0;
     tp = uni(min(max(p.lens[b], 0), p.Tp));
     const int n0 = c0 / p.rep, n1 = min((c0 + 16 * CT - 1) / p.rep, p.N - 1);
-    const int W = p.window > 0 ? p.window : INT_MAX;
-    mask.tp = tp;
-    mask.tree = p.tree != 0;
+    const int W = p.window > 0 ? p.window : INT_MAX / 2;  // (sums with positions stay in range)
     const int rows = tp + p.N;
+    mask.tp = tp;
+    mask.rows = rows;
+    mask.window = W;
+    mask.words = p.tree == 2 ? p.anc + b * p.anc_sb : tw.w;
     int lo_min, hi_max;
     if (p.tree) {
       lo_min = p.window > 0 ? max(0, tp - 1 - W + 1) : 0;             // an empty word sits at tp - 1
@@ -386,16 +511,7 @@ struct Q8Tile {
 #pragma unroll
       for (int i = 0; i < D / 32; ++i)
         qf[ct][i] = *reinterpret_cast<const bf16x8*>(q + 64 * (i / 2) + 16 * g + 8 * (i % 2));
-      int pos = tp + node;
-      mask.word[ct] = 0;
-      mask.hi[ct] = pos + 1;
-      if (p.tree) {
-        const uint64_t w = p.tree == 1 ? tw.w[node] : p.anc[b * p.anc_sb + node];
-        mask.word[ct] = w;
-        mask.hi[ct] = rows;
-        pos = tp + __popcll(w) - 1;
-      }
-      mask.lo[ct] = p.window > 0 ? pos - W + 1 : 0;
+      mask.node[ct] = node;
     }
     const int64_t kv = b * p.c_sb + kvh * p.c_sh, ss = b * p.s_sb + kvh * p.s_sh;
     src.k = p.kc + kv;
@@ -415,8 +531,10 @@ struct Q8Tile {
   __device__ __forceinline__ Q8Mask<CT> mask2(int T2) const {
     Q8Mask<CT> k;
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) { k.lo[ct] = 0; k.hi[ct] = T2; k.word[ct] = 0; }
-    k.tp = 0; k.full_lo = 0; k.full_hi = T2; k.tree = false;
+    for (int ct = 0; ct < CT; ++ct) k.node[ct] = 0;
+    k.tp = k.window = k.full_lo = 0;
+    k.rows = k.full_hi = T2;
+    k.words = nullptr;
     return k;
   }
 };
@@ -448,8 +566,8 @@ __device__ __forceinline__ int64_t q8_out_off(const Q8Params& p, int b, int kvh,
 // Many columns (prompts): a wave per column tile, no exchange between waves.
 // The second segment follows the walk in two passes (its maxima and sums, then
 // its rows weighted by g1 / sum), so that it needs no accumulators of its own.
-template <int D, int KT, int CT>
-__global__ __launch_bounds__(256, D == 64 ? 2 : 1) void k_attn8_wide(Q8Params p, Q8Words tw) {
+template <int D, int KT, int CT, bool SEG2>
+__global__ __launch_bounds__(256, 2) void k_attn8_wide(Q8Params p, Q8Words tw) {
   const int lane = threadIdx.x & 63, w = uni(threadIdx.x >> 6);
   const int BH = p.B * p.Hkv;
   // later tiles see the most keys and start first; the tiles of a head share an XCD where BH % 8 == 0
@@ -458,34 +576,28 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void k_attn8_wide(Q8Params p,
   if (c0 >= p.cols) return;
   Q8Tile<D, CT> t;
   t.init(p, tw, bh, c0, lane);
-  f32x4 acc[CT][D / 16];
-  float m[CT], l[CT];
+  Q8State<CT, D> st;
+  st.clear();
+  q8_walk<D, KT, CT, Q8_SOFTMAX, Q8_CHAIN>(t.src, t.first, 0, 1, t.steps, t.mask, p.c, t.qf, st, lane);
+  const float g0 = SEG2 ? p.gates[0] : 1.0f;
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
-    m[ct] = kNegInf;
-    l[ct] = 0.0f;
-#pragma unroll
-    for (int d = 0; d < D / 16; ++d) acc[ct][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  }
-  q8_walk<D, KT, CT, Q8_SOFTMAX>(t.src, t.first, 0, 1, t.steps, t.mask, p.c, t.qf, acc, m, l, lane);
-  const float g0 = p.T2 > 0 ? p.gates[0] : 1.0f;
-#pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    const float sum = q8_sum4(l[ct]);
+    const float sum = q8_sum4(st.l[ct]);
     const float inv = sum == 0.0f ? 0.0f : g0 / sum;
 #pragma unroll
-    for (int d = 0; d < D / 16; ++d) acc[ct][d] *= inv;
-    m[ct] = kNegInf;
-    l[ct] = 0.0f;
+    for (int d = 0; d < D / 16; ++d) st.acc[ct][d] *= inv;
+    st.m[ct] = 0.0f;
+    st.lim[ct] = kNegInf;
+    st.l[ct] = 0.0f;
   }
-  if (p.T2 > 0) {
+  if constexpr (SEG2) {
     const Q8Mask<CT> mk = t.mask2(p.T2);
     const int s1 = (p.T2 + 31) / 32;
-    q8_walk<D, KV_BF16, CT, Q8_STATS>(t.src2, 0, 0, 1, s1, mk, p.c, t.qf, acc, m, l, lane);
+    q8_walk<D, KV_BF16, CT, Q8_STATS, Q8_ALL>(t.src2, 0, 0, 1, s1, mk, p.c, t.qf, st, lane);
     const float g1 = p.gates[1];
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) l[ct] = g1 / q8_sum4(l[ct]);
-    q8_walk<D, KV_BF16, CT, Q8_FIXED>(t.src2, 0, 0, 1, s1, mk, p.c, t.qf, acc, m, l, lane);
+    for (int ct = 0; ct < CT; ++ct) st.l[ct] = g1 / q8_sum4(st.l[ct]);
+    q8_walk<D, KV_BF16, CT, Q8_FIXED, Q8_ALL>(t.src2, 0, 0, 1, s1, mk, p.c, t.qf, st, lane);
   }
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
@@ -495,7 +607,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void k_attn8_wide(Q8Params p,
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int d = 0; d < D / 16; ++d) v[i * (D / 16) + d] = acc[ct][d][i];
+        for (int d = 0; d < D / 16; ++d) v[i * (D / 16) + d] = st.acc[ct][d][i];
       q8_store<D / 4>(p, q8_out_off(p, t.b, t.kvh, col) + (lane >> 4) * (D / 4), v);
     }
   }
@@ -505,43 +617,37 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void k_attn8_wide(Q8Params p,
 // and over the 4 waves of each; a fifth wave takes the second segment (in the
 // last split).  The waves' (acc, m, l) meet in LDS; with one split the result
 // is written, else the split's partial (relative to its own maxima).
-template <int D, int KT, int CT>
-__global__ __launch_bounds__(320, 1) void k_attn8_split(Q8Params p, Q8Words tw) {
+template <int D, int KT, int CT, int KIND, bool SEG2>
+__global__ __launch_bounds__(SEG2 ? 320 : 256, 2) void k_attn8_split(Q8Params p, Q8Words tw) {
   constexpr int PD = D + 4;  // row pitch: four columns' 16-byte writes on distinct banks
-  __shared__ __attribute__((aligned(16))) float s_o[5 * 16 * PD];
-  __shared__ float s_m[5][16 * CT], s_l[5][16 * CT];
+  constexpr int NW = SEG2 ? 5 : 4;
+  __shared__ __attribute__((aligned(16))) float s_o[NW * 16 * PD];
+  __shared__ float s_m[NW][16 * CT], s_l[NW][16 * CT];
   const int lane = threadIdx.x & 63, w = uni(threadIdx.x >> 6);
   const int BH = p.B * p.Hkv;
   const int bh = blockIdx.x % BH, rest = blockIdx.x / BH;
   const int grp = rest % p.groups, split = rest / p.groups;
   Q8Tile<D, CT> t;
   t.init(p, tw, bh, grp * 16 * CT, lane);
-  f32x4 acc[CT][D / 16];
-  float m[CT], l[CT];
-#pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    m[ct] = kNegInf;
-    l[ct] = 0.0f;
-#pragma unroll
-    for (int d = 0; d < D / 16; ++d) acc[ct][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  }
-  const bool second = p.T2 > 0 && split == p.splits - 1;
-  if (w < 4) {
+  Q8State<CT, D> st;
+  st.clear();
+  const bool second = SEG2 && split == p.splits - 1;
+  if (!SEG2 || w < 4) {
     const int per = (t.steps + p.splits - 1) / p.splits;
     const int s1 = min(t.steps, (split + 1) * per);
-    q8_walk<D, KT, CT, Q8_SOFTMAX>(t.src, t.first, split * per + w, 4, s1, t.mask, p.c, t.qf, acc, m, l, lane);
+    q8_walk<D, KT, CT, Q8_SOFTMAX, KIND>(t.src, t.first, split * per + w, 4, s1, t.mask, p.c, t.qf, st, lane);
   } else if (second) {
-    q8_walk<D, KV_BF16, CT, Q8_SOFTMAX>(t.src2, 0, 0, 1, (p.T2 + 31) / 32, t.mask2(p.T2), p.c, t.qf, acc, m, l, lane);
+    q8_walk<D, KV_BF16, CT, Q8_SOFTMAX, Q8_ALL>(t.src2, 0, 0, 1, (p.T2 + 31) / 32, t.mask2(p.T2), p.c, t.qf, st, lane);
   }
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
-    l[ct] = q8_sum4(l[ct]);
+    const float l = q8_sum4(st.l[ct]);
     if (lane < 16) {
-      s_m[w][16 * ct + lane] = m[ct];
-      s_l[w][16 * ct + lane] = l[ct];
+      s_m[w][16 * ct + lane] = st.lim[ct] == kNegInf ? kNegInf : st.m[ct];
+      s_l[w][16 * ct + lane] = l;
     }
   }
-  const float g0 = p.T2 > 0 ? p.gates[0] : 1.0f, g1 = p.T2 > 0 ? p.gates[1] : 0.0f;
+  const float g0 = SEG2 ? p.gates[0] : 1.0f, g1 = SEG2 ? p.gates[1] : 0.0f;
   const int64_t unit = (int64_t)bh * p.groups + grp;
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
@@ -551,7 +657,7 @@ __global__ __launch_bounds__(320, 1) void k_attn8_split(Q8Params p, Q8Words tw) 
 #pragma unroll
       for (int d = 0; d < D / 16; d += 4)
         *reinterpret_cast<f32x4*>(o + i * (D / 16) + d) =
-            f32x4{acc[ct][d][i], acc[ct][d + 1][i], acc[ct][d + 2][i], acc[ct][d + 3][i]};
+            f32x4{st.acc[ct][d][i], st.acc[ct][d + 1][i], st.acc[ct][d + 2][i], st.acc[ct][d + 3][i]};
     __syncthreads();
     const int cc = threadIdx.x / 16, dd = threadIdx.x % 16 * (D / 16);
     const int col = t.col0 + 16 * ct + cc;
@@ -570,11 +676,12 @@ __global__ __launch_bounds__(320, 1) void k_attn8_split(Q8Params p, Q8Words tw) 
       }
       if (p.splits == 1) {
         const float inv = sum == 0.0f ? 0.0f : g0 / sum;
-        const float inv2 = second ? g1 / s_l[4][16 * ct + cc] : 0.0f;
 #pragma unroll
-        for (int d = 0; d < D / 16; ++d) {
-          v[d] *= inv;
-          if (second) v[d] = fmaf(s_o[(4 * 16 + cc) * PD + dd + d], inv2, v[d]);
+        for (int d = 0; d < D / 16; ++d) v[d] *= inv;
+        if constexpr (SEG2) {
+          const float inv2 = g1 / s_l[4][16 * ct + cc];
+#pragma unroll
+          for (int d = 0; d < D / 16; ++d) v[d] = fmaf(s_o[(4 * 16 + cc) * PD + dd + d], inv2, v[d]);
         }
         q8_store<D / 16>(p, q8_out_off(p, t.b, t.kvh, col) + dd, v);
       } else {
@@ -583,7 +690,7 @@ __global__ __launch_bounds__(320, 1) void k_attn8_split(Q8Params p, Q8Words tw) 
         for (int d = 0; d < D / 16; d += 4)
           *reinterpret_cast<f32x4*>(p.part_o + r * D + dd + d) = f32x4{v[d], v[d + 1], v[d + 2], v[d + 3]};
         if (dd == 0) p.part_ml[r] = make_float2(mx, sum);
-        if (second) {
+        if constexpr (SEG2) if (second) {
           const int64_t r2 = (unit * p.slots + p.splits) * (16 * CT) + 16 * ct + cc;
 #pragma unroll
           for (int d = 0; d < D / 16; ++d) v[d] = s_o[(4 * 16 + cc) * PD + dd + d];
@@ -651,7 +758,7 @@ Q8Plan q8_plan(const vnx_attn_q8_args* a) {
   const int cus = device_cus();
   Q8Plan pl{};
   pl.ct = most;
-  pl.wide = BH * ((tiles + most - 1) / most) >= 4 * (int64_t)cus;
+  pl.wide = !a->anc && !a->anc_host && BH * ((tiles + most - 1) / most) >= 4 * (int64_t)cus;
   if (pl.wide) {
     pl.groups = (int)((tiles + 4 * most - 1) / (4 * most));
     pl.splits = 1;
@@ -707,23 +814,26 @@ inline bool q8_strides(const int64_t* s, int n, int64_t unit) {
   return true;
 }
 
-template <int D, int KT, int CT>
+template <int D, int KT, int CT, int KIND, bool SEG2>
 void q8_launch(const Q8Params& p, const Q8Words& tw, const Q8Plan& pl, hipStream_t st) {
   const unsigned bh = (unsigned)(p.B * p.Hkv);
-  if (pl.wide)
-    hipLaunchKernelGGL((k_attn8_wide<D, KT, CT>), dim3(bh * pl.groups), dim3(256), 0, st, p, tw);
-  else
-    hipLaunchKernelGGL((k_attn8_split<D, KT, CT>), dim3(bh * pl.groups * pl.splits), dim3(p.T2 > 0 ? 320 : 256), 0, st,
-                       p, tw);
+  if constexpr (KIND == Q8_CHAIN) {  // (a tree's 64 nodes make few columns)
+    if (pl.wide) {
+      hipLaunchKernelGGL((k_attn8_wide<D, KT, CT, SEG2>), dim3(bh * pl.groups), dim3(256), 0, st, p, tw);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((k_attn8_split<D, KT, CT, KIND, SEG2>), dim3(bh * pl.groups * pl.splits), dim3(SEG2 ? 320 : 256), 0,
+                     st, p, tw);
 }
 
-template <int D, int KT>
+template <int D, int KT, int KIND, bool SEG2>
 int q8_by_ct(const Q8Params& p, const Q8Words& tw, const Q8Plan& pl, hipStream_t st) {
-  if (pl.ct == 1) q8_launch<D, KT, 1>(p, tw, pl, st);
-  else if (pl.ct == 2) q8_launch<D, KT, 2>(p, tw, pl, st);
+  if (pl.ct == 1) q8_launch<D, KT, 1, KIND, SEG2>(p, tw, pl, st);
+  else if (pl.ct == 2) q8_launch<D, KT, 2, KIND, SEG2>(p, tw, pl, st);
   if constexpr (D == 64) {
-    if (pl.ct == 3) q8_launch<D, KT, 3>(p, tw, pl, st);
-    else if (pl.ct == 4) q8_launch<D, KT, 4>(p, tw, pl, st);
+    if (pl.ct == 3) q8_launch<D, KT, 3, KIND, SEG2>(p, tw, pl, st);
+    else if (pl.ct == 4) q8_launch<D, KT, 4, KIND, SEG2>(p, tw, pl, st);
   }
   VNX_LAUNCH_CHECK();
   if (pl.splits > 1) {
@@ -800,9 +910,13 @@ int vnx_tree_attn_q8(const vnx_attn_q8_args* a, void* workspace, size_t workspac
   p.f16 = a->out_dtype == VNX_F16;
   p.c = (float)((double)a->scale * 1.4426950408889634);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (a->d == 64)
-    return a->kv_dtype == VNX_I8 ? q8_by_ct<64, KV_I8>(p, tw, pl, st) : q8_by_ct<64, KV_E4M3>(p, tw, pl, st);
-  return a->kv_dtype == VNX_I8 ? q8_by_ct<128, KV_I8>(p, tw, pl, st) : q8_by_ct<128, KV_E4M3>(p, tw, pl, st);
+  auto go = [&](auto d, auto kt) {
+    constexpr int D = decltype(d)::value, KT = decltype(kt)::value;
+    if (p.tree) return p.T2 > 0 ? q8_by_ct<D, KT, Q8_TREE, true>(p, tw, pl, st) : q8_by_ct<D, KT, Q8_TREE, false>(p, tw, pl, st);
+    return p.T2 > 0 ? q8_by_ct<D, KT, Q8_CHAIN, true>(p, tw, pl, st) : q8_by_ct<D, KT, Q8_CHAIN, false>(p, tw, pl, st);
+  };
+  if (a->d == 64) return a->kv_dtype == VNX_I8 ? go(IntC<64>{}, IntC<KV_I8>{}) : go(IntC<64>{}, IntC<KV_E4M3>{});
+  return a->kv_dtype == VNX_I8 ? go(IntC<128>{}, IntC<KV_I8>{}) : go(IntC<128>{}, IntC<KV_E4M3>{});
 }
 
 }  // extern "C"
