@@ -90,6 +90,18 @@ __device__ __forceinline__ float q8_sum4(float x) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// v_max3_f32: a NaN is passed over (fmaxf would quiet every operand first).
+__device__ __forceinline__ float q8_max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+__device__ __forceinline__ float q8_absmax3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, |%2|, |%3|" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
 // Where a wave's keys lie.
 struct Q8Src {
   const char* k;
@@ -284,8 +296,6 @@ __device__ __forceinline__ uint32_t q8_hidden(int tp, int window, int rows, cons
   return hide;
 }
 
-enum { Q8_SOFTMAX = 0, Q8_STATS = 1, Q8_FIXED = 2 };
-
 template <int CT, int D>
 struct Q8State {
   f32x4 acc[CT][D / 16];
@@ -310,14 +320,11 @@ struct Q8State {
   }
 };
 
-// Walks steps s0, s0 + ds, .. < s1 of 32 keys from key `first` on.
-//   Q8_SOFTMAX  online softmax into st
-//   Q8_STATS    m and l alone
-//   Q8_FIXED    acc += (exp2(x - m) * l) sv v: given maxima, l a weight
-// Codes: P sv / R in fp16 (2^-11), R the largest sv so far times 2^-6: P <= 2^8
+// Walks steps s0, s0 + ds, .. < s1 of 32 keys from key `first` on: online
+// softmax into st.  Codes: P sv / R in fp16 (2^-11), R the largest sv so far times 2^-6: P <= 2^8
 // and sv / R <= 2^7 stay in range, and a term keeps its 11 bits down to 2^-21 of
 // the largest row's scale (below: 2^-32 of it).  bf16 rows: P in two bf16 parts.
-template <int D, int KT, int CT, int MODE, int KIND>
+template <int D, int KT, int CT, int KIND>
 __device__ __forceinline__ void q8_walk(const Q8Src& src, int first, int s0, int ds, int s1, const Q8Mask<CT>& mk,
                                         float c, const bf16x8 (&qf)[CT][D / 32], Q8State<CT, D>& st, int lane) {
   if (s0 >= s1) return;
@@ -325,50 +332,43 @@ __device__ __forceinline__ void q8_walk(const Q8Src& src, int first, int s0, int
   Q8Keys<D, KT> keys;
   Q8Vals<D, KT> vals;
   auto left = [&](int s) { return s < s1 ? src.rows - (first + 32 * s) : 0; };
-  // All scores before the values where they take fewer registers than the key
-  // operands that they replace.
-  constexpr bool EARLY = CT * 8 <= D / 4;
   float R = 0.0f, iR = __builtin_inff();
   keys.load(src, first + 32 * s0, left(s0), lane);
-  if constexpr (MODE != Q8_STATS) vals.load(src, first + 32 * s0, left(s0), lane);
+  vals.load(src, first + 32 * s0, left(s0), lane);
   for (int s = s0; s < s1; s += ds) {
     const int k0 = first + 32 * s;
-    bf16x8 kf[2][D / 32];
-    keys.frag(0, kf[0]);
-    keys.frag(1, kf[1]);
-    float fk[8];
+    float x[CT][8];  // scores relative to the maxima, in the exp2 domain
+    {
+      bf16x8 kf[2][D / 32];
+      keys.frag(0, kf[0]);
+      keys.frag(1, kf[1]);
+      float fk[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) fk[e] = KT == KV_BF16 ? c : keys.sk[e / 4][e % 4] * c;
-    keys.load(src, k0 + 32 * ds, left(s + ds), lane);
-    float x[EARLY ? CT : 1][8];
-    // scores relative to the maxima, in the exp2 domain
-    auto scores = [&](int ct, float (&y)[8]) {
+      for (int e = 0; e < 8; ++e) fk[e] = KT == KV_BF16 ? c : keys.sk[e / 4][e % 4] * c;
+      keys.load(src, k0 + 32 * ds, left(s + ds), lane);
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        f32x4 a = {0.0f, 0.0f, 0.0f, 0.0f};
+      for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[t][i], qf[ct][i], a, 0, 0, 0);
+        for (int t = 0; t < 2; ++t) {
+          f32x4 a = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) y[4 * t + i] = fmaf(a[i], fk[4 * t + i], -st.m[ct]);
-      }
-    };
-    if constexpr (EARLY) {
+          for (int i = 0; i < D / 32; ++i) a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[t][i], qf[ct][i], a, 0, 0, 0);
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) scores(ct, x[ct]);
+          for (int i = 0; i < 4; ++i) x[ct][4 * t + i] = fmaf(a[i], fk[4 * t + i], -st.m[ct]);
+        }
     }
     u32x4 vf[D / 16];
     float sv[8];
-    if constexpr (MODE != Q8_STATS) {
+    {
       vals.frag(vf);
 #pragma unroll
       for (int d = 0; d < D / 16; ++d) asm volatile("" : "+v"(vf[d]));  // converted here: the rows' registers are free
       if constexpr (KT != KV_BF16) {
         float top = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          sv[e] = vals.sv[e / 4][e % 4];
-          top = fmaxf(top, fabsf(sv[e]));  // (NaN is passed over)
-        }
+        for (int e = 0; e < 8; ++e) sv[e] = vals.sv[e / 4][e % 4];
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) top = q8_absmax3(top, sv[e], sv[e + 1]);
         if (__any(!(top * iR <= 128.0f))) {
           top = 0x1p-110f;
 #pragma unroll
@@ -378,7 +378,7 @@ __device__ __forceinline__ void q8_walk(const Q8Src& src, int first, int s0, int
           }
           top = fmaxf(q8_max4(top) * 0x1p-6f, R);
           iR = 1.0f / top;
-          if constexpr (MODE == Q8_SOFTMAX) st.scale(R * iR);
+          st.scale(R * iR);
           R = top;
         }
 #pragma unroll
@@ -386,53 +386,64 @@ __device__ __forceinline__ void q8_walk(const Q8Src& src, int first, int s0, int
       }
       vals.load(src, k0 + 32 * ds, left(s + ds), lane);
     }
-    const bool full = k0 >= mk.full_lo && k0 + 32 <= mk.full_hi;
+    if (k0 < mk.full_lo || k0 + 32 > mk.full_hi) {
+      // some column does not see some key.  A scale that is not finite must
+      // reach the columns that see its key alone: through the score, not sv
+      uint32_t bad = 0;
+      if constexpr (KT != KV_BF16) {
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-      float(&xx)[8] = x[EARLY ? ct : 0];
-      if constexpr (!EARLY) scores(ct, xx);
-      uint32_t hide = 0;
-      if (!full) {
-        hide = q8_hidden<KIND>(mk.tp, mk.window, mk.rows, mk.words, mk.node[ct], k0, g4);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) xx[e] = hide & (1u << e) ? kNegInf : xx[e];
-      }
-      float& l = st.l[ct];
-      if constexpr (MODE != Q8_FIXED) {
-        float top = xx[0];
-#pragma unroll
-        for (int e = 1; e < 8; ++e) top = fmaxf(top, xx[e]);
-        if (__any(top > st.lim[ct])) {
-          const bool none = st.lim[ct] == kNegInf;
-          top = q8_max4(top);
-          const float up = top > (none ? kNegInf : 0.0f) ? top : 0.0f;
-          const float al = none ? 0.0f : q8_ex2(-up);
-          st.m[ct] += up;
-          if (top > kNegInf) st.lim[ct] = kQ8Jump;
-          l *= al;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) xx[e] -= up;
-          if constexpr (MODE == Q8_SOFTMAX) {
-#pragma unroll
-            for (int d = 0; d < D / 16; ++d) st.acc[ct][d] *= al;
-          }
+        for (int e = 0; e < 8; ++e) {
+          const bool b = !(fabsf(sv[e]) < __builtin_inff());
+          bad |= (uint32_t)b << e;
+          sv[e] = b ? 0.0f : sv[e];
         }
       }
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        const uint32_t hide = q8_hidden<KIND>(mk.tp, mk.window, mk.rows, mk.words, mk.node[ct], k0, g4);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          x[ct][e] = hide >> e & 1 ? kNegInf : bad >> e & 1 ? __builtin_nanf("") : x[ct][e];
+      }
+    }
+    {
+      float top[CT];
+      bool any = false;
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        top[ct] = q8_max3(q8_max3(x[ct][0], x[ct][1], x[ct][2]), q8_max3(x[ct][3], x[ct][4], x[ct][5]),
+                          fmaxf(x[ct][6], x[ct][7]));
+        any |= top[ct] > st.lim[ct];
+      }
+      if (__any(any)) {
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+          const bool none = st.lim[ct] == kNegInf;
+          const float t = q8_max4(top[ct]);
+          const float up = t > (none ? kNegInf : 0.0f) ? t : 0.0f;
+          const float al = none ? 0.0f : q8_ex2(-up);
+          st.m[ct] += up;
+          if (t > kNegInf) st.lim[ct] = kQ8Jump;
+          st.l[ct] *= al;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[ct][e] -= up;
+#pragma unroll
+          for (int d = 0; d < D / 16; ++d) st.acc[ct][d] *= al;
+        }
+      }
+    }
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
       float p[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        p[e] = q8_ex2(xx[e]);
-        if constexpr (MODE == Q8_FIXED) p[e] *= l;
-        else l += p[e];
+        p[e] = q8_ex2(x[ct][e]);
+        st.l[ct] += p[e];
       }
-      if constexpr (MODE != Q8_STATS) {
+      {
         if constexpr (KT != KV_BF16) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) p[e] *= sv[e];
-          if (!full) {  // a hidden row's scale may be NaN: nothing of it is kept
-#pragma unroll
-            for (int e = 0; e < 8; ++e) p[e] = hide & (1u << e) ? 0.0f : p[e];
-          }
           const u32x4 w = {q8_pk_f16(p[0], p[1]), q8_pk_f16(p[2], p[3]), q8_pk_f16(p[4], p[5]), q8_pk_f16(p[6], p[7])};
 #pragma unroll
           for (int d = 0; d < D / 16; ++d)
@@ -456,7 +467,7 @@ __device__ __forceinline__ void q8_walk(const Q8Src& src, int first, int s0, int
       }
     }
   }
-  if constexpr (KT != KV_BF16 && MODE == Q8_SOFTMAX) st.scale(R);
+  if constexpr (KT != KV_BF16) st.scale(R);
 }
 
 // A column's node and query head.
@@ -563,154 +574,173 @@ __device__ __forceinline__ int64_t q8_out_off(const Q8Params& p, int b, int kvh,
   return b * p.o_sb + (int64_t)(kvh * p.rep + h) * p.o_sh + (int64_t)node * p.o_sr;
 }
 
-// Many columns (prompts): a wave per column tile, no exchange between waves.
-// The second segment follows the walk in two passes (its maxima and sums, then
-// its rows weighted by g1 / sum), so that it needs no accumulators of its own.
-template <int D, int KT, int CT, bool SEG2>
-__global__ __launch_bounds__(256, 2) void k_attn8_wide(Q8Params p, Q8Words tw) {
+// A workgroup is CW column tiles (16 CT columns each) by KW waves that share a
+// tile's keys, 32 at a time in turn; `splits` workgroups share them further.
+//   KW = 1          many tiles (prompts): no exchange between waves;
+//   KW = 2, 4, 8    the waves' (acc, m, l) meet in LDS, 16 columns at a time.
+// With one split the result is written, else the split's partial (relative to
+// its own maxima).  The second segment: for KW <= 2 it is walked first, its
+// weighted result kept in LDS meanwhile (KW = 1: by the lane, else by the
+// thread that adds it again); for KW >= 4 (few steps a wave) a wave of its own
+// walks it beside the others, in the last split.  (us, 32 x 7 rows over 617,
+// 128 global rows: 7.8 with that wave, 10.1 walked first; 4 x 512 rows, KW = 2:
+// 18.1 walked first, 26 with the wave and KW = 4.)
+template <int D, int KT, int CT, int KIND, bool SEG2, int KW, int CW>
+__global__ __launch_bounds__((KW * CW + (SEG2 && KW >= 4)) * 64, 2) void k_attn8(Q8Params p, Q8Words tw) {
+  constexpr bool WAVE2 = SEG2 && KW >= 4, LDS2 = SEG2 && KW < 4;
+  constexpr int NW = KW * CW + WAVE2, COLS = 16 * CT;
+  constexpr int PD = D + 4;                         // row pitch in LDS
+  constexpr int TPC = KW == 2 ? 8 : 16;             // threads a column in the merge
+  constexpr int DP = D / TPC;                       // their dims
+  __shared__ __attribute__((aligned(16))) float s_o[KW > 1 ? NW * 16 * PD : 4];
+  __shared__ __attribute__((aligned(16))) float s_2[LDS2 ? CW * COLS * D : 4];
+  __shared__ float s_m[KW > 1 ? NW : 1][COLS], s_l[KW > 1 ? NW : 1][COLS];
   const int lane = threadIdx.x & 63, w = uni(threadIdx.x >> 6);
+  const bool extra = WAVE2 && w == KW;
+  const int kw = w % KW, cw = extra ? 0 : w / KW;
   const int BH = p.B * p.Hkv;
-  // later tiles see the most keys and start first; the tiles of a head share an XCD where BH % 8 == 0
-  const int bh = blockIdx.x % BH, grp = p.groups - 1 - blockIdx.x / BH;
-  const int c0 = (grp * 4 + w) * 16 * CT;
-  if (c0 >= p.cols) return;
+  // later tiles see the most keys and start first; a head's workgroups share an XCD where BH % 8 == 0
+  const int bh = blockIdx.x % BH, rest = blockIdx.x / BH;
+  const int grp = p.groups - 1 - rest % p.groups, split = rest / p.groups;
   Q8Tile<D, CT> t;
-  t.init(p, tw, bh, c0, lane);
+  t.init(p, tw, bh, min((grp * CW + cw) * COLS, (p.cols - 1) / COLS * COLS), lane);  // (a tile past the last: the last again)
   Q8State<CT, D> st;
-  st.clear();
-  q8_walk<D, KT, CT, Q8_SOFTMAX, Q8_CHAIN>(t.src, t.first, 0, 1, t.steps, t.mask, p.c, t.qf, st, lane);
-  const float g0 = SEG2 ? p.gates[0] : 1.0f;
+  // where this thread stands in the merge
+  const int mc = threadIdx.x / TPC, dd = threadIdx.x % TPC * DP;   // column (of 16 CW), first dim
+  const int mcw = mc / 16, cc = mc % 16;
+  const bool merges = mc < 16 * CW;
+  const int gcol = (grp * CW + mcw) * COLS + cc;                   // + 16 ct: the column
+  const int64_t unit = (int64_t)bh * p.groups + grp;
+
+  // Calls f(ct, values of DP dims, maximum, sum) for this thread's columns.
+  auto merge = [&](auto&& f) {
 #pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    const float sum = q8_sum4(st.l[ct]);
-    const float inv = sum == 0.0f ? 0.0f : g0 / sum;
+    for (int ct = 0; ct < CT; ++ct) {
+      const float l = q8_sum4(st.l[ct]);
+      if (lane < 16) {
+        s_m[w][16 * ct + lane] = st.lim[ct] == kNegInf ? kNegInf : st.m[ct];
+        s_l[w][16 * ct + lane] = l;
+      }
+    }
 #pragma unroll
-    for (int d = 0; d < D / 16; ++d) st.acc[ct][d] *= inv;
-    st.m[ct] = 0.0f;
-    st.lim[ct] = kNegInf;
-    st.l[ct] = 0.0f;
-  }
-  if constexpr (SEG2) {
-    const Q8Mask<CT> mk = t.mask2(p.T2);
-    const int s1 = (p.T2 + 31) / 32;
-    q8_walk<D, KV_BF16, CT, Q8_STATS, Q8_ALL>(t.src2, 0, 0, 1, s1, mk, p.c, t.qf, st, lane);
-    const float g1 = p.gates[1];
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) st.l[ct] = g1 / q8_sum4(st.l[ct]);
-    q8_walk<D, KV_BF16, CT, Q8_FIXED, Q8_ALL>(t.src2, 0, 0, 1, s1, mk, p.c, t.qf, st, lane);
-  }
-#pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    const int col = c0 + 16 * ct + (lane & 15);
-    if (col < p.cols) {
-      float v[D / 4];
+    for (int ct = 0; ct < CT; ++ct) {
+      float* o = s_o + (w * 16 + (lane & 15)) * PD + (lane >> 4) * (D / 4);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int d = 0; d < D / 16; ++d) v[i * (D / 16) + d] = st.acc[ct][d][i];
-      q8_store<D / 4>(p, q8_out_off(p, t.b, t.kvh, col) + (lane >> 4) * (D / 4), v);
-    }
-  }
-}
-
-// Few columns: the keys of a column group are split over `splits` workgroups
-// and over the 4 waves of each; a fifth wave takes the second segment (in the
-// last split).  The waves' (acc, m, l) meet in LDS; with one split the result
-// is written, else the split's partial (relative to its own maxima).
-template <int D, int KT, int CT, int KIND, bool SEG2>
-__global__ __launch_bounds__(SEG2 ? 320 : 256, 2) void k_attn8_split(Q8Params p, Q8Words tw) {
-  constexpr int PD = D + 4;  // row pitch: four columns' 16-byte writes on distinct banks
-  constexpr int NW = SEG2 ? 5 : 4;
-  __shared__ __attribute__((aligned(16))) float s_o[NW * 16 * PD];
-  __shared__ float s_m[NW][16 * CT], s_l[NW][16 * CT];
-  const int lane = threadIdx.x & 63, w = uni(threadIdx.x >> 6);
-  const int BH = p.B * p.Hkv;
-  const int bh = blockIdx.x % BH, rest = blockIdx.x / BH;
-  const int grp = rest % p.groups, split = rest / p.groups;
-  Q8Tile<D, CT> t;
-  t.init(p, tw, bh, grp * 16 * CT, lane);
-  Q8State<CT, D> st;
-  st.clear();
-  const bool second = SEG2 && split == p.splits - 1;
-  if (!SEG2 || w < 4) {
-    const int per = (t.steps + p.splits - 1) / p.splits;
-    const int s1 = min(t.steps, (split + 1) * per);
-    q8_walk<D, KT, CT, Q8_SOFTMAX, KIND>(t.src, t.first, split * per + w, 4, s1, t.mask, p.c, t.qf, st, lane);
-  } else if (second) {
-    q8_walk<D, KV_BF16, CT, Q8_SOFTMAX, Q8_ALL>(t.src2, 0, 0, 1, (p.T2 + 31) / 32, t.mask2(p.T2), p.c, t.qf, st, lane);
-  }
-#pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    const float l = q8_sum4(st.l[ct]);
-    if (lane < 16) {
-      s_m[w][16 * ct + lane] = st.lim[ct] == kNegInf ? kNegInf : st.m[ct];
-      s_l[w][16 * ct + lane] = l;
-    }
-  }
-  const float g0 = SEG2 ? p.gates[0] : 1.0f, g1 = SEG2 ? p.gates[1] : 0.0f;
-  const int64_t unit = (int64_t)bh * p.groups + grp;
-#pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    float* o = s_o + (w * 16 + (lane & 15)) * PD + (lane >> 4) * (D / 4);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int d = 0; d < D / 16; d += 4)
-        *reinterpret_cast<f32x4*>(o + i * (D / 16) + d) =
-            f32x4{st.acc[ct][d][i], st.acc[ct][d + 1][i], st.acc[ct][d + 2][i], st.acc[ct][d + 3][i]};
-    __syncthreads();
-    const int cc = threadIdx.x / 16, dd = threadIdx.x % 16 * (D / 16);
-    const int col = t.col0 + 16 * ct + cc;
-    if (threadIdx.x < 256 && col < p.cols) {
-      float mx = kNegInf;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s_m[i][16 * ct + cc]);
-      float sum = 0.0f, v[D / 16] = {};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float mi = s_m[i][16 * ct + cc];
-        const float e = mi == kNegInf ? 0.0f : q8_ex2(mi - mx);
-        sum += s_l[i][16 * ct + cc] * e;
-#pragma unroll
-        for (int d = 0; d < D / 16; ++d) v[d] = fmaf(s_o[(i * 16 + cc) * PD + dd + d], e, v[d]);
-      }
-      if (p.splits == 1) {
-        const float inv = sum == 0.0f ? 0.0f : g0 / sum;
-#pragma unroll
-        for (int d = 0; d < D / 16; ++d) v[d] *= inv;
-        if constexpr (SEG2) {
-          const float inv2 = g1 / s_l[4][16 * ct + cc];
-#pragma unroll
-          for (int d = 0; d < D / 16; ++d) v[d] = fmaf(s_o[(4 * 16 + cc) * PD + dd + d], inv2, v[d]);
-        }
-        q8_store<D / 16>(p, q8_out_off(p, t.b, t.kvh, col) + dd, v);
-      } else {
-        const int64_t r = (unit * p.slots + split) * (16 * CT) + 16 * ct + cc;
-#pragma unroll
         for (int d = 0; d < D / 16; d += 4)
+          *reinterpret_cast<f32x4*>(o + i * (D / 16) + d) =
+              f32x4{st.acc[ct][d][i], st.acc[ct][d + 1][i], st.acc[ct][d + 2][i], st.acc[ct][d + 3][i]};
+      __syncthreads();
+      if (merges) {
+        float mx = kNegInf;
+#pragma unroll
+        for (int i = 0; i < KW; ++i) mx = fmaxf(mx, s_m[mcw * KW + i][16 * ct + cc]);
+        float sum = 0.0f, v[DP] = {};
+#pragma unroll
+        for (int i = 0; i < KW; ++i) {
+          const float mi = s_m[mcw * KW + i][16 * ct + cc];
+          const float e = mi == kNegInf ? 0.0f : q8_ex2(mi - mx);
+          sum += s_l[mcw * KW + i][16 * ct + cc] * e;
+          const float* r = s_o + ((mcw * KW + i) * 16 + cc) * PD + dd;
+#pragma unroll
+          for (int d = 0; d < DP; ++d) v[d] = fmaf(r[d], e, v[d]);
+        }
+        f(ct, v, mx, sum);
+      }
+      __syncthreads();  // s_o (s_m, s_l) may be written again
+    }
+  };
+
+  float g0 = 1.0f, g1 = 0.0f;
+  if constexpr (SEG2) {
+    g0 = p.gates[0];
+    g1 = p.gates[1];
+  }
+  if constexpr (LDS2) {
+    st.clear();
+    q8_walk<D, KV_BF16, CT, Q8_ALL>(t.src2, 0, kw, KW, (p.T2 + 31) / 32, t.mask2(p.T2), p.c, t.qf, st, lane);
+    if constexpr (KW > 1) {
+      merge([&](int ct, float (&v)[DP], float mx, float sum) {
+#pragma unroll
+        for (int d = 0; d < DP; ++d) s_2[(mcw * COLS + 16 * ct + cc) * D + dd + d] = v[d] * (g1 / sum);
+      });
+    } else {
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        const float inv = g1 / q8_sum4(st.l[ct]);
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d)
+          *reinterpret_cast<f32x4*>(s_2 + (((w * CT + ct) * (D / 16) + d) * 64 + lane) * 4) = st.acc[ct][d] * inv;
+      }
+    }
+  }
+  st.clear();
+  const bool second = WAVE2 && split == p.splits - 1;
+  if (!extra) {
+    const int per = (t.steps + p.splits - 1) / p.splits;
+    q8_walk<D, KT, CT, KIND>(t.src, t.first, split * per + kw, KW, min(t.steps, (split + 1) * per), t.mask, p.c, t.qf,
+                             st, lane);
+  } else if (second) {
+    q8_walk<D, KV_BF16, CT, Q8_ALL>(t.src2, 0, 0, 1, (p.T2 + 31) / 32, t.mask2(p.T2), p.c, t.qf, st, lane);
+  }
+  if constexpr (KW > 1) {
+    merge([&](int ct, float (&v)[DP], float mx, float sum) {
+      const int col = gcol + 16 * ct;
+      if (col >= p.cols) return;
+      const float* o2 = s_o + (KW * 16 + cc) * PD + dd;  // (WAVE2)
+      if (p.splits > 1) {
+        const int64_t r = (unit * p.slots + split) * COLS + 16 * ct + cc;  // (CW = 1)
+#pragma unroll
+        for (int d = 0; d < DP; d += 4)
           *reinterpret_cast<f32x4*>(p.part_o + r * D + dd + d) = f32x4{v[d], v[d + 1], v[d + 2], v[d + 3]};
         if (dd == 0) p.part_ml[r] = make_float2(mx, sum);
-        if constexpr (SEG2) if (second) {
-          const int64_t r2 = (unit * p.slots + p.splits) * (16 * CT) + 16 * ct + cc;
+        if (second) {
 #pragma unroll
-          for (int d = 0; d < D / 16; ++d) v[d] = s_o[(4 * 16 + cc) * PD + dd + d];
-#pragma unroll
-          for (int d = 0; d < D / 16; d += 4)
-            *reinterpret_cast<f32x4*>(p.part_o + r2 * D + dd + d) = f32x4{v[d], v[d + 1], v[d + 2], v[d + 3]};
-          if (dd == 0) p.part_ml[r2] = make_float2(s_m[4][16 * ct + cc], s_l[4][16 * ct + cc]);
+          for (int d = 0; d < DP; d += 4)
+            *reinterpret_cast<f32x4*>(p.part_o + (r + COLS) * D + dd + d) = *reinterpret_cast<const f32x4*>(o2 + d);
+          if (dd == 0) p.part_ml[r + COLS] = make_float2(s_m[KW][16 * ct + cc], s_l[KW][16 * ct + cc]);
         }
+        return;
       }
+      const float inv = sum == 0.0f ? 0.0f : g0 / sum;
+      float inv2 = 0.0f;
+      if constexpr (WAVE2) inv2 = g1 / s_l[KW][16 * ct + cc];
+#pragma unroll
+      for (int d = 0; d < DP; ++d) {
+        v[d] *= inv;
+        if constexpr (LDS2) v[d] += s_2[(mcw * COLS + 16 * ct + cc) * D + dd + d];
+        if constexpr (WAVE2) v[d] = fmaf(o2[d], inv2, v[d]);
+      }
+      q8_store<DP>(p, q8_out_off(p, t.b, t.kvh, col) + dd, v);
+    });
+  } else {
+    const int c0 = (grp * CW + cw) * COLS;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      const float sum = q8_sum4(st.l[ct]);
+      const float inv = sum == 0.0f ? 0.0f : g0 / sum;
+      float v[D / 4];
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) {
+        f32x4 o = st.acc[ct][d] * inv;
+        if constexpr (SEG2) o += *reinterpret_cast<const f32x4*>(s_2 + (((w * CT + ct) * (D / 16) + d) * 64 + lane) * 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i * (D / 16) + d] = o[i];
+      }
+      const int col = c0 + 16 * ct + (lane & 15);
+      if (col < p.cols) q8_store<D / 4>(p, q8_out_off(p, t.b, t.kvh, col) + (lane >> 4) * (D / 4), v);
     }
-    if (ct + 1 < CT) __syncthreads();  // s_o is written again
   }
 }
 
-// Joins the splits' partials: four dims of a column a thread.
+// Joins the splits' partials, a wave a column: lane s takes split s's weight,
+// then D / 4 lanes (four dims each) walk the splits 256 / D at a time.
 template <int D>
 __global__ __launch_bounds__(256) void k_attn8_join(Q8Params p, int ct16) {
-  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int dd = (int)(id % (D / 4)) * 4;
-  const int64_t cell = id / (D / 4);   // unit * ct16 + column of the group
+  constexpr int L = D / 4, G = 64 / L;
+  const int lane = threadIdx.x & 63;
+  const int64_t cell = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);  // unit * ct16 + column of the group (CW = 1)
   const int64_t unit = cell / ct16;
   if (unit >= (int64_t)p.B * p.Hkv * p.groups) return;
   const int cc = (int)(cell - unit * ct16);
@@ -718,19 +748,29 @@ __global__ __launch_bounds__(256) void k_attn8_join(Q8Params p, int ct16) {
   const int col = grp * ct16 + cc;
   if (col >= p.cols) return;
   const int64_t r0 = unit * p.slots * ct16 + cc;
-  float mx = kNegInf;
-  for (int s = 0; s < p.splits; ++s) mx = fmaxf(mx, p.part_ml[r0 + (int64_t)s * ct16].x);
-  float sum = 0.0f;
-  f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int s = 0; s < p.splits; ++s) {
-    const int64_t r = r0 + (int64_t)s * ct16;
-    const float2 ml = p.part_ml[r];
-    const float e = ml.x == kNegInf ? 0.0f : q8_ex2(ml.x - mx);
-    sum += ml.y * e;
-    const f32x4 o = *reinterpret_cast<const f32x4*>(p.part_o + r * D + dd);
+  float2 ml = make_float2(kNegInf, 0.0f);
+  if (lane < p.splits) ml = p.part_ml[r0 + (int64_t)lane * ct16];
+  float mx = ml.x;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = fmaf(o[i], e, v[i]);
+  for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
+  const float e = ml.x == kNegInf ? 0.0f : q8_ex2(ml.x - mx);
+  float sum = ml.y * e;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+  const int g = lane / L, dd = lane % L * 4;
+  f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+  for (int s = g; s < p.splits; s += G) {
+    const float w = __shfl(e, s, 64);
+    const f32x4 o = *reinterpret_cast<const f32x4*>(p.part_o + (r0 + (int64_t)s * ct16) * D + dd);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = fmaf(o[i], w, v[i]);
   }
+#pragma unroll
+  for (int o = L; o < 64; o <<= 1)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] += __shfl_xor(v[i], o, 64);
+  if (g) return;
   const float g0 = p.T2 > 0 ? p.gates[0] : 1.0f;
   v *= sum == 0.0f ? 0.0f : g0 / sum;
   if (p.T2 > 0) {
@@ -745,34 +785,87 @@ __global__ __launch_bounds__(256) void k_attn8_join(Q8Params p, int ct16) {
   q8_store<4>(p, q8_out_off(p, b, kvh, col) + dd, t);
 }
 
-// The launch shape: column tiles of 16 a wave, column groups, key splits.
+// The launch shape: column tiles of 16 a wave, waves that share a tile's keys,
+// column groups, key splits.
 struct Q8Plan {
-  int ct, groups, splits;
-  bool wide;
+  int ct, kw, groups, splits;
 };
 
-Q8Plan q8_plan(const vnx_attn_q8_args* a) {
-  const int64_t cols = (int64_t)(a->H / a->Hkv) * a->N, BH = (int64_t)a->B * a->Hkv;
-  const int most = a->d == 64 ? 4 : 2;
-  const int64_t tiles = (cols + 15) / 16;
-  const int cus = device_cus();
-  Q8Plan pl{};
-  pl.ct = most;
-  pl.wide = !a->anc && !a->anc_host && BH * ((tiles + most - 1) / most) >= 4 * (int64_t)cus;
-  if (pl.wide) {
-    pl.groups = (int)((tiles + 4 * most - 1) / (4 * most));
-    pl.splits = 1;
-    return pl;
+// Waves that share a workgroup's columns, per keys wave.
+constexpr int q8_cw(int kw) { return kw == 1 ? 4 : kw == 2 ? 2 : 1; }
+
+// Estimated us of a launch shape, for comparing shapes.  A wave's step costs
+// the conversion of its rows and its columns' softmax; a SIMD issues for two
+// waves at once what one wave issues in half the slots (one instruction a
+// wave in 8 cycles, measured), so a step's share of the chip shrinks with
+// the waves beside it until both slots are taken; rows read by several column
+// groups cost HBM and L2 time again; splits cost a second launch and their
+// partials.  The constants are fitted to 1,700 timings of 70 shapes (1-64
+// sequences, 1-2,048 new rows, 1-16,000 keys, both head sizes): the shape
+// picked is the fastest of them within 3% on average and 21% at worst.
+// us, 16 trees of 40 nodes over 2,048 rows: ct 3 x 8 waves 18.8, ct 1 x 4 waves 23.5;
+// 4 prompts of 512: ct 2 x 2 waves 18.1, ct 4 x 4 waves 24.6; 8 x 5 rows over 16,000,
+// heads of 128: ct 2 x 4 splits 55.6, no split 139, ct 1 x 4 splits 76.
+float q8_cost(int BH, int tiles, int d2, float last, float mean, float mem, int T2, int cus, int ct, int kw, int S,
+              int groups) {
+  constexpr float kMerge = 0.571f, kJoin = 1.0f, kPart = 8.249e-3f, kStep = 0.205f, kConv = 0.284f, kCol = 0.252f,
+                  kSeg2 = 0.219f, kWide = 3.43f, kLone = 2.836f, kRound = 6.258f, kAgain = 1.709f;
+  const int cw = q8_cw(kw);
+  const float v = kCol * (kConv * d2 + ct * (1.0f + 0.3f * (d2 - 1)));
+  const int occ = d2 == 1 ? (ct == 1 ? 4 : ct == 2 ? 3 : 2) : 2;  // waves a SIMD has registers for
+  const int waves = kw * cw + (T2 > 0 && kw >= 4);
+  const int per = occ * 4 / waves > 1 ? occ * 4 / waves : 1;      // workgroups a CU
+  const float wgs = (float)BH * groups * S, rounds = wgs / ((float)cus * per);
+  const float nl = __builtin_ceilf(__builtin_ceilf(last / 32) / (kw * S));
+  const float nm = mean / 32 > kw * S ? mean / 32 / (kw * S) : 1.0f;
+  const float here = wgs / cus < per ? wgs / cus : per;
+  const float busy = here * kw * cw / 4 > 2.0f ? here * kw * cw / 8 : 1.0f;
+  float t;
+  if (rounds <= 1.0f) {
+    const float one = nl * v, all = nm * v * busy;
+    t = nl * kStep + (one > all ? one : all);
+  } else {
+    t = (nm * kStep + nm * v * busy) * (rounds < 2.5f ? __builtin_ceilf(rounds) : rounds + 0.3f);
+    t += kRound * (__builtin_ceilf(rounds) - 1);
   }
-  pl.groups = (int)((tiles + most - 1) / most);
-  pl.ct = (int)((tiles + pl.groups - 1) / pl.groups);
-  // keys a column group walks: about a workgroup a CU, 128 keys a split at least
-  const int64_t keys = a->window > 0 && a->window < a->Tp + a->N ? (int64_t)a->window + a->N : (int64_t)a->Tp + a->N;
-  const int64_t units = BH * pl.groups;
-  int64_t s = units >= cus ? 1 : (cus + units - 1) / units;
-  s = s < keys / 128 ? s : keys / 128;
-  pl.splits = (int)(s < 1 ? 1 : s > kQ8Split ? kQ8Split : s);
-  return pl;
+  t += (kw > 1 ? kMerge * ct * d2 : kLone) * busy * (rounds > 1.0f ? rounds : 1.0f) + (kw == 8 ? kWide : 0.0f);
+  const float m = mem * (1.0f + kAgain * (groups * cw - 1));
+  t = t > m ? t : m;
+  if (S > 1) t += kJoin + kPart * BH * groups * ct * S * d2;
+  if (T2 > 0 && kw < 4) t += kSeg2 * (1 + (T2 + 31) / 32 / kw);
+  return t;
+}
+
+Q8Plan q8_plan(const vnx_attn_q8_args* a) {
+  const int rep = a->H / a->Hkv, BH = a->B * a->Hkv, d2 = a->d / 64;
+  const int tiles = (int)(((int64_t)rep * a->N + 15) / 16);
+  const bool tree = a->anc || a->anc_host;
+  const float W = a->window > 0 ? (float)a->window : 1e9f, keys = (float)a->Tp + a->N;
+  const int cus = device_cus();
+  // HBM time of the rows once, at 10 TB/s (the fit's way to say that it overlaps)
+  const float mem = BH * (keys < W + a->N ? keys : W + a->N) * 2 * (a->d + 4) / 10.2e6f;
+  Q8Plan best{1, 4, tiles, 1};
+  float least = 1e30f;
+  const int most = tiles < 4 / d2 ? tiles : 4 / d2;
+  for (int ct = 1; ct <= most; ++ct) {
+    const float span = (float)(16 * ct / rep + 2 < a->N ? 16 * ct / rep + 2 : a->N);  // rows of a tile
+    const float end = tree ? (float)a->N : span;
+    const float last = keys < W + end ? keys : W + end;
+    const float mid = tree ? keys : (float)a->Tp + (a->N + span) / 2;
+    const float mean = mid < W + end ? mid : W + end;
+    for (int kw = tree ? 4 : 1; kw <= (a->T2 > 0 ? 4 : 8); kw *= 2) {
+      const int groups = (tiles + ct * q8_cw(kw) - 1) / (ct * q8_cw(kw));
+      for (int S = 1; S <= (kw < 4 ? 1 : kQ8Split); S *= 2) {
+        if (S > 1 && ((int64_t)BH * groups * S > 6 * cus || last < 32 * S)) break;
+        const float t = q8_cost(BH, tiles, d2, last, mean, mem, a->T2, cus, ct, kw, S, groups);
+        if (t < least) {
+          least = t;
+          best = {ct, kw, groups, S};
+        }
+      }
+    }
+  }
+  return best;
 }
 
 size_t q8_ws_bytes(const vnx_attn_q8_args* a, const Q8Plan& pl, Q8Params* p, void* ws) {
@@ -816,15 +909,24 @@ inline bool q8_strides(const int64_t* s, int n, int64_t unit) {
 
 template <int D, int KT, int CT, int KIND, bool SEG2>
 void q8_launch(const Q8Params& p, const Q8Words& tw, const Q8Plan& pl, hipStream_t st) {
-  const unsigned bh = (unsigned)(p.B * p.Hkv);
+  const dim3 grid((unsigned)(p.B * p.Hkv * pl.groups * pl.splits));
   if constexpr (KIND == Q8_CHAIN) {  // (a tree's 64 nodes make few columns)
-    if (pl.wide) {
-      hipLaunchKernelGGL((k_attn8_wide<D, KT, CT, SEG2>), dim3(bh * pl.groups), dim3(256), 0, st, p, tw);
+    if (pl.kw == 1) {
+      hipLaunchKernelGGL((k_attn8<D, KT, CT, KIND, SEG2, 1, 4>), grid, dim3(256), 0, st, p, tw);
+      return;
+    }
+    if (pl.kw == 2) {
+      hipLaunchKernelGGL((k_attn8<D, KT, CT, KIND, SEG2, 2, 2>), grid, dim3(256), 0, st, p, tw);
       return;
     }
   }
-  hipLaunchKernelGGL((k_attn8_split<D, KT, CT, KIND, SEG2>), dim3(bh * pl.groups * pl.splits), dim3(SEG2 ? 320 : 256), 0,
-                     st, p, tw);
+  if constexpr (!SEG2) {  // (a ninth wave would leave 168 registers a lane)
+    if (pl.kw == 8) {
+      hipLaunchKernelGGL((k_attn8<D, KT, CT, KIND, SEG2, 8, 1>), grid, dim3(512), 0, st, p, tw);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((k_attn8<D, KT, CT, KIND, SEG2, 4, 1>), grid, dim3(256 + 64 * SEG2), 0, st, p, tw);
 }
 
 template <int D, int KT, int KIND, bool SEG2>
@@ -837,8 +939,8 @@ int q8_by_ct(const Q8Params& p, const Q8Words& tw, const Q8Plan& pl, hipStream_t
   }
   VNX_LAUNCH_CHECK();
   if (pl.splits > 1) {
-    const int64_t work = (int64_t)p.B * p.Hkv * p.groups * 16 * pl.ct * (D / 4);
-    hipLaunchKernelGGL((k_attn8_join<D>), dim3((unsigned)((work + 255) / 256)), dim3(256), 0, st, p, 16 * pl.ct);
+    hipLaunchKernelGGL((k_attn8_join<D>), dim3((unsigned)(p.B * p.Hkv * p.groups * 4 * pl.ct)), dim3(256), 0, st, p,
+                       16 * pl.ct);
     VNX_LAUNCH_CHECK();
   }
   return VNX_OK;
