@@ -236,3 +236,84 @@ def test_rows_past_4_gib(hip):
     o = hip.tree_attention_q8(q[:, :, -3:], kc, vc, ks, vs, [cap - 3]).cpu()
     ref, mag = R.attention(q[:, :, -3:].cpu(), R.values(*kd), R.values(*vd), [cap - 3], cap - 3)
     assert ((o.to(R.F64) - ref).abs() <= 2.0 ** -8 * (1.02 * mag + ref.abs())).all()
+
+
+def test_binding_and_general_path_agree(hip):
+    """The calls that the binding serves and the same calls through the general path (lengths as a list, scales' strides
+    alike): the same bits.  What the binding leaves: strides and types that need a copy."""
+    dev = hip.torch_device
+    B, n, H, Hkv, d, cap = 2, 3, 4, 2, 64, 16
+    g = R.gen(21)
+    x = torch.randn(B, n, (H + 2 * Hkv) * d, generator=g).to(torch.bfloat16).to(dev)
+    ang = torch.rand(cap, d // 2, generator=g) * 6.28
+    cos, sin = (torch.cat([f(ang)] * 2, 1).to(dev) for f in (torch.cos, torch.sin))
+    lens = torch.tensor([4, 11], dtype=torch.int32, device=dev)
+    b, st = hip._bind, hip._stream()
+    got = []
+    for ln in (lens, [4, 11]):
+        kc, vc = (torch.zeros(B, Hkv, cap, d, dtype=E4, device=dev) for _ in range(2))
+        ks, vs = (torch.zeros(B, Hkv, cap, device=dev) for _ in range(2))
+        q = hip.kv_write(x, kc, vc, ln, k_scale=ks, v_scale=vs, cos=cos, sin=sin)
+        k, v = hip.kv_read(kc, vc, ks, vs, start=ln, rows=n)
+        o = hip.tree_attention_q8(q, kc, vc, ks, vs, ln)
+        got.append((q, kc.view(torch.uint8), vc.view(torch.uint8), ks, vs, k, v, o))
+    for a, c in zip(*got):
+        assert torch.equal(a, c)
+    assert b.kv_write(0, st, kc, vc, ks, vs, x, lens, cos, sin, None, None, 1e-6) is not None
+    for xx in (x.double(), x[:, :, :-32], x.expand(B, n, -1)[:1], x.transpose(1, 2)):
+        assert b.kv_write(0, st, kc, vc, ks, vs, xx, lens, cos, sin, None, None, 1e-6) is None
+    assert b.kv_write(0, st, kc, vc, ks, vs, x, lens.long(), cos, sin, None, None, 1e-6) is None
+    assert b.kv_write(0, st, kc, vc, ks, vs, x, lens, cos, None, None, None, 1e-6) is None
+    assert b.kv_write(1, st, kc, vc, ks, vs, x, lens, cos, sin, None, None, 1e-6) is None
+    assert b.tree_attn_q8(0, st, kc, vc, ks, vs, q.float(), lens, None, None, None, None, 0, None, torch.bfloat16,
+                          None) is None
+    assert b.tree_attn_q8(0, st, kc, vc, ks, vs, q, lens, None, None, None, None, 0, cap, torch.bfloat16, None) is None
+    assert b.tree_attn_q8(0, st, kc, vc, ks, vs, q, lens, None, -1.0, None, None, 0, None, torch.bfloat16,
+                          None) == -1
+
+
+def test_refusals(hip):
+    """What neither path can serve raises ValueError and writes nothing."""
+    dev = hip.torch_device
+    B, n, H, Hkv, d, cap = 2, 3, 4, 2, 64, 16
+    kc, vc, ks, vs = _empty(B, Hkv, cap, d, I8, dev)
+    x = torch.zeros(B, n, (H + 2 * Hkv) * d, device=dev)
+    q = torch.zeros(B, H, n, d, dtype=torch.bfloat16, device=dev)
+    lens = [1, 2]
+    cos = torch.zeros(cap, d, device=dev)
+    before = [t.clone() for t in (kc, ks)]
+    bad = [
+        lambda: hip.kv_write(x[:, :, :-1], kc, vc, lens, ks, vs), lambda: hip.kv_write(x[:1], kc, vc, lens, ks, vs),
+        lambda: hip.kv_write(x.long(), kc, vc, lens, ks, vs), lambda: hip.kv_write(x, kc, vc, [1], ks, vs),
+        lambda: hip.kv_write(x, kc, vc, lens), lambda: hip.kv_write(x, kc.cpu(), vc, lens, ks, vs),
+        lambda: hip.kv_write(x, kc, vc[:, :, :8], lens, ks, vs), lambda: hip.kv_write(x, kc, vc, lens, ks, vs, cos=cos),
+        lambda: hip.kv_write(x, kc, vc, lens, ks, vs, cos=cos[:, :32], sin=cos[:, :32]),
+        lambda: hip.kv_write(x, kc, vc, lens, ks, vs, q_norm=cos[0, :32]),
+        lambda: hip.kv_write(x, kc, vc, lens, ks.double(), vs.double()), lambda: hip.kv_write(x, kc.short(), vc.short(), lens),
+        lambda: hip.kv_write(x[:, :, :4 * d], kc, vc, lens, ks, vs),
+        lambda: hip.kv_read(kc, vc, ks, vs, rows=-1), lambda: hip.kv_read(kc, vc, ks[:, :, :4], vs[:, :, :4]),
+        lambda: hip.kv_read(kc, vc, ks, vs, out_dtype=torch.float64), lambda: hip.kv_read(kc, vc),
+        lambda: hip.kv_read(kc[..., 1:], vc[..., 1:], ks, vs),
+        lambda: hip.tree_attention_q8(q, kc, vc, ks, vs, lens, max_len=cap), lambda: hip.tree_attention_q8(q, kc, vc, ks, vs, [1]),
+        lambda: hip.tree_attention_q8(q[..., :32], kc, vc, ks, vs, lens), lambda: hip.tree_attention_q8(q[:, :3], kc, vc, ks, vs, lens),
+        lambda: hip.tree_attention_q8(q, kc, vc, ks, vs, lens, window=-1), lambda: hip.tree_attention_q8(q, kc, vc, ks, vs, lens, scale=0.0),
+        lambda: hip.tree_attention_q8(q, kc, vc, ks, vs, lens, anc=[1, 3]),
+        lambda: hip.tree_attention_q8(q, kc, vc, ks, vs, lens, anc=[1, 3, 7], window=2),
+        lambda: hip.tree_attention_q8(q, kc, vc, ks, vs, lens, out_dtype=torch.float32),
+        lambda: hip.tree_attention_q8(q, kc, vc, ks, vs, lens, out=q.float()), lambda: hip.tree_attention_q8(q, kc, vc, ks, vs, lens, out=q[:1]),
+        lambda: hip.tree_attention_q8(q, kc, vc, ks, vs, lens, seg2=(q[:, :2], q[:, :2])),
+        lambda: hip.tree_attention_q8(q, kc, vc, ks, vs, lens, seg2=(q[:, :2, :0], q[:, :2, :0]), gates=[1, 1]),
+        lambda: hip.tree_attention_q8(q, kc.bfloat16(), vc.bfloat16(), None, None, lens),
+    ]
+    for i, f in enumerate(bad):
+        with pytest.raises(ValueError):
+            f()
+            print("accepted:", i)
+    torch.cuda.synchronize(dev)
+    for t, w in zip((kc, ks), before):
+        assert torch.equal(t, w)
+    # empty batches and ranges are no errors
+    assert hip.kv_read(kc, vc, ks, vs, rows=0)[0].shape == (B, Hkv, 0, d)
+    assert hip.kv_read(kc[:0], vc[:0], ks[:0], vs[:0])[0].shape == (0, Hkv, cap, d)
+    assert hip.kv_write(x[:0], kc[:0], vc[:0], [], ks[:0], vs[:0]).shape == (0, H, n, d)
+    assert hip.tree_attention_q8(q[:0], kc[:0], vc[:0], ks[:0], vs[:0], []).shape == (0, H, n, d)

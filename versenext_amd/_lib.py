@@ -277,6 +277,29 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
+_bind = None
+
+
+def bind():
+    """The _vnx_bind module (csrc/bind.cpp), pointed at the loaded library's
+    entries (raises RuntimeError if it is not built)."""
+    global _bind
+    if _bind is not None:
+        return _bind
+    L = lib()
+    try:
+        from . import _vnx_bind
+    except ImportError as e:
+        raise RuntimeError(f"vnx binding not found in {_PKG_DIR} ({e}); build it with "
+                           "`python -m versenext_amd.build`") from e
+    with _lock:
+        if _bind is None:
+            _vnx_bind.init(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
+                L.vnx_kv_write, L.vnx_kv_read, L.vnx_tree_attn_q8_workspace, L.vnx_tree_attn_q8)))
+            _bind = _vnx_bind
+    return _bind
+
+
 def check(status: int, what: str = "vnx call") -> None:
     """Maps a vnx_status to the reference's error conventions
     (ValueError for arguments, RuntimeError for the device; speculative.py:188-196,

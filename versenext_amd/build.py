@@ -1,4 +1,5 @@
-"""Builds libvnx_hip.so (all HIP sources under csrc/) in-tree for gfx950.
+"""Builds libvnx_hip.so (all HIP sources under csrc/, gfx950) and _vnx_bind.so
+(csrc/bind.cpp, the Python binding of its 8-bit KV cache entries) in-tree.
 
 Usage: python -m versenext_amd.build   (or versenext_amd.build.build_library())
 """
@@ -14,6 +15,7 @@ PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_NAME = "libvnx_hip.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
+BIND_PATH = os.path.join(PKG_DIR, "_vnx_bind.so")
 OBJ_DIR = os.path.join(PKG_DIR, "_build")
 
 ARCH = "gfx950"
@@ -45,8 +47,30 @@ def sources() -> list[str]:
     return sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".hip"))
 
 
+def build_bind(verbose: bool = False) -> str:
+    """Compiles csrc/bind.cpp against this Python and PyTorch into BIND_PATH."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+    inc = [f"-isystem{d}" for d in cpp_extension.include_paths()] + [f"-I{sysconfig.get_paths()['include']}"]
+    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    tmp = BIND_PATH + ".tmp"
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *inc, os.path.join(CSRC, "bind.cpp"),
+           "-o", tmp, f"-L{lib}", f"-Wl,-rpath,{lib}", "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"the binding did not compile:\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, BIND_PATH)
+    return BIND_PATH
+
+
 def build_library(verbose: bool = False, jobs: int | None = None) -> str:
-    """Compiles every csrc/*.hip for gfx950 and links LIB_PATH. Returns the path."""
+    """Compiles every csrc/*.hip for gfx950 and links LIB_PATH, and the Python
+    binding beside it (build_bind). Returns LIB_PATH."""
     hipcc = _hipcc()
     os.makedirs(OBJ_DIR, exist_ok=True)
     srcs = sources()
@@ -63,10 +87,12 @@ def build_library(verbose: bool = False, jobs: int | None = None) -> str:
         return res.stderr
 
     jobs = jobs or min(8, os.cpu_count() or 1, len(srcs))
-    with ThreadPoolExecutor(max_workers=jobs) as ex:
+    with ThreadPoolExecutor(max_workers=jobs + 1) as ex:
+        bind = ex.submit(build_bind, verbose)
         for warn in ex.map(compile_one, zip(srcs, objs)):
             if verbose and warn:
                 print(warn, file=sys.stderr)
+        bind.result()
     tmp = LIB_PATH + ".tmp"
     cmd = [hipcc, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp, *objs]
     res = subprocess.run(cmd, capture_output=True, text=True)

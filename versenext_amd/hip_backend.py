@@ -63,6 +63,7 @@ class HipBackend(DeviceBackend):
         with torch.cuda.device(idx):
             _lib.check(L.vnx_init(idx), "vnx_init")
         self._L = L
+        self._bind = _lib.bind()
         self._ws = {}
         self._ws_lock = threading.Lock()
 
@@ -715,6 +716,13 @@ class HipBackend(DeviceBackend):
         t = t.contiguous()
         return t.clone() if t.data_ptr() % 16 else t
 
+    @staticmethod
+    def _bound(r, what: str):
+        """A result of the binding: tensors, or the C entry's status."""
+        if type(r) is int:
+            _lib.check(r, what)
+        return r
+
     _KV_DTYPES = (torch.int8, torch.float8_e4m3fn, torch.bfloat16)
 
     def kv_write(self, qkv, k_cache, v_cache, lens, k_scale=None, v_scale=None, cos=None, sin=None, q_norm=None,
@@ -729,6 +737,10 @@ class HipBackend(DeviceBackend):
         rotate queries and keys; q_norm / k_norm (d,) norm every query / key
         head before that.  Positions outside the cache (or the tables) are
         skipped and their queries zero."""
+        r = self._bind.kv_write(self._index, self._stream(), k_cache, v_cache, k_scale, v_scale, qkv, lens, cos, sin,
+                                q_norm, k_norm, eps)
+        if r is not None:      # (None: a call that needs the conversions or the errors below)
+            return self._bound(r, "kv_write")
         B, Hkv, cap, d, code, ss = self._kv_cache(k_cache, v_cache, k_scale, v_scale, self._KV_DTYPES)
         x = _to_tensor(qkv, self._torch_device).resolve_neg()
         if x.dtype not in _lib.DTYPE_CODES:
@@ -763,6 +775,9 @@ class HipBackend(DeviceBackend):
         float16): what rows start[b] .. start[b] + rows - 1 of a cache as
         kv_write fills it stand for (vnx_kv_read); start None: from row 0,
         rows None: cap of them.  Rows outside the cache are zeros."""
+        r = self._bind.kv_read(self._index, self._stream(), k_cache, v_cache, k_scale, v_scale, start, rows, out_dtype)
+        if r is not None:
+            return self._bound(r, "kv_read")
         B, Hkv, cap, d, code, ss = self._kv_cache(k_cache, v_cache, k_scale, v_scale, self._KV_DTYPES)
         if out_dtype not in _lib.DTYPE_CODES:
             raise ValueError("out_dtype must be torch.float32, torch.bfloat16 or torch.float16")
@@ -793,6 +808,10 @@ class HipBackend(DeviceBackend):
         it), from which the launch is sized.  Returns (B, H, N, d) bfloat16 or
         float16, written into `out` (any strides with unit last stride) when
         given."""
+        r = self._bind.tree_attn_q8(self._index, self._stream(), k_cache, v_cache, k_scale, v_scale, q, lens, anc,
+                                    scale, seg2, gates, window, max_len, out_dtype, out)
+        if r is not None:
+            return self._bound(r, "tree_attention_q8")
         dev = self._torch_device
         B, Hkv, cap, d, code, ss = self._kv_cache(k_cache, v_cache, k_scale, v_scale, self._KV_DTYPES[:2])
         qt = self._heads_bf16(q, "q")
