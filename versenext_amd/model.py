@@ -39,6 +39,10 @@ Kernels of libvnx_hip.so (gfx950) on the decode and verify forwards:
   (vnx_mod_route_x) and the routed expert products (vnx_expert_gemm_bf16);
 - the INT4 group-128 draft GEMVs (vnx_gemv_w4 and its fused RMSNorm / RoPE /
   SwiGLU / residual forms) and the verify-pass LM head (vnx_gemm_bf16).
+With kv_dtype (int8 or e4m3) the caches hold 8-bit codes and a scale a row and
+head: vnx_kv_write rotates, quantises and writes the new rows, vnx_tree_attn_q8
+attends over them (chunks of any length; vnx_kv_read and PyTorch where it does
+not apply).
 Prefill-size forwards (more rows than one verify round) take the same calls
 with the norms apart (vnx_rmsnorm) and, for the MoD layers, the row lists
 built first (vnx_mod_lists, vnx_expert_gemm_bf16_rows); INT4 models run their
@@ -597,10 +601,21 @@ class CometSparkGPU:
     sequence at positions lens[b] .. lens[b]+n-1, writes their keys / values
     into the cache there and returns the final-norm hidden states (B, n, D)
     fp32.  Committing a verify result is `lens += accepted + 1` (the rest of
-    the written rows is overwritten by the next call)."""
+    the written rows is overwritten by the next call).
+
+    kv_dtype torch.int8 or torch.float8_e4m3fn: the cache in 8 bits (half its
+    bytes, to hold and to read; heads of 16 to 256, a power of two; dtype
+    bfloat16).  None: in dtype."""
 
     def __init__(self, cfg: ModelConfig, weights: Dict[str, torch.Tensor], hip, batch: int, capacity: int,
-                 dtype=torch.bfloat16, int4: bool = False):
+                 dtype=torch.bfloat16, int4: bool = False, kv_dtype: Optional[torch.dtype] = None):
+        if kv_dtype is not None:
+            if kv_dtype not in (torch.int8, torch.float8_e4m3fn):
+                raise ValueError(f"kv_dtype must be torch.int8 or torch.float8_e4m3fn, got {kv_dtype}")
+            hd = cfg.head_dim
+            if dtype != torch.bfloat16 or not 16 <= hd <= 256 or hd & (hd - 1):
+                raise ValueError("a cache in 8 bits needs dtype bfloat16 and heads of 16, 32, 64, 128 or 256")
+        self.kv_dtype = kv_dtype
         self.cfg = cfg
         self.hip = hip
         self.dev = hip.torch_device
@@ -695,8 +710,13 @@ class CometSparkGPU:
         self.sin = torch.from_numpy(sin).to(dev)
         self.slopes = torch.from_numpy(alibi_slopes(cfg.n_head)).to(dev)
         Hkv = cfg.n_kv_head
-        self.kc = [torch.zeros((self.B, Hkv, self.cap, d), dtype=dtype, device=dev) for _ in self.layers]
-        self.vc = [torch.zeros((self.B, Hkv, self.cap, d), dtype=dtype, device=dev) for _ in self.layers]
+        kvt = kv_dtype or dtype
+        self.kc = [torch.zeros((self.B, Hkv, self.cap, d), dtype=kvt, device=dev) for _ in self.layers]
+        self.vc = [torch.zeros((self.B, Hkv, self.cap, d), dtype=kvt, device=dev) for _ in self.layers]
+        # the rows' scales (8-bit caches)
+        sc = self.layers if kv_dtype is not None else ()
+        self.ks = [torch.zeros((self.B, Hkv, self.cap), dtype=torch.float32, device=dev) for _ in sc]
+        self.vs = [torch.zeros((self.B, Hkv, self.cap), dtype=torch.float32, device=dev) for _ in sc]
         self._words = {}
         self.cus = torch.cuda.get_device_properties(dev).multi_processor_count
         self._neg = torch.full((), -1e9, dtype=torch.float32, device=dev)  # the reference's mask value
@@ -705,6 +725,8 @@ class CometSparkGPU:
         # 32 (chunks of any length)
         self.f32_rows = dtype == torch.float32 and d in (8, 16, 32)
         self.kernel_attention = (dtype == torch.bfloat16 and d in (64, 128)) or self.f32_rows
+        # vnx_tree_attn_q8: the window and the global rows, no ALiBi
+        self.kernel_q8 = kv_dtype is not None and d in (64, 128) and not cfg.use_alibi
         # dtype of the activations fed to the projections: fp16 for the INT4
         # GEMVs, else the compute dtype
         self.act_dtype = torch.float16 if int4 else dtype
@@ -715,7 +737,8 @@ class CometSparkGPU:
 
     @classmethod
     def from_vn(cls, path: str, hip, batch: int, capacity: int, dtype=torch.bfloat16, int4: bool = True,
-                chunk_bytes: int = 64 << 20, cfg: Optional[ModelConfig] = None) -> "CometSparkGPU":
+                chunk_bytes: int = 64 << 20, cfg: Optional[ModelConfig] = None,
+                kv_dtype: Optional[torch.dtype] = None) -> "CometSparkGPU":
         """The model saved in a .vn file (CometSparkNexLM.save_vn /
         CometSparkV05LM.save_vn, cometspark.py:1014-1060; loaded by the
         reference through VNFileReader, spark/mate/model/model.py:271-285),
@@ -735,7 +758,7 @@ class CometSparkGPU:
                                 chunk_bytes=chunk_bytes, skip=lambda n: tied and n == "head.weight")
         if cfg is None:
             cfg = config_from_vn(conf, W, name=f"{path} (.vn)")
-        return cls(cfg, W, hip, batch, capacity, dtype, int4)
+        return cls(cfg, W, hip, batch, capacity, dtype, int4, kv_dtype)
 
     # ---- pieces ---------------------------------------------------------
     def _st(self) -> int:
@@ -817,6 +840,19 @@ class CometSparkGPU:
                         True, o, seg2=(Ly.gk, Ly.gv), gates=Ly.gates, qkv=qkv)
         return o
 
+    def _attn_q8(self, q, li, lens, n, Tmax):
+        """Both paths over an 8-bit cache that already holds the n new rows
+        (vnx_tree_attn_q8, any n).  q (B, H, n, d) bf16."""
+        cfg = self.cfg
+        B, H, d = self.B, cfg.n_head, cfg.head_dim
+        Ly = self.layers[li]
+        o = torch.empty((B * n, H * d), dtype=self.act_dtype, device=self.dev)
+        self.hip.tree_attention_q8(q, self.kc[li], self.vc[li], self.ks[li], self.vs[li], lens,
+                                   seg2=(Ly.gk, Ly.gv) if Ly.gk.shape[2] else None, gates=Ly.gates,
+                                   window=cfg.window_size, max_len=Tmax,
+                                   out=o.view(B, n, H, d).permute(0, 2, 1, 3))   # the proj input layout
+        return o
+
     def _attn_long(self, q, li, lens, n, Tmax):
         """bf16 forwards of more rows than one vnx_tree_attn call takes
         (prefill); the cache already holds the n new rows.  q (B, H, n, d)."""
@@ -879,8 +915,12 @@ class CometSparkGPU:
         B, H, _, d = q.shape
         rep = H // cfg.n_kv_head
         Tk = Tmax + n
-        k = self.kc[li][:, :, :Tk].float().repeat_interleave(rep, dim=1)
-        v = self.vc[li][:, :, :Tk].float().repeat_interleave(rep, dim=1)
+        if self.kv_dtype is not None:
+            k, v = self.hip.kv_read(self.kc[li], self.vc[li], self.ks[li], self.vs[li], rows=Tk,
+                                    out_dtype=torch.float32)
+        else:
+            k, v = self.kc[li][:, :, :Tk].float(), self.vc[li][:, :, :Tk].float()
+        k, v = k.repeat_interleave(rep, dim=1), v.repeat_interleave(rep, dim=1)
         qf = q.float()
         scale = 1.0 / math.sqrt(d)
         scores = torch.matmul(qf, k.transpose(-1, -2).contiguous()) * scale        # (B, H, n, Tk)
@@ -1061,9 +1101,10 @@ class CometSparkGPU:
             x = (self.emb[tok].float() * self.emb_scale).contiguous()
         else:
             x = torch.empty((M, D), dtype=torch.float32, device=self.dev)                # fp32 residual stream
-        use_kernel = self.kernel_attention and (self.f32_rows or (n <= 64 and n <= cfg.window_size))
+        kv8 = self.kv_dtype is not None
+        use_kernel = self.kernel_attention and not kv8 and (self.f32_rows or (n <= 64 and n <= cfg.window_size))
         # longer bf16 forwards (prefill)
-        long = self.kernel_attention and not use_kernel
+        long = self.kernel_attention and not kv8 and not use_kernel
         pending = None
         for li, L in enumerate(self.layers):
             # bf16 forwards: the residual adds live in the projections
@@ -1084,13 +1125,14 @@ class CometSparkGPU:
                       and pending is None)
             h = None
             qkv = None
-            q = torch.empty((B, H, n, d), dtype=self.dtype, device=self.dev)
             kc, vc = self.kc[li], self.vc[li]
-            rk = _lib.RopeKvArgs(P(lens.data_ptr()), n, H, Hkv, d, P(self.cos.data_ptr()), P(self.sin.data_ptr()),
-                                 self.cos.shape[0], int(cfg.use_rope), P(q.data_ptr()), P(kc.data_ptr()),
-                                 P(vc.data_ptr()), kc.stride(0), kc.stride(1), kc.stride(2), self.cap)
+            if not kv8:
+                q = torch.empty((B, H, n, d), dtype=self.dtype, device=self.dev)
+                rk = _lib.RopeKvArgs(P(lens.data_ptr()), n, H, Hkv, d, P(self.cos.data_ptr()), P(self.sin.data_ptr()),
+                                     self.cos.shape[0], int(cfg.use_rope), P(q.data_ptr()), P(kc.data_ptr()),
+                                     P(vc.data_ptr()), kc.stride(0), kc.stride(1), kc.stride(2), self.cap)
             done = False                                   # q and the cache rows written
-            if li == 0 and qfused and self.embed_fold and L.wqkv.rope_kv_embed(
+            if li == 0 and qfused and not kv8 and self.embed_fold and L.wqkv.rope_kv_embed(
                     tok, self.emb, self.emb_scale, x, rk, L.norm1, cfg.eps):
                 done = True                                # embedding, norm, q|k|v, RoPE, cache rows: one call
             elif li == 0 and norm_in and self.embed_fold and (qkv := L.wqkv.gemm_norm_embed(
@@ -1101,13 +1143,13 @@ class CometSparkGPU:
                 self._embed_rms(tok, L.norm1, x, h)        # token embedding folded into the first norm
             elif norm_in:
                 qkv = L.wqkv.gemm_norm(x, L.norm1, cfg.eps)
-            elif qfused:
+            elif qfused and not kv8:
                 done = L.wqkv.rope_kv(x, rk, L.norm1, cfg.eps)
             else:
                 h = torch.empty((M, D), dtype=self.act_dtype, device=self.dev)
                 self._rms(x, pending, L.norm1, h)
                 pending = None
-            if not done and qkv is None:
+            if not done and qkv is None and not kv8:
                 done = L.wqkv.rope_kv(h, rk)               # INT4: projection with RoPE + cache write fused
             attn_qkv = None
             if not done:
@@ -1116,7 +1158,10 @@ class CometSparkGPU:
                 if use_kernel and qkv.dtype == torch.bfloat16 and qkv.stride(1) == 1:
                     attn_qkv = qkv                         # RoPE + cache write inside the attention call
                     done = True
-            if not done:
+            if kv8:                                        # RoPE, the rows quantised into the cache
+                q = self.hip.kv_write(qkv.view(B, n, -1), kc, vc, lens, self.ks[li], self.vs[li],
+                                      cos=self.cos if cfg.use_rope else None, sin=self.sin if cfg.use_rope else None)
+            elif not done:
                 _lib.check(L_.vnx_rope_kv(
                     P(qkv.data_ptr()), _lib.DTYPE_CODES[qkv.dtype], qkv.stride(0), B, n, H, Hkv, d,
                     P(lens.data_ptr()), P(self.cos.data_ptr()), P(self.sin.data_ptr()), self.cos.shape[0],
@@ -1125,7 +1170,9 @@ class CometSparkGPU:
                     "rope_kv")
             if cache_only and attn_qkv is None and li == len(self.layers) - 1:
                 return None                                # every layer's new cache rows are written
-            if use_kernel:
+            if self.kernel_q8:
+                o = self._attn_q8(q, li, lens, n, Tmax)
+            elif use_kernel:
                 o = self._attn_kernel(q, li, lens, n, Tmax, qkv=attn_qkv)
             elif long:
                 o = self._attn_long(q, li, lens, n, Tmax)
