@@ -135,7 +135,8 @@ __device__ __forceinline__ void q8_scales(const float* s, int k0, int left, int 
 }
 
 // The loaded rows of one step of 32 keys from k0 on, `left` of them to be read.
-template <int D, int KT>
+// AUX 2: past the caches (rows that nobody reads again).
+template <int D, int KT, int AUX>
 struct Q8Keys {
   static constexpr int E = KT == KV_BF16 ? 2 : 1;
   static constexpr int W = D / 64 * E;  // 16-byte loads a key tile
@@ -151,7 +152,7 @@ struct Q8Keys {
 #pragma unroll
       for (int i = 0; i < W; ++i)
         k[t][i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
-            rs, o + (E == 1 ? 64 * i : 128 * (i / 2) + 16 * (i % 2)), 16 * t * (int)s.sr, 0));
+            rs, o + (E == 1 ? 64 * i : 128 * (i / 2) + 16 * (i % 2)), 16 * t * (int)s.sr, AUX));
     if constexpr (KT != KV_BF16) q8_scales(s.ks, k0, left, g, sk);
   }
 
@@ -183,7 +184,7 @@ struct Q8Keys {
   }
 };
 
-template <int D, int KT>
+template <int D, int KT, int AUX>
 struct Q8Vals {
   static constexpr int E = KT == KV_BF16 ? 2 : 1;
   static constexpr int W = D / 64 * E;  // words of a key's values a lane
@@ -198,12 +199,12 @@ struct Q8Vals {
     for (int j = 0; j < 8; ++j) {
       const int so = ((j < 4 ? 0 : 16) + (j & 3)) * (int)s.sr;
       if constexpr (W == 1) {
-        v[j][0] = __builtin_amdgcn_raw_buffer_load_b32(rs, o, so, 0);
+        v[j][0] = __builtin_amdgcn_raw_buffer_load_b32(rs, o, so, AUX);
       } else if constexpr (W == 2) {
-        const auto w = __builtin_amdgcn_raw_buffer_load_b64(rs, o, so, 0);
+        const auto w = __builtin_amdgcn_raw_buffer_load_b64(rs, o, so, AUX);
         v[j][0] = w[0]; v[j][1] = w[1];
       } else {
-        const auto w = __builtin_amdgcn_raw_buffer_load_b128(rs, o, so, 0);
+        const auto w = __builtin_amdgcn_raw_buffer_load_b128(rs, o, so, AUX);
         v[j][0] = w[0]; v[j][1] = w[1]; v[j][2] = w[2]; v[j][3] = w[3];
       }
     }
@@ -324,13 +325,13 @@ struct Q8State {
 // softmax into st.  Codes: P sv / R in fp16 (2^-11), R the largest sv so far times 2^-6: P <= 2^8
 // and sv / R <= 2^7 stay in range, and a term keeps its 11 bits down to 2^-21 of
 // the largest row's scale (below: 2^-32 of it).  bf16 rows: P in two bf16 parts.
-template <int D, int KT, int CT, int KIND>
+template <int D, int KT, int CT, int KIND, int AUX = 0>
 __device__ __forceinline__ void q8_walk(const Q8Src& src, int first, int s0, int ds, int s1, const Q8Mask<CT>& mk,
                                         float c, const bf16x8 (&qf)[CT][D / 32], Q8State<CT, D>& st, int lane) {
   if (s0 >= s1) return;
   const int g4 = (lane >> 4) * 4;
-  Q8Keys<D, KT> keys;
-  Q8Vals<D, KT> vals;
+  Q8Keys<D, KT, AUX> keys;
+  Q8Vals<D, KT, AUX> vals;
   auto left = [&](int s) { return s < s1 ? src.rows - (first + 32 * s) : 0; };
   float R = 0.0f, iR = __builtin_inff();
   keys.load(src, first + 32 * s0, left(s0), lane);
@@ -585,7 +586,7 @@ __device__ __forceinline__ int64_t q8_out_off(const Q8Params& p, int b, int kvh,
 // walks it beside the others, in the last split.  (us, 32 x 7 rows over 617,
 // 128 global rows: 7.8 with that wave, 10.1 walked first; 4 x 512 rows, KW = 2:
 // 18.1 walked first, 26 with the wave and KW = 4.)
-template <int D, int KT, int CT, int KIND, bool SEG2, int KW, int CW>
+template <int D, int KT, int CT, int KIND, bool SEG2, int KW, int CW, int AUX = 0>
 __global__ __launch_bounds__((KW * CW + (SEG2 && KW >= 4)) * 64, 2) void k_attn8(Q8Params p, Q8Words tw) {
   constexpr bool WAVE2 = SEG2 && KW >= 4, LDS2 = SEG2 && KW < 4;
   constexpr int NW = KW * CW + WAVE2, COLS = 16 * CT;
@@ -679,7 +680,7 @@ __global__ __launch_bounds__((KW * CW + (SEG2 && KW >= 4)) * 64, 2) void k_attn8
   const bool second = WAVE2 && split == p.splits - 1;
   if (!extra) {
     const int per = (t.steps + p.splits - 1) / p.splits;
-    q8_walk<D, KT, CT, KIND>(t.src, t.first, split * per + kw, KW, min(t.steps, (split + 1) * per), t.mask, p.c, t.qf,
+    q8_walk<D, KT, CT, KIND, AUX>(t.src, t.first, split * per + kw, KW, min(t.steps, (split + 1) * per), t.mask, p.c, t.qf,
                              st, lane);
   } else if (second) {
     q8_walk<D, KV_BF16, CT, Q8_ALL>(t.src2, 0, 0, 1, (p.T2 + 31) / 32, t.mask2(p.T2), p.c, t.qf, st, lane);
@@ -920,13 +921,24 @@ void q8_launch(const Q8Params& p, const Q8Words& tw, const Q8Plan& pl, hipStream
       return;
     }
   }
-  if constexpr (!SEG2) {  // (a ninth wave would leave 168 registers a lane)
-    if (pl.kw == 8) {
-      hipLaunchKernelGGL((k_attn8<D, KT, CT, KIND, SEG2, 8, 1>), grid, dim3(512), 0, st, p, tw);
-      return;
+  auto go = [&](auto aux) {
+    constexpr int AUX = decltype(aux)::value;
+    if constexpr (!SEG2) {  // (a ninth wave would leave 168 registers a lane)
+      if (pl.kw == 8) {
+        hipLaunchKernelGGL((k_attn8<D, KT, CT, KIND, SEG2, 8, 1, AUX>), grid, dim3(512), 0, st, p, tw);
+        return;
+      }
     }
+    hipLaunchKernelGGL((k_attn8<D, KT, CT, KIND, SEG2, 4, 1, AUX>), grid, dim3(256 + 64 * SEG2), 0, st, p, tw);
+  };
+  // Rows that one column group reads and no cache holds until the next call go
+  // past the caches (us, 8 x 5 rows over 16,000 keys, 240 MB: 57.7 / 54.3; re-read
+  // rows lose by it, 16 trees over 2,048 17.5 / 19.7).
+  const int64_t rows = p.window > 0 && p.window < p.Tp ? p.window : p.Tp;
+  if constexpr (CT <= 2) {
+    if (pl.groups == 1 && (int64_t)p.B * p.Hkv * rows * 2 * D >= (128 << 20)) return go(IntC<2>{});
   }
-  hipLaunchKernelGGL((k_attn8<D, KT, CT, KIND, SEG2, 4, 1>), grid, dim3(256 + 64 * SEG2), 0, st, p, tw);
+  go(IntC<0>{});
 }
 
 template <int D, int KT, int KIND, bool SEG2>

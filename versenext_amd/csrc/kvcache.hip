@@ -42,7 +42,9 @@ struct KvWriteParams {
   int64_t c_sb, c_sh, c_sr;  // elements
   int64_t s_sb, s_sh;
   int64_t cap;               // rows below cap (and the tables') are written
-  uint32_t slots;            // B * n * (H + 2 Hkv)
+  uint32_t tokens;           // B * n
+  int chunks, per;           // waves a token, head groups a wave
+  int past;                  // queries past the caches
   int n, H, Hkv;
   float eps;
 };
@@ -54,7 +56,7 @@ __device__ __forceinline__ void kv_ld8(const T* p, float (&v)[8]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
   } else {
-    const u32x4 a = *reinterpret_cast<const u32x4*>(p);
+    const u32x4 a = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));  // (read once)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if constexpr (__is_same(T, _Float16)) {
@@ -103,99 +105,120 @@ __device__ __forceinline__ uint2 kv_codes(const float (&v)[8], float r) {
   return make_uint2(w[0], w[1]);
 }
 
-// L = d / 16 lanes a head.
+// L = d / 16 lanes a head, a wave 64 / L heads of one token at a time, `per`
+// times: the tables' row is loaded once for all of them, the next heads' values
+// under the current ones' arithmetic.
 template <typename TS, int KT, int L>
 __global__ __launch_bounds__(256) void k_kv_write(KvWriteParams p) {
-  constexpr int D = 16 * L, HD = D / 2;
-  const uint32_t at = (uint32_t)blockIdx.x * (256 / L) + threadIdx.x / L;
-  const int lane = threadIdx.x % L;
-  if (at >= p.slots) return;  // whole heads leave together: the reductions below stay inside one
-  const int HT = p.H + 2 * p.Hkv;
-  const uint32_t tok = at / (uint32_t)HT;
-  const int head = (int)(at - tok * (uint32_t)HT);
+  constexpr int D = 16 * L, HD = D / 2, G = 64 / L;
+  const int lane = threadIdx.x % L, gi = threadIdx.x % 64 / L;
+  const uint32_t unit = (uint32_t)__builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+  const uint32_t tok = unit / (uint32_t)p.chunks;
+  if (tok >= p.tokens) return;
   const int b = (int)(tok / (uint32_t)p.n), i = (int)(tok - (uint32_t)b * (uint32_t)p.n);
   const int64_t pos = (int64_t)p.lens[b] + i;
   const bool in = pos >= 0 && pos < p.cap;
-  const bool is_q = head < p.H;
-  if (!in && !is_q) return;
-  const TS* src = static_cast<const TS*>(p.qkv) + (int64_t)tok * p.ldq + (int64_t)head * D + lane * 8;
-  float lo[8], hi[8];
-  kv_ld8(src, lo);
-  kv_ld8(src + HD, hi);
-  const bool is_v = head >= p.H + p.Hkv;
-  if (!is_v) {
-    const float* nw = is_q ? p.qn : p.kn;
-    if (nw) {
-      float ss = 0.0f;
+  const int HT = p.H + 2 * p.Hkv, HQK = p.H + p.Hkv;
+  const int h0 = (int)(unit - tok * (uint32_t)p.chunks) * p.per * G + gi;
+  const int h1 = min(HT, h0 - gi + p.per * G);
+  const TS* src = static_cast<const TS*>(p.qkv) + (int64_t)tok * p.ldq + lane * 8;
+  float nlo[8], nhi[8];
+  auto fetch = [&](int head) {
+    if (head < h1) {
+      kv_ld8(src + (int64_t)head * D, nlo);
+      kv_ld8(src + (int64_t)head * D + HD, nhi);
+    }
+  };
+  fetch(h0);
+  const bool turn = p.cos && in && h0 - gi < HQK;
+  float cl[8], ch[8], sl[8], sh[8];
+  if (turn) {
+    const float* c = p.cos + pos * D + lane * 8;
+    const float* s = p.sin + pos * D + lane * 8;
+    kv_ld8(c, cl);
+    kv_ld8(c + HD, ch);
+    kv_ld8(s, sl);
+    kv_ld8(s + HD, sh);
+  }
+  for (int head = h0; head < h1; head += G) {
+    float lo[8], hi[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) ss = fmaf(lo[e], lo[e], fmaf(hi[e], hi[e], ss));
+    for (int e = 0; e < 8; ++e) { lo[e] = nlo[e]; hi[e] = nhi[e]; }
+    fetch(head + G);
+    const bool is_q = head < p.H, is_v = head >= HQK;
+    if (!in && !is_q) continue;  // (a head's lanes go together: the reductions below stay inside one)
+    if (!is_v) {
+      const float* nw = is_q ? p.qn : p.kn;
+      if (nw) {
+        float ss = 0.0f;
 #pragma unroll
-      for (int off = L / 2; off > 0; off >>= 1) ss += __shfl_xor(ss, off, L);
-      const float r = 1.0f / sqrtf(ss * (1.0f / D) + p.eps);
-      float wl[8], wh[8];
-      kv_ld8(nw + lane * 8, wl);
-      kv_ld8(nw + HD + lane * 8, wh);
+        for (int e = 0; e < 8; ++e) ss = fmaf(lo[e], lo[e], fmaf(hi[e], hi[e], ss));
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        lo[e] = lo[e] * r * wl[e];
-        hi[e] = hi[e] * r * wh[e];
+        for (int off = L / 2; off > 0; off >>= 1) ss += __shfl_xor(ss, off, L);
+        const float r = 1.0f / sqrtf(ss * (1.0f / D) + p.eps);
+        float wl[8], wh[8];
+        kv_ld8(nw + lane * 8, wl);
+        kv_ld8(nw + HD + lane * 8, wh);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          lo[e] = lo[e] * r * wl[e];
+          hi[e] = hi[e] * r * wh[e];
+        }
+      }
+      if (turn) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float x = lo[e], y = hi[e];
+          lo[e] = x * cl[e] - y * sl[e];
+          hi[e] = y * ch[e] + x * sh[e];
+        }
       }
     }
-    if (p.cos && in) {
-      const float* c = p.cos + pos * D + lane * 8;
-      const float* s = p.sin + pos * D + lane * 8;
-      float cl[8], ch[8], sl[8], sh[8];
-      kv_ld8(c, cl);
-      kv_ld8(c + HD, ch);
-      kv_ld8(s, sl);
-      kv_ld8(s + HD, sh);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float x = lo[e], y = hi[e];
-        lo[e] = x * cl[e] - y * sl[e];
-        hi[e] = y * ch[e] + x * sh[e];
+    if (is_q) {
+      uint16_t* o = p.q + (((int64_t)b * p.H + head) * p.n + i) * D + lane * 8;
+      u32x4 x = kv_bf16x8(lo), y = kv_bf16x8(hi);
+      if (!in) x = y = u32x4{0, 0, 0, 0};  // a position outside the cache: zeros
+      if (p.past) {
+        __builtin_nontemporal_store(x, reinterpret_cast<u32x4*>(o));
+        __builtin_nontemporal_store(y, reinterpret_cast<u32x4*>(o + HD));
+      } else {
+        *reinterpret_cast<u32x4*>(o) = x;
+        *reinterpret_cast<u32x4*>(o + HD) = y;
       }
+      continue;
     }
-  }
-  if (is_q) {
-    uint16_t* o = p.q + (((int64_t)b * p.H + head) * p.n + i) * D + lane * 8;
-    u32x4 a = kv_bf16x8(lo), c = kv_bf16x8(hi);
-    if (!in) a = c = u32x4{0, 0, 0, 0};  // a position outside the cache: zeros
-    *reinterpret_cast<u32x4*>(o) = a;
-    *reinterpret_cast<u32x4*>(o + HD) = c;
-    return;
-  }
-  const int kvh = head - p.H - (is_v ? p.Hkv : 0);
-  char* cache = is_v ? p.vc : p.kc;
-  const int64_t off = (int64_t)b * p.c_sb + (int64_t)kvh * p.c_sh + pos * p.c_sr + lane * 8;
-  if constexpr (KT == KV_BF16) {
-    uint16_t* o = reinterpret_cast<uint16_t*>(cache) + off;
-    *reinterpret_cast<u32x4*>(o) = kv_bf16x8(lo);
-    *reinterpret_cast<u32x4*>(o + HD) = kv_bf16x8(hi);
-  } else {
-    // the maximum of the magnitudes' bit patterns: NaN above infinity above
-    // every number, so one test finds a row that has either
-    uint32_t am = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      am = max(am, __float_as_uint(lo[e]) & 0x7FFFFFFFu);
-      am = max(am, __float_as_uint(hi[e]) & 0x7FFFFFFFu);
-    }
-#pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) am = max(am, (uint32_t)__shfl_xor((int)am, o, L));
-    constexpr float top = KT == KV_I8 ? 127.0f : 448.0f;
-    const float amax = __uint_as_float(am);
-    float r = 0.0f, s = am >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : 0.0f;
-    if (am < 0x7F800000u && amax >= kKvTiny) {
-      r = top / amax;
-      s = amax / top;
+    const int kvh = head - p.H - (is_v ? p.Hkv : 0);
+    char* cache = is_v ? p.vc : p.kc;
+    const int64_t off = (int64_t)b * p.c_sb + (int64_t)kvh * p.c_sh + pos * p.c_sr + lane * 8;
+    if constexpr (KT == KV_BF16) {
+      uint16_t* o = reinterpret_cast<uint16_t*>(cache) + off;
+      *reinterpret_cast<u32x4*>(o) = kv_bf16x8(lo);
+      *reinterpret_cast<u32x4*>(o + HD) = kv_bf16x8(hi);
     } else {
+      // the maximum of the magnitudes' bit patterns: NaN above infinity above
+      // every number, so one test finds a row that has either
+      uint32_t am = 0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) lo[e] = hi[e] = 0.0f;  // not x * 0: -0, or NaN
+      for (int e = 0; e < 8; ++e) {
+        am = max(am, __float_as_uint(lo[e]) & 0x7FFFFFFFu);
+        am = max(am, __float_as_uint(hi[e]) & 0x7FFFFFFFu);
+      }
+#pragma unroll
+      for (int o = L / 2; o > 0; o >>= 1) am = max(am, (uint32_t)__shfl_xor((int)am, o, L));
+      constexpr float top = KT == KV_I8 ? 127.0f : 448.0f;
+      const float amax = __uint_as_float(am);
+      float r = 0.0f, s = am >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : 0.0f;
+      if (am < 0x7F800000u && amax >= kKvTiny) {
+        r = top / amax;
+        s = amax / top;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) lo[e] = hi[e] = 0.0f;  // not x * 0: -0, or NaN
+      }
+      *reinterpret_cast<uint2*>(cache + off) = kv_codes<KT>(lo, r);
+      *reinterpret_cast<uint2*>(cache + off + HD) = kv_codes<KT>(hi, r);
+      if (lane == 0) (is_v ? p.vs : p.ks)[(int64_t)b * p.s_sb + (int64_t)kvh * p.s_sh + pos] = s;
     }
-    *reinterpret_cast<uint2*>(cache + off) = kv_codes<KT>(lo, r);
-    *reinterpret_cast<uint2*>(cache + off + HD) = kv_codes<KT>(hi, r);
-    if (lane == 0) (is_v ? p.vs : p.ks)[(int64_t)b * p.s_sb + (int64_t)kvh * p.s_sh + pos] = s;
   }
 }
 
@@ -268,10 +291,17 @@ inline bool strides16(const int64_t* s, int64_t bytes) {
 }
 
 template <typename TS, int KT>
-int kv_write_launch(const KvWriteParams& p, int d, hipStream_t st) {
+int kv_write_launch(KvWriteParams p, int d, hipStream_t st) {
   return by_lanes<1, 16>(d / 16, [&](auto l) {
     constexpr int L = decltype(l)::value;
-    const unsigned grid = (unsigned)(((int64_t)p.slots + 256 / L - 1) / (256 / L));
+    // a wave a head group while that leaves the chip room (16 waves a CU), else a
+    // token's all (us, 16,384 tokens x 48 heads of 128 with norms: 83 / 81).
+    // Queries that no cache will hold until they are read go past it (81 / 77).
+    const int groups = (p.H + 2 * p.Hkv + 64 / L - 1) / (64 / L);
+    p.per = (int64_t)p.tokens * groups <= 16 * (int64_t)device_cus() ? 1 : groups;
+    p.chunks = (groups + p.per - 1) / p.per;
+    p.past = (int64_t)p.tokens * p.H * d * 2 >= (64 << 20);
+    const unsigned grid = (unsigned)(((int64_t)p.tokens * p.chunks + 3) / 4);
     hipLaunchKernelGGL((k_kv_write<TS, KT, L>), dim3(grid), dim3(256), 0, st, p);
     VNX_LAUNCH_CHECK();
     return (int)VNX_OK;
@@ -325,7 +355,7 @@ int vnx_kv_write(const vnx_kv_write_args* a, void* stream) {
   p.c_sb = a->cache_strides[0]; p.c_sh = a->cache_strides[1]; p.c_sr = a->cache_strides[2];
   p.s_sb = a->scale_strides[0]; p.s_sh = a->scale_strides[1];
   p.cap = a->cos_table && a->table_rows < a->cap ? a->table_rows : a->cap;
-  p.slots = (uint32_t)(a->B * a->n * HT);
+  p.tokens = (uint32_t)(a->B * a->n);
   p.n = a->n; p.H = a->H; p.Hkv = a->Hkv; p.eps = a->eps;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (a->dtype == VNX_F32) return kv_write_cache<float>(p, a->cache_dtype, a->d, st);
