@@ -14,7 +14,7 @@
 // query head kvh * rep + c % rep, so heads that share K and V share every
 // loaded row) and walks keys 32 at a time.  No row passes through LDS: each
 // operand is loaded in the order in which the matrix core wants it.
-//   S^T[key][col]    A = K: a lane holds 16 consecutive bytes of key lane % 16
+//   S^T[key][col]    A = K: a lane holds D / 4 consecutive bytes of key lane % 16
 //                    (the order of d inside a product is free, q is loaded
 //                    the same way);
 //   O^T[dim][col]    A = V^T: a lane holds D / 16 consecutive bytes of each of
@@ -146,13 +146,13 @@ struct Q8Keys {
   __device__ __forceinline__ void load(const Q8Src& s, int k0, int left, int lane) {
     const int m = lane & 15, g = lane >> 4;
     const auto rs = q8_buffer<D * E>(s.k + (int64_t)k0 * s.sr, s.sr, left);
-    const int o = m * (int)s.sr + g * (16 * E);
+    const int o = m * (int)s.sr + g * (D / 4 * E);
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int i = 0; i < W; ++i)
         k[t][i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
-            rs, o + (E == 1 ? 64 * i : 128 * (i / 2) + 16 * (i % 2)), 16 * t * (int)s.sr, AUX));
+            rs, o + 16 * i, 16 * t * (int)s.sr, AUX));
     if constexpr (KT != KV_BF16) q8_scales(s.ks, k0, left, g, sk);
   }
 
@@ -522,7 +522,7 @@ struct Q8Tile {
       const uint16_t* q = p.q + b * p.q_sb + (int64_t)(kvh * p.rep + h) * p.q_sh + (int64_t)node * p.q_sr;
 #pragma unroll
       for (int i = 0; i < D / 32; ++i)
-        qf[ct][i] = *reinterpret_cast<const bf16x8*>(q + 64 * (i / 2) + 16 * g + 8 * (i % 2));
+        qf[ct][i] = *reinterpret_cast<const bf16x8*>(q + D / 4 * g + 8 * i);
       mask.node[ct] = node;
     }
     const int64_t kv = b * p.c_sb + kvh * p.c_sh, ss = b * p.s_sb + kvh * p.s_sh;
@@ -795,46 +795,49 @@ struct Q8Plan {
 // Waves that share a workgroup's columns, per keys wave.
 constexpr int q8_cw(int kw) { return kw == 1 ? 4 : kw == 2 ? 2 : 1; }
 
-// Estimated us of a launch shape, for comparing shapes.  A wave's step costs
-// the conversion of its rows and its columns' softmax; a SIMD issues for two
-// waves at once what one wave issues in half the slots (one instruction a
-// wave in 8 cycles, measured), so a step's share of the chip shrinks with
-// the waves beside it until both slots are taken; rows read by several column
-// groups cost HBM and L2 time again; splits cost a second launch and their
-// partials.  The constants are fitted to 1,700 timings of 70 shapes (1-64
-// sequences, 1-2,048 new rows, 1-16,000 keys, both head sizes): the shape
-// picked is the fastest of them within 3% on average and 21% at worst.
-// us, 16 trees of 40 nodes over 2,048 rows: ct 3 x 8 waves 18.8, ct 1 x 4 waves 23.5;
-// 4 prompts of 512: ct 2 x 2 waves 18.1, ct 4 x 4 waves 24.6; 8 x 5 rows over 16,000,
-// heads of 128: ct 2 x 4 splits 55.6, no split 139, ct 1 x 4 splits 76.
-float q8_cost(int BH, int tiles, int d2, float last, float mean, float mem, int T2, int cus, int ct, int kw, int S,
+// Estimated us of a launch shape, for comparing shapes.  A step of a wave costs
+// the conversion of its rows and its columns' softmax: kCol a column tile in a
+// lone wave; per SIMD half of it, a wave issuing one instruction in 8 cycles and
+// a SIMD one in 4 (measured), and there the conversions count (in column
+// tiles, kConv).  Rows read by several column groups cost memory time again.  A
+// second launch joins splits.  The constants are fitted to 1,700 timings of 70
+// shapes (1-64 sequences, 1-1,500 new rows, 1-16,000 keys, both head sizes); of 67
+// others it picks the fastest launch shape within 2% on average and 21% at
+// worst.  us, 16 trees of 40 nodes over 2,048 rows: ct 3 x 8 waves 18.8, ct 1 x 4
+// waves 23.5; 4 prompts of 512: ct 2 x 2 waves 18.1, ct 4 x 4 waves 24.6; 8 x 5 rows
+// over 16,000, heads of 128: ct 2 x 4 splits 55.6, no split 139, ct 1 x 4 splits 76.
+float q8_cost(int BH, int d2, bool i8, float last, float mean, float mem, int T2, int cus, int ct, int kw, int S,
               int groups) {
-  constexpr float kMerge = 0.571f, kJoin = 1.0f, kPart = 8.249e-3f, kStep = 0.205f, kConv = 0.284f, kCol = 0.252f,
-                  kSeg2 = 0.219f, kWide = 3.43f, kLone = 2.836f, kRound = 6.258f, kAgain = 1.709f;
+  constexpr float kMerge = 0.813f, kLone = 1.66f, kJoin = 1.09f, kPart = 5.9e-3f, kStep = 0.078f, kCol = 0.252f,
+                  kSeg2 = 1.32f, kEight = 3.7f, kRound = 7.0f, kAgain = 2.07f;
+  const float kConv = i8 ? 3.35f : 2.26f;
   const int cw = q8_cw(kw);
-  const float v = kCol * (kConv * d2 + ct * (1.0f + 0.3f * (d2 - 1)));
+  const float cols = ct * (1.0f + 0.3f * (d2 - 1));
   const int occ = d2 == 1 ? (ct == 1 ? 4 : ct == 2 ? 3 : 2) : 2;  // waves a SIMD has registers for
   const int waves = kw * cw + (T2 > 0 && kw >= 4);
   const int per = occ * 4 / waves > 1 ? occ * 4 / waves : 1;      // workgroups a CU
   const float wgs = (float)BH * groups * S, rounds = wgs / ((float)cus * per);
-  const float nl = __builtin_ceilf(__builtin_ceilf(last / 32) / (kw * S));
-  const float nm = mean / 32 > kw * S ? mean / 32 / (kw * S) : 1.0f;
-  const float here = wgs / cus < per ? wgs / cus : per;
-  const float busy = here * kw * cw / 4 > 2.0f ? here * kw * cw / 8 : 1.0f;
+  float nl = __builtin_ceilf(__builtin_ceilf(last / 32) / (kw * S));  // steps of the longest wave, of the mean one
+  float nm = mean / 32 > kw * S ? mean / 32 / (kw * S) : 1.0f;
+  if (T2 > 0 && kw < 4) {
+    const float e = __builtin_ceilf((float)T2 / 32 / kw);
+    nl += e;
+    nm += e;
+  }
+  const float simd = (wgs / cus < per ? wgs / cus : per) * kw * cw / 4;  // waves a SIMD at a time
+  const float lone = kCol * (0.284f * d2 + cols), all = nm * 0.25f * (kConv * d2 + cols) * simd / 2;
   float t;
   if (rounds <= 1.0f) {
-    const float one = nl * v, all = nm * v * busy;
-    t = nl * kStep + (one > all ? one : all);
+    t = nl * kStep + (nl * lone > all ? nl * lone : all);
   } else {
-    t = (nm * kStep + nm * v * busy) * (rounds < 2.5f ? __builtin_ceilf(rounds) : rounds + 0.3f);
+    t = (nm * kStep + (nm * lone > all ? nm * lone : all)) * (rounds < 2.5f ? __builtin_ceilf(rounds) : rounds + 0.3f);
     t += kRound * (__builtin_ceilf(rounds) - 1);
   }
-  t += (kw > 1 ? kMerge * ct * d2 : kLone) * busy * (rounds > 1.0f ? rounds : 1.0f) + (kw == 8 ? kWide : 0.0f);
-  const float m = mem * (1.0f + kAgain * (groups * cw - 1));
+  t += (kw > 1 ? kMerge * ct * d2 : kLone) * (simd > 2.0f ? simd / 2 : 1.0f) * (rounds > 1.0f ? rounds : 1.0f);
+  t += (kw == 8 ? kEight : 0.0f) + (T2 > 0 && kw < 4 ? kSeg2 : 0.0f);
+  const float m = mem * (1.0f + kAgain * (groups * cw < 4 ? groups * cw - 1 : 3));
   t = t > m ? t : m;
-  if (S > 1) t += kJoin + kPart * BH * groups * ct * S * d2;
-  if (T2 > 0 && kw < 4) t += kSeg2 * (1 + (T2 + 31) / 32 / kw);
-  return t;
+  return S > 1 ? t + kJoin + kPart * BH * groups * ct * S * d2 : t;
 }
 
 Q8Plan q8_plan(const vnx_attn_q8_args* a) {
@@ -843,7 +846,7 @@ Q8Plan q8_plan(const vnx_attn_q8_args* a) {
   const bool tree = a->anc || a->anc_host;
   const float W = a->window > 0 ? (float)a->window : 1e9f, keys = (float)a->Tp + a->N;
   const int cus = device_cus();
-  // HBM time of the rows once, at 10 TB/s (the fit's way to say that it overlaps)
+  // memory time of the rows once, us (the rate is the fit's)
   const float mem = BH * (keys < W + a->N ? keys : W + a->N) * 2 * (a->d + 4) / 10.2e6f;
   Q8Plan best{1, 4, tiles, 1};
   float least = 1e30f;
@@ -858,7 +861,7 @@ Q8Plan q8_plan(const vnx_attn_q8_args* a) {
       const int groups = (tiles + ct * q8_cw(kw) - 1) / (ct * q8_cw(kw));
       for (int S = 1; S <= (kw < 4 ? 1 : kQ8Split); S *= 2) {
         if (S > 1 && ((int64_t)BH * groups * S > 6 * cus || last < 32 * S)) break;
-        const float t = q8_cost(BH, tiles, d2, last, mean, mem, a->T2, cus, ct, kw, S, groups);
+        const float t = q8_cost(BH, d2, a->kv_dtype == VNX_I8, last, mean, mem, a->T2, cus, ct, kw, S, groups);
         if (t < least) {
           least = t;
           best = {ct, kw, groups, S};
