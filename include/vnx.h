@@ -879,7 +879,8 @@ int vnx_expert_gemm_bf16_rows(const void* x, int64_t ldx, int64_t sxb, const voi
  *     lens[b] + i, cache_dtype VNX_I8, VNX_E4M3 or VNX_BF16 (the values rounded;
  *     k_scale / v_scale not used).
  * Positions outside [0, cap) (and the tables) are skipped, their q_out rows
- * zero.  d in {16, 32, 64, 128, 256}; pointers 16-byte aligned, ldq and strides
+ * zero.  Batch rows and heads of the cache must not overlap (a stride 0 is
+ * refused; reading takes it).  d in {16, 32, 64, 128, 256}; pointers 16-byte aligned, ldq and strides
  * multiples of 16 bytes.
  * ------------------------------------------------------------------------- */
 typedef struct vnx_kv_write_args {

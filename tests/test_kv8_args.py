@@ -55,6 +55,8 @@ INVALID, UNSUPPORTED = _lib.VNX_ERR_INVALID_ARG, _lib.VNX_ERR_UNSUPPORTED
     (INVALID, dict(eps=-1.0)), (INVALID, dict(eps=float("nan"))), (INVALID, dict(n=0)), (INVALID, dict(H=0)),
     (INVALID, dict(Hkv=0)), (INVALID, dict(B=-1)), (INVALID, dict(cap=0)), (INVALID, dict(ldq=32 * 64 - 8)),
     (INVALID, dict(cache_strides=[51200, 6400, 48])), (INVALID, dict(scale_strides=[-1, 100])),
+    (INVALID, dict(cache_strides=[0, 6400, 64])), (INVALID, dict(cache_strides=[51200, 0, 64])),
+    (INVALID, dict(scale_strides=[0, 100])), (INVALID, dict(scale_strides=[800, 0])),
     (UNSUPPORTED, dict(dtype=_lib.VNX_I8)), (UNSUPPORTED, dict(cache_dtype=_lib.VNX_F16)),
     (UNSUPPORTED, dict(cache_dtype=9)), (UNSUPPORTED, dict(d=48)), (UNSUPPORTED, dict(d=8)), (UNSUPPORTED, dict(d=512)),
     (UNSUPPORTED, dict(qkv=AT + 8)), (UNSUPPORTED, dict(ldq=32 * 64 + 4)), (UNSUPPORTED, dict(k_cache=AT + 8)),

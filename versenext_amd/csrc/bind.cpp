@@ -11,6 +11,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -154,6 +155,7 @@ PyObject* kv_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
       !p.cos_table != !p.sin_table || !vec_of(a[10], 1, c.d, (int)dev, &p.q_norm, nullptr) ||
       !vec_of(a[11], 1, c.d, (int)dev, &p.k_norm, nullptr))
     Py_RETURN_NONE;
+  const c10::DeviceGuard guard(x->device());  // (the null stream is the current device's)
   at::Tensor q = at::empty({c.B, H, rows, c.d}, x->options().dtype(at::kBFloat16));
   p.qkv = x->data_ptr(), p.ldq = ld, p.q_out = q.data_ptr();
   p.k_cache = c.k->data_ptr(), p.v_cache = c.v->data_ptr();
@@ -181,6 +183,7 @@ PyObject* kv_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const auto t = reinterpret_cast<THPDtype*>(a[8])->scalar_type;
   p.out_dtype = code_of(t);
   if (rows > INT_MAX || p.out_dtype < 0) Py_RETURN_NONE;
+  const c10::DeviceGuard guard(c.k->device());
   at::Tensor k = at::empty({c.B, c.Hkv, rows, c.d}, c.k->options().dtype(t)), v = at::empty_like(k);
   p.k_cache = c.k->data_ptr(), p.v_cache = c.v->data_ptr(), p.k_scale = c.kscale(), p.v_scale = c.vscale();
   p.k_out = k.data_ptr(), p.v_out = v.data_ptr();
@@ -260,6 +263,7 @@ PyObject* tree_attn_q8(PyObject*, PyObject* const* a, Py_ssize_t n) {
     p.seg2_strides[1] = k2->stride(1), p.seg2_strides[2] = k2->stride(2);
     p.T2 = (int)k2->size(2);
   }
+  const c10::DeviceGuard guard(q->device());
   at::Tensor fresh;
   const at::Tensor* out;
   if (a[15] == Py_None) {

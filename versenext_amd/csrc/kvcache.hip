@@ -339,6 +339,11 @@ int vnx_kv_write(const vnx_kv_write_args* a, void* stream) {
   const int64_t HT = (int64_t)a->H + 2 * (int64_t)a->Hkv;
   if (a->ldq < HT * a->d || a->cache_strides[2] < a->d || a->scale_strides[0] < 0 || a->scale_strides[1] < 0)
     return VNX_ERR_INVALID_ARG;
+  // rows written must not lie on one another
+  const bool many = a->B > 1, heads = a->Hkv > 1;
+  if ((many && !a->cache_strides[0]) || (heads && !a->cache_strides[1]) ||
+      (q8 && ((many && !a->scale_strides[0]) || (heads && !a->scale_strides[1]))))
+    return VNX_ERR_INVALID_ARG;
   if (HT > INT_MAX || a->B > INT_MAX / a->n || a->B * a->n > (INT_MAX - 256) / HT) return VNX_ERR_UNSUPPORTED;
   // 16-byte loads and stores
   if (!aligned16(a->qkv) || a->ldq * elem_size(a->dtype) % 16 || !aligned16(a->q_out) || !aligned16(a->k_cache) ||

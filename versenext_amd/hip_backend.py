@@ -739,8 +739,12 @@ class HipBackend(DeviceBackend):
         skipped and their queries zero."""
         r = self._bind.kv_write(self._index, self._stream(), k_cache, v_cache, k_scale, v_scale, qkv, lens, cos, sin,
                                 q_norm, k_norm, eps)
-        if r is not None:      # (None: a call that needs the conversions or the errors below)
+        if r is not None:      # (None: a call that needs the general path's conversions or errors)
             return self._bound(r, "kv_write")
+        with torch.cuda.device(self._index):
+            return self._kv_write(qkv, k_cache, v_cache, lens, k_scale, v_scale, cos, sin, q_norm, k_norm, eps)
+
+    def _kv_write(self, qkv, k_cache, v_cache, lens, k_scale, v_scale, cos, sin, q_norm, k_norm, eps):
         B, Hkv, cap, d, code, ss = self._kv_cache(k_cache, v_cache, k_scale, v_scale, self._KV_DTYPES)
         x = _to_tensor(qkv, self._torch_device).resolve_neg()
         if x.dtype not in _lib.DTYPE_CODES:
@@ -778,6 +782,10 @@ class HipBackend(DeviceBackend):
         r = self._bind.kv_read(self._index, self._stream(), k_cache, v_cache, k_scale, v_scale, start, rows, out_dtype)
         if r is not None:
             return self._bound(r, "kv_read")
+        with torch.cuda.device(self._index):
+            return self._kv_read(k_cache, v_cache, k_scale, v_scale, start, rows, out_dtype)
+
+    def _kv_read(self, k_cache, v_cache, k_scale, v_scale, start, rows, out_dtype):
         B, Hkv, cap, d, code, ss = self._kv_cache(k_cache, v_cache, k_scale, v_scale, self._KV_DTYPES)
         if out_dtype not in _lib.DTYPE_CODES:
             raise ValueError("out_dtype must be torch.float32, torch.bfloat16 or torch.float16")
@@ -812,6 +820,12 @@ class HipBackend(DeviceBackend):
                                     scale, seg2, gates, window, max_len, out_dtype, out)
         if r is not None:
             return self._bound(r, "tree_attention_q8")
+        with torch.cuda.device(self._index):
+            return self._tree_attention_q8(q, k_cache, v_cache, k_scale, v_scale, lens, anc, scale, seg2, gates, window,
+                                           max_len, out_dtype, out)
+
+    def _tree_attention_q8(self, q, k_cache, v_cache, k_scale, v_scale, lens, anc, scale, seg2, gates, window, max_len,
+                           out_dtype, out):
         dev = self._torch_device
         B, Hkv, cap, d, code, ss = self._kv_cache(k_cache, v_cache, k_scale, v_scale, self._KV_DTYPES[:2])
         qt = self._heads_bf16(q, "q")
