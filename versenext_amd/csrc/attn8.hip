@@ -25,8 +25,14 @@
 // Statistics and sums are fp32; P * sv is rounded once to fp16 (2^-11 of each
 // term; see q8_walk for its range).
 // The running maximum of a column moves only when a score passes it by 2^8:
-// until then P stays below 2^8 in fp32 sums and bf16 operands, and the step
-// needs no exchange between lanes and no rescaling.
+// until then P stays below 2^8, and the step needs no exchange between lanes
+// and no rescaling.
+//
+// Long caches with few rows are bound by HBM (8 x 5 rows over 16,000 keys, heads
+// of 128: 46.8 us for 269 MB, 5.7 TB/s, and 4.7 for the join), prompts by the
+// vector ALU's issue rate beside the products (2,048 rows over 8,192: 110 us,
+// 0.71 PFLOP/s of the 1.17 of a large bf16 product), small steps by launch,
+// prologue and merge (32 x 7 rows over 617: 7.4 us, 5 of them with no key).
 #include <climits>
 
 #include "kvcache.h"
@@ -934,12 +940,16 @@ void q8_launch(const Q8Params& p, const Q8Words& tw, const Q8Plan& pl, hipStream
     }
     hipLaunchKernelGGL((k_attn8<D, KT, CT, KIND, SEG2, 4, 1, AUX>), grid, dim3(256 + 64 * SEG2), 0, st, p, tw);
   };
-  // Rows that one column group reads and no cache holds until the next call go
-  // past the caches (us, 8 x 5 rows over 16,000 keys, 240 MB: 57.7 / 54.3; re-read
-  // rows lose by it, 16 trees over 2,048 17.5 / 19.7).
+  // Rows that one column group reads go past the caches from 192 MiB on, where
+  // the next layer's rows push them out before they are read again.  us past /
+  // cached, 5 rows a sequence, heads of 128, two caches read in turn: 125 MiB
+  // 32.3 / 29.7, 156 51.1 / 49.1, 188 49.1 / 49.0, 219 49.8 / 51.3, 250 51.8 /
+  // 56.1, 500 (heads of 64) 93.1 / 101.7.  A single cache read again at once
+  // keeps more: 250 MiB 51.4 / 48.2.  Rows that several groups read lose (16
+  // trees over 2,048: 19.7 / 17.5).
   const int64_t rows = p.window > 0 && p.window < p.Tp ? p.window : p.Tp;
   if constexpr (CT <= 2) {
-    if (pl.groups == 1 && (int64_t)p.B * p.Hkv * rows * 2 * D >= (128 << 20)) return go(IntC<2>{});
+    if (pl.groups == 1 && (int64_t)p.B * p.Hkv * rows * 2 * D >= (192 << 20)) return go(IntC<2>{});
   }
   go(IntC<0>{});
 }

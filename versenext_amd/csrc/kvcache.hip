@@ -16,7 +16,10 @@
 // half that rotate with them, so the rotation needs no exchange and the norm
 // and the maximum one reduction over the head's lanes.
 // vnx_kv_read: codes * scale of a range of rows.
-// Both are bound by HBM where the rows are many and by the launch elsewhere.
+// Both are bound by HBM where the rows are many (on the GPU: 16,384 tokens x 48
+// heads of 128 with norms, int8, 73 us for 371 MB, 5.1 TB/s; 131,072 rows x 8
+// heads of 128 from e4m3, 151 us, 5.4 TB/s; a large copy runs at 5.3) and by the
+// launch elsewhere (one token: 2.8 us and 2.9).
 #include <climits>
 
 #include "kvcache.h"
@@ -296,7 +299,8 @@ int kv_write_launch(KvWriteParams p, int d, hipStream_t st) {
     constexpr int L = decltype(l)::value;
     // a wave a head group while that leaves the chip room (16 waves a CU), else a
     // token's all (us, 16,384 tokens x 48 heads of 128 with norms: 83 / 81).
-    // Queries that no cache will hold until they are read go past it (81 / 77).
+    // Queries that no cache will hold until they are read go past it (81 / 77
+    // together with the inputs, which are read once and always do).
     const int groups = (p.H + 2 * p.Hkv + 64 / L - 1) / (64 / L);
     p.per = (int64_t)p.tokens * groups <= 16 * (int64_t)device_cus() ? 1 : groups;
     p.chunks = (groups + p.per - 1) / p.per;
