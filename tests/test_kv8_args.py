@@ -91,7 +91,7 @@ def test_read_refusals(status, over):
     (UNSUPPORTED, dict(d=32)), (UNSUPPORTED, dict(kv_dtype=_lib.VNX_BF16)), (UNSUPPORTED, dict(out_dtype=_lib.VNX_F32)),
     (UNSUPPORTED, dict(anc=AT, N=65, Tp=30)), (UNSUPPORTED, dict(anc=AT, window=2)), (UNSUPPORTED, dict(anc=AT + 4)),
     (UNSUPPORTED, dict(q=AT + 8)), (UNSUPPORTED, dict(v_cache=AT + 8)), (UNSUPPORTED, dict(out=AT + 8)),
-    (UNSUPPORTED, dict(q_strides=[3072 + 4, 192, 64])), (UNSUPPORTED, dict(out_strides=[3072, 196, 64])),
+    (UNSUPPORTED, dict(q_strides=[4096 + 4, 192, 64])), (UNSUPPORTED, dict(out_strides=[4096, 196, 64])),
     (UNSUPPORTED, dict(cache_strides=[51200, 6400, 72])), (UNSUPPORTED, dict(seg2_strides=[0, 644, 64])),
     (UNSUPPORTED, dict(seg2_strides=[0, 640, 1 << 24])), (UNSUPPORTED, dict(cache_strides=[0, 0, 1 << 25])),
     (UNSUPPORTED, dict(cap=2 ** 31)), (UNSUPPORTED, dict(B=1 << 24, N=80, Tp=20)), (0, dict(B=0, q=None, lens=None)),
