@@ -30,8 +30,8 @@
 //
 // Long caches with few rows are bound by HBM (8 x 5 rows over 16,000 keys, heads
 // of 128: 46.8 us for 269 MB, 5.7 TB/s, and 4.7 for the join), prompts by the
-// vector ALU's issue rate beside the products (2,048 rows over 8,192: 110 us,
-// 0.71 PFLOP/s of the 1.17 of a large bf16 product), small steps by launch,
+// vector ALU's issue rate beside the products (2,048 rows over 8,192: 109-112 us,
+// 0.7 PFLOP/s of the 1.17 of a large bf16 product), small steps by launch,
 // prologue and merge (32 x 7 rows over 617: 7.4 us, 5 of them with no key).
 #include <climits>
 
