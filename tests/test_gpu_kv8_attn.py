@@ -316,3 +316,29 @@ def test_same_call_on_two_streams(hip):
     torch.cuda.synchronize(dev)
     for w, many in zip(want, got):
         assert all(torch.equal(w, o) for o in many)
+
+
+@pytest.mark.parametrize("dtype", [I8, E4], ids=["int8", "e4m3"])
+@pytest.mark.parametrize("d,B,N,rep,window", [(64, 16, 3, 2, 0), (64, 16, 1, 4, 0), (128, 8, 5, 4, 0), (128, 8, 1, 1, 0),
+                                              (64, 18, 2, 2, 15000)])
+def test_rows_read_past_the_caches(hip, d, B, N, rep, window, dtype):
+    """192 MiB of rows and more, which one column group reads: every head and sequence shares one head's rows (strides
+    of 0), so the memory is small.  NaN behind the last row."""
+    dev = hip.torch_device
+    Hkv, Tp = 8, 16001
+    assert B * Hkv * (window or Tp) * 2 * d >= 192 << 20
+    g = R.gen(d + N)
+    kc, ks = R.cache(g, 1, 1, Tp + N + 40, d, dtype)
+    vc, vs = R.cache(g, 1, 1, Tp + N + 40, d, dtype)
+    _poison(kc, vc, ks, vs, [Tp + N])
+    q = (torch.randn(B, rep * Hkv, N, d, generator=g) * 1.5).to(torch.bfloat16)
+    lens = [Tp, 0, 31, 32, 15970] + [Tp - 17 * b for b in range(B - 5)]
+    print(f"d={d} B={B} N={N} rep={rep} window={window} {dtype}", flush=True)
+    wide = [t.to(dev).expand(B, Hkv, *t.shape[2:]) for t in (kc, vc, ks, vs)]
+    for _ in range(2):                      # one call behind the other: the same rows again
+        o = hip.tree_attention_q8(q, *wide, lens, window=window, max_len=Tp)
+    pick = [0, 1, 2, 3, 4, B - 1]           # sequences of the 64-bit form, two KV heads of each
+    heads = list(range(rep)) + list(range((Hkv - 1) * rep, Hkv * rep))
+    k, v = (R.values(c, s).expand(len(pick), 2, -1, -1) for c, s in ((kc, ks), (vc, vs)))
+    ref, mag = R.attention(q[pick][:, heads], k, v, [lens[b] for b in pick], Tp, window=window)
+    _close(o[pick][:, heads], ref, mag)
