@@ -944,8 +944,9 @@ int vnx_kv_read(const vnx_kv_read_args* args, void* stream);
  *     >= N, else VNX_ERR_UNSUPPORTED).
  * A node that sees no row gets zeros from the first term.  T2 > 0: a second
  * segment of bf16 rows ((B or 1, Hkv, T2, d), batch stride 0 when shared), all
- * seen, and gates, two fp32 on the device; T2 == 0: g0 = 1 and no second term
- * (TriSparse's global path and gates, tri_sparse_attn.py:469-495, :585-608).
+ * seen.  gates (fp32 on the device): g0 = gates[0], g1 = gates[1]; T2 == 0: no
+ * second term, only gates[0] is read and NULL means g0 = 1 (TriSparse's global
+ * path and gates, tri_sparse_attn.py:469-495, :585-608).
  * Query head h reads KV head h / (H / Hkv).  q bf16 (B, H, N, d), out VNX_BF16
  * or VNX_F16, strides {batch, head, row} multiples of 8, pointers 16-byte
  * aligned.  d in {64, 128}.  Tp + N <= cap.  Codes of e4m3 NaN must not stand in

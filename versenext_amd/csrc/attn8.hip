@@ -4,6 +4,7 @@
 //   S_ij = scale * sk_j * (q_i . kc_j),  P = softmax over the keys i sees,
 //   O_i = sum_j P_ij sv_j vc_j           (kc, vc codes; sk, sv their scales)
 //   out_i = g0 * O_i + g1 * (the same over the second segment, bf16 rows)
+//   (g0, g1 = gates[0], gates[1]; no gates: g0 = 1)
 //
 // A code is exact in bf16 and in fp16 (8 significant bits), so the products run
 // on v_mfma_f32_16x16x32_bf16 (the scores, with the bf16 queries) and _f16 (the
@@ -659,11 +660,8 @@ __global__ __launch_bounds__((KW * CW + (SEG2 && KW >= 4)) * 64, 2) void k_attn8
     }
   };
 
-  float g0 = 1.0f, g1 = 0.0f;
-  if constexpr (SEG2) {
-    g0 = p.gates[0];
-    g1 = p.gates[1];
-  }
+  const float g0 = SEG2 || p.gates ? p.gates[0] : 1.0f;
+  const float g1 = SEG2 ? p.gates[1] : 0.0f;
   if constexpr (LDS2) {
     st.clear();
     q8_walk<D, KV_BF16, CT, Q8_ALL>(t.src2, 0, kw, KW, (p.T2 + 31) / 32, t.mask2(p.T2), p.c, t.qf, st, lane);
@@ -778,7 +776,7 @@ __global__ __launch_bounds__(256) void k_attn8_join(Q8Params p, int ct16) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] += __shfl_xor(v[i], o, 64);
   if (g) return;
-  const float g0 = p.T2 > 0 ? p.gates[0] : 1.0f;
+  const float g0 = p.gates ? p.gates[0] : 1.0f;
   v *= sum == 0.0f ? 0.0f : g0 / sum;
   if (p.T2 > 0) {
     const int64_t r = r0 + (int64_t)p.splits * ct16;
@@ -1000,7 +998,7 @@ int vnx_tree_attn_q8(const vnx_attn_q8_args* a, void* workspace, size_t workspac
       (a->T2 > 0 && a->seg2_strides[2] >= (1 << 24)))
     return VNX_ERR_UNSUPPORTED;
   if (!aligned16(a->q) || !aligned16(a->k_cache) || !aligned16(a->v_cache) || !aligned16(a->out) ||
-      (a->T2 > 0 && (!aligned16(a->k_seg2) || !aligned16(a->v_seg2) || !aligned_to(a->gates, 4))) ||
+      (a->T2 > 0 && (!aligned16(a->k_seg2) || !aligned16(a->v_seg2))) || !aligned_to(a->gates, 4) ||
       !aligned_to(a->k_scale, 4) || !aligned_to(a->v_scale, 4) || !aligned_to(a->lens, 4) || !aligned_to(a->anc, 8))
     return VNX_ERR_UNSUPPORTED;
   const Q8Plan pl = q8_plan(a);
@@ -1022,8 +1020,8 @@ int vnx_tree_attn_q8(const vnx_attn_q8_args* a, void* workspace, size_t workspac
   if (a->T2 > 0) {
     p.k2 = static_cast<const char*>(a->k_seg2); p.v2 = static_cast<const char*>(a->v_seg2);
     p.s2_sb = 2 * a->seg2_strides[0]; p.s2_sh = 2 * a->seg2_strides[1]; p.s2_sr = 2 * a->seg2_strides[2];
-    p.gates = a->gates;
   }
+  p.gates = a->gates;
   Q8Words tw{};
   if (a->anc) {
     p.tree = 2;

@@ -249,16 +249,21 @@ PyObject* tree_attn_q8(PyObject*, PyObject* const* a, Py_ssize_t n) {
   double scale = 1.0 / std::sqrt((double)c.d);
   if (a[9] != Py_None && !float_of(a[9], &scale)) Py_RETURN_NONE;
   if (!int_of(a[12], 0, INT_MAX, &window)) Py_RETURN_NONE;
+  const int64_t ngates = a[10] != Py_None ? 2 : 1;
+  if (a[11] != Py_None) {
+    const at::Tensor* g = tensor(a[11], (int)dev);
+    if (!g || g->scalar_type() != at::kFloat || g->dim() != 1 || g->size(0) < ngates || g->stride(0) != 1)
+      Py_RETURN_NONE;
+    p.gates = static_cast<const float*>(g->data_ptr());
+  }
   if (a[10] != Py_None) {
     if (!PyTuple_Check(a[10]) || PyTuple_GET_SIZE(a[10]) != 2) Py_RETURN_NONE;
     const at::Tensor *k2 = heads(PyTuple_GET_ITEM(a[10], 0), (int)dev, c.d),
-                     *v2 = heads(PyTuple_GET_ITEM(a[10], 1), (int)dev, c.d), *g = tensor(a[11], (int)dev);
+                     *v2 = heads(PyTuple_GET_ITEM(a[10], 1), (int)dev, c.d);
     if (!k2 || !v2 || !same_layout(*k2, *v2) || (k2->size(0) != 1 && k2->size(0) != c.B) || k2->size(1) != c.Hkv ||
-        k2->size(2) < 1 || k2->size(2) > INT_MAX || !g || g->scalar_type() != at::kFloat || g->dim() != 1 ||
-        g->size(0) < 2 || g->stride(0) != 1)
+        k2->size(2) < 1 || k2->size(2) > INT_MAX || !p.gates)
       Py_RETURN_NONE;
     p.k_seg2 = k2->data_ptr(), p.v_seg2 = v2->data_ptr();
-    p.gates = static_cast<const float*>(g->data_ptr());
     p.seg2_strides[0] = k2->size(0) == 1 ? 0 : k2->stride(0);
     p.seg2_strides[1] = k2->stride(1), p.seg2_strides[2] = k2->stride(2);
     p.T2 = (int)k2->size(2);

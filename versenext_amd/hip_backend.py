@@ -811,7 +811,8 @@ class HipBackend(DeviceBackend):
         q (B, H, N, d), read as bf16; lens (B,) int32; anc None: a chain of any
         N (one token, drafts, a prompt); or (N,) / (B, N) ancestor words
         (tree.ancestor_words) of a token tree of at most 64 nodes.  window,
-        seg2 and gates as in tree_attention (no ALiBi).  max_len: a bound of
+        seg2 and gates as in tree_attention (no ALiBi); without seg2, gates[0]
+        (None: 1) still scales the result.  max_len: a bound of
         lens known to the caller (cap - N by default; longer lens are cut to
         it), from which the launch is sized.  Returns (B, H, N, d) bfloat16 or
         float16, written into `out` (any strides with unit last stride) when
@@ -865,10 +866,11 @@ class HipBackend(DeviceBackend):
                 k2, v2 = k2.contiguous(), v2.contiguous()
             if gates is None:
                 raise ValueError("a second segment needs the two gates")
-            g = _to_tensor(gates, dev, torch.float32).reshape(-1).contiguous()
-            if g.numel() < 2:
-                raise ValueError("gates must hold two values")
             s2 = (0 if k2.shape[0] == 1 else k2.stride(0), k2.stride(1), k2.stride(2))
+        if gates is not None:
+            g = _to_tensor(gates, dev, torch.float32).reshape(-1).contiguous()
+            if g.numel() < (1 if seg2 is None else 2):
+                raise ValueError("gates must hold two values with a second segment, one without")
         args = _lib.pack_attn_q8(
             qt.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
             ln.data_ptr(), _ptr(anc_t) or 0, a.ctypes.data if a is not None and anc_t is None else 0, out.data_ptr(),
