@@ -491,7 +491,9 @@ typedef struct vnx_tree_attn_args {
    *         over the T2 rows)
    * with gates a device array of 2 fp32.  seg2_strides {batch, head, row} in
    * elements (batch 0: one segment shared by all rows), multiples of 8.
-   * T2 == 0 (or zero-initialised trailing fields): no second segment. */
+   * T2 == 0 (or zero-initialised trailing fields): no second segment; gates,
+   * when not NULL, then still scale: out = gates[0] * (the attention over
+   * prefix + tree). */
   const void* k_seg2;
   const void* v_seg2;
   int64_t seg2_strides[3];

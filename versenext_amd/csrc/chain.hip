@@ -325,7 +325,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void k_chain_attn(ChainParams
       }
       __syncthreads();                 // read before the next segment stages
     }
-    const float gate = (has2 || p.slopes) ? p.gates[seg] : 1.0f;
+    const float gate = p.gates ? p.gates[seg] : 1.0f;
     const float inv = l > 0.0f ? gate / l : 0.0f;
 #pragma unroll
     for (int t = 0; t < DT; ++t)
@@ -387,7 +387,7 @@ int vnx_chain_attn(const vnx_tree_attn_args* a, void* stream) {
   if (B == 0) return VNX_OK;
   if (!a->q || !a->k_cache || !a->v_cache || !a->out) return VNX_ERR_INVALID_ARG;
   const auto mis4 = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 3u) != 0; };
-  if ((a->T2 > 0 || a->alibi_slopes) && (!a->gates || mis4(a->gates))) return VNX_ERR_INVALID_ARG;
+  if (((a->T2 > 0 || a->alibi_slopes) && !a->gates) || mis4(a->gates)) return VNX_ERR_INVALID_ARG;
   if (mis4(a->alibi_slopes) || mis4(a->tp_batch)) return VNX_ERR_INVALID_ARG;
   if (a->T2 > 0 && (!a->k_seg2 || !a->v_seg2)) return VNX_ERR_INVALID_ARG;
   // 16-byte loads of bf16 rows; 16-byte (fp32) / 8-byte (16-bit) output stores

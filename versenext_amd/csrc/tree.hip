@@ -69,7 +69,8 @@ struct TreeAttnParams {
   const int32_t* tp_batch;          // per-batch prefix rows (<= Tp), or NULL
   int tree_follows_prefix;          // tree row j of batch b is tree row tp_b + j
   // Second key segment: T2 rows visible to every node, normalised on its own
-  // and mixed as gates[0] * segment 1 + gates[1] * segment 2 (T2 == 0: none).
+  // and mixed as gates[0] * segment 1 + gates[1] * segment 2 (T2 == 0: none;
+  // gates NULL: segment 1 as it is).
   const uint16_t* k2;
   const uint16_t* v2;
   int64_t s2_sb, s2_sh, s2_sr;
@@ -595,7 +596,7 @@ __global__ __launch_bounds__(NW * 64, (PF == 2 && D == 64 && NW == 4) ? 2 : 1) v
     if (grp == 0) s_ml[(w * QT + qt) * 16 + col] = make_float2(m[qt], l[qt]);
   }
   __syncthreads();
-  const float g1 = (has2 || alibi) && p.S == 1 ? p.gates[0] : 1.0f;
+  const float g1 = p.gates && p.S == 1 ? p.gates[0] : 1.0f;
   const float g2 = has2 && p.S == 1 ? p.gates[1] : 0.0f;
   const float g3 = has3 ? p.gates[2] : 0.0f;  // ALiBi launches have one split
   for (int t = w; t < QT * DT; t += NW) {
@@ -667,7 +668,7 @@ __global__ __launch_bounds__(256) void k_tree_merge(TreeAttnParams p) {
     const f32x4 o2 = *reinterpret_cast<const f32x4*>(p.part_o + (row * SS + p.S) * D + c4 * 4);
     v = acc * (L > 0.0f ? p.gates[0] / L : 0.0f) + o2 * (L2 > 0.0f ? p.gates[1] / L2 : 0.0f);
   } else {
-    v = acc * (L > 0.0f ? 1.0f / L : 0.0f);
+    v = acc * (L > 0.0f ? (p.gates ? p.gates[0] : 1.0f) / L : 0.0f);
   }
   const int node = (int)(row % p.N);
   const int64_t bh = row / p.N;
@@ -1002,7 +1003,7 @@ __global__ __launch_bounds__(256) void k_attn_rows_f32(F32RowsParams p) {
   rs_merge<D>(A);
   if (alibi) rs_merge<D>(C);
   const bool has2 = p.T2 > 0;
-  const float g1 = (has2 || p.slopes) ? p.gates[0] : 1.0f;
+  const float g1 = p.gates ? p.gates[0] : 1.0f;
   RowSoftmax<D> S2;
   rs_init(S2);
   if (has2) {
@@ -1053,7 +1054,7 @@ static int tree_attn_f32(const vnx_tree_attn_args* a, void* stream) {
   if (B == 0) return VNX_OK;
   if (!a->q || !a->k_tree || !a->v_tree || !a->out) return VNX_ERR_INVALID_ARG;
   if (Tp > 0 && (!a->k_cache || !a->v_cache)) return VNX_ERR_INVALID_ARG;
-  if ((a->T2 > 0 || a->alibi_slopes) && (!a->gates || (reinterpret_cast<uintptr_t>(a->gates) & 3u)))
+  if (((a->T2 > 0 || a->alibi_slopes) && !a->gates) || (reinterpret_cast<uintptr_t>(a->gates) & 3u))
     return VNX_ERR_INVALID_ARG;
   if (a->alibi_slopes && (reinterpret_cast<uintptr_t>(a->alibi_slopes) & 3u)) return VNX_ERR_INVALID_ARG;
   if (a->T2 > 0 && (!a->k_seg2 || !a->v_seg2)) return VNX_ERR_INVALID_ARG;
@@ -1156,12 +1157,11 @@ int vnx_tree_attn(const vnx_tree_attn_args* a, void* workspace, size_t workspace
   if (a->window < 0 || a->alibi_max_keys < 0 || a->force_splits < 0 || a->force_waves < 0)
     return VNX_ERR_INVALID_ARG;
   if (a->window > 0 && a->window < N) return VNX_ERR_UNSUPPORTED;  // tree keys always inside the window
-  if (a->alibi_slopes && (!a->gates || (reinterpret_cast<uintptr_t>(a->gates) & 3u) ||
-                          (reinterpret_cast<uintptr_t>(a->alibi_slopes) & 3u)))
+  if (reinterpret_cast<uintptr_t>(a->gates) & 3u) return VNX_ERR_INVALID_ARG;
+  if (a->alibi_slopes && (!a->gates || (reinterpret_cast<uintptr_t>(a->alibi_slopes) & 3u)))
     return VNX_ERR_INVALID_ARG;
   if (a->T2 > 0) {
-    if (!a->k_seg2 || !a->v_seg2 || !a->gates || (reinterpret_cast<uintptr_t>(a->gates) & 3u))
-      return VNX_ERR_INVALID_ARG;
+    if (!a->k_seg2 || !a->v_seg2 || !a->gates) return VNX_ERR_INVALID_ARG;
     if (!strides_ok(a->seg2_strides[0], a->seg2_strides[1], a->seg2_strides[2], 8) ||
         !aligned16(a->k_seg2) || !aligned16(a->v_seg2))
       return VNX_ERR_UNSUPPORTED;
@@ -1213,13 +1213,12 @@ int vnx_tree_attn(const vnx_tree_attn_args* a, void* workspace, size_t workspace
     p.v2 = static_cast<const uint16_t*>(a->v_seg2);
     p.s2_sb = a->seg2_strides[0]; p.s2_sh = a->seg2_strides[1]; p.s2_sr = a->seg2_strides[2];
     p.T2 = a->T2;
-    p.gates = a->gates;
   }
+  p.gates = a->gates;
   p.c = (float)((double)a->scale * 1.4426950408889634);
   p.window = window;
   p.slopes = a->alibi_slopes;
   p.alibi_max = a->alibi_max_keys;
-  if (p.slopes) p.gates = a->gates;
   if (a->qkv) {
     p.qkv = static_cast<const uint16_t*>(a->qkv);
     p.qkv_ld = a->qkv_ld;

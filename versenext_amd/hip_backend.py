@@ -556,7 +556,8 @@ class HipBackend(DeviceBackend):
         in out_dtype (torch.float32, torch.bfloat16 or torch.float16).
         seg2 = (k2, v2), each (B or 1, Hkv, T2, d), with gates (2,) adds
         TriSparse's gated global path: out = gates[0] * (the tree attention)
-        + gates[1] * (attention over the T2 rows, all visible).  tp (B,)
+        + gates[1] * (attention over the T2 rows, all visible); without
+        seg2, gates[0] (None: 1) still scales the tree attention.  tp (B,)
         int32: per-row prefix lengths (ragged caches).  window > 0 keeps
         keys less than window positions behind each node; alibi_slopes (H,)
         with gates (3,) adds the ALiBi path as gates[2] * it for rows with
@@ -642,13 +643,9 @@ class HipBackend(DeviceBackend):
                 raise ValueError(f"alibi_slopes must have {H} entries")
             if gates is None:
                 raise ValueError("the ALiBi path needs three gates")
-            g3 = _to_tensor(gates, dev, torch.float32).reshape(-1).contiguous()
-            if g3.numel() < 3:
-                raise ValueError("gates must hold three values with ALiBi")
-            keep += [sl, g3]
+            keep.append(sl)
             args.alibi_slopes = sl.data_ptr()
             args.alibi_max_keys = int(alibi_max_keys)
-            args.gates = g3.data_ptr()
         if seg2 is not None:
             k2 = self._heads_bf16(seg2[0], "k_seg2", rows)
             v2 = self._heads_bf16(seg2[1], "v_seg2", rows)
@@ -658,13 +655,15 @@ class HipBackend(DeviceBackend):
                 k2, v2 = k2.contiguous(), v2.contiguous()
             if gates is None:
                 raise ValueError("a second segment needs the two gates")
-            g = _to_tensor(gates, dev, torch.float32).reshape(-1).contiguous()
-            if g.numel() < 2:
-                raise ValueError("gates must hold two values")
-            keep += [k2, v2, g]
+            keep += [k2, v2]
             args.k_seg2, args.v_seg2 = k2.data_ptr(), v2.data_ptr()
             args.seg2_strides[:] = [0 if k2.shape[0] == 1 else k2.stride(0), k2.stride(1), k2.stride(2)]
             args.T2 = k2.shape[2]
+        if gates is not None:
+            g = _to_tensor(gates, dev, torch.float32).reshape(-1).contiguous()
+            if g.numel() < (3 if alibi_slopes is not None else 2 if seg2 is not None else 1):
+                raise ValueError("gates must hold three values with ALiBi, two with a second segment, one without")
+            keep.append(g)
             args.gates = g.data_ptr()
         ws = self._workspace(self._L.vnx_tree_attn_workspace_args(ctypes.byref(args)))
         _lib.check(self._L.vnx_tree_attn(ctypes.byref(args), _ptr(ws), ws.numel(),
