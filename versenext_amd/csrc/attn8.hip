@@ -24,7 +24,7 @@
 //                    the score registers into the B operand as it is.
 // A step's rows are loaded into registers under the previous step's math.
 // Statistics and sums are fp32; P * sv is rounded once to fp16 (2^-11 of each
-// term; see q8_walk for its range).
+// term), or goes in two bf16 parts where the scales lie far apart (q8_steps).
 // The running maximum of a column moves only when a score passes it by 2^8:
 // until then P stays below 2^8, and the step needs no exchange between lanes
 // and no rescaling.
@@ -103,9 +103,16 @@ __device__ __forceinline__ float q8_max3(float a, float b, float c) {
   asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
   return r;
 }
+
 __device__ __forceinline__ float q8_absmax3(float a, float b, float c) {
   float r;
   asm("v_max3_f32 %0, %1, |%2|, |%3|" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
+__device__ __forceinline__ float q8_absmin3(float a, float b, float c) {
+  float r;
+  asm("v_min3_f32 %0, %1, |%2|, |%3|" : "=v"(r) : "v"(a), "v"(b), "v"(c));
   return r;
 }
 
@@ -219,7 +226,8 @@ struct Q8Vals {
   }
 
   // Operands of dim tiles 4 x .. (codes; 2 x .. of bf16 rows) from word x: the
-  // 8 keys of this lane, fp16 (codes) or bf16 pairs.
+  // 8 keys of this lane, bf16 pairs, or fp16 pairs of codes.
+  template <bool BF16>
   __device__ __forceinline__ void frag(u32x4 (&f)[D / 16]) const {
 #pragma unroll
     for (int x = 0; x < W; ++x) {
@@ -235,8 +243,14 @@ struct Q8Vals {
           uint32_t c[2][2];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            c[h][0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v[2 * j + h][x], 1.0f, false));
-            c[h][1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v[2 * j + h][x], 1.0f, true));
+            const uint32_t w = v[2 * j + h][x];
+            if constexpr (BF16) {
+              c[h][0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false));
+              c[h][1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true));
+            } else {
+              c[h][0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false));
+              c[h][1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true));
+            }
           }
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -252,7 +266,8 @@ struct Q8Vals {
           kv_f32x4<KV_I8>(v[2 * j + 1][x], b);
 #pragma unroll
           for (int i = 0; i < 4; ++i)  // (exact: the rounding mode does not matter)
-            f[4 * x + i][j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a[i], b[i]));
+            f[4 * x + i][j] = BF16 ? kv_pk_bf16(a[i], b[i])
+                                   : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a[i], b[i]));
         }
       }
     }
@@ -328,22 +343,45 @@ struct Q8State {
   }
 };
 
+// Eight fp32 values in two bf16 parts (2^-17 of each value).
+__device__ __forceinline__ void q8_split(const float (&p)[8], u32x4& hi, u32x4& lo) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t h = kv_pk_bf16(p[2 * e], p[2 * e + 1]);
+    hi[e] = h;
+    lo[e] = kv_pk_bf16(p[2 * e] - __uint_as_float(h << 16), p[2 * e + 1] - __uint_as_float(h & 0xFFFF0000u));
+  }
+}
+
 // Walks steps s0, s0 + ds, .. < s1 of 32 keys from key `first` on: online
-// softmax into st.  Codes: P sv / R in fp16 (2^-11), R the largest sv so far times 2^-6: P <= 2^8
-// and sv / R <= 2^7 stay in range, and a term keeps its 11 bits down to 2^-21 of
-// the largest row's scale (below: 2^-32 of it).  bf16 rows: P in two bf16 parts.
-template <int D, int KT, int CT, int KIND, int AUX = 0>
-__device__ __forceinline__ void q8_walk(const Q8Src& src, int first, int s0, int ds, int s1, const Q8Mask<CT>& mk,
-                                        float c, const bf16x8 (&qf)[CT][D / 32], Q8State<CT, D>& st, int lane) {
-  if (s0 >= s1) return;
+// softmax into st, acc in units of R.
+//   not WIDE  codes only: P sv / R in fp16, 2^-11 of a term.  R is a power of two
+//             that puts the largest scale so far in [2^6, 2^7) R: P <= 2^8 stays
+//             in range, and fp16's smallest step costs a term 2^-25 R at most.  R
+//             moves with every loaded row, seen or not, and a row's scale may lie
+//             far below it, so the walk gives up (true) at a step with a scale
+//             outside [2^-6, 2^7) R, to be walked again WIDE.
+//   WIDE      P sv / R (bf16 rows: P) in two bf16 parts: 2^-17 of a term, in
+//             fp32's range (R at most 2^40, moved by scales of 2^80 R and more): no
+//             row that a column does not see costs it a bit.
+template <int D, int KT, int CT, int KIND, int AUX, bool WIDE>
+__device__ __forceinline__ bool q8_steps(const Q8Src& src, int first, int s0, int ds, int s1, const Q8Mask<CT>& mk,
+                                        float c, const bf16x8 (&qf)[CT][D / 32], Q8State<CT, D>& st, float& R, int lane) {
+  if (s0 >= s1) return false;
   const int g4 = (lane >> 4) * 4;
   Q8Keys<D, KT, AUX> keys;
   Q8Vals<D, KT, AUX> vals;
   auto left = [&](int s) { return s < s1 ? src.rows - (first + 32 * s) : 0; };
-  float R = 0.0f, iR = __builtin_inff();
+  int end = uni(s1);
+  float iR = 1.0f / R;  // (infinite before the first row)
+  // the rows in the order in which the loop waits for them (in another order its
+  // waits for a step's keys are waits for its values too: 8 x 5 rows over 16,000
+  // 58.9 us instead of 50.6)
   keys.load(src, first + 32 * s0, left(s0), lane);
+  __builtin_amdgcn_sched_barrier(0);
   vals.load(src, first + 32 * s0, left(s0), lane);
-  for (int s = s0; s < s1; s += ds) {
+  __builtin_amdgcn_sched_barrier(0);
+  for (int s = s0; s < end; s += ds) {
     const int k0 = first + 32 * s;
     float x[CT][8];  // scores relative to the maxima, in the exp2 domain
     {
@@ -368,29 +406,47 @@ __device__ __forceinline__ void q8_walk(const Q8Src& src, int first, int s0, int
     u32x4 vf[D / 16];
     float sv[8];
     {
-      vals.frag(vf);
+      vals.template frag<WIDE>(vf);
 #pragma unroll
       for (int d = 0; d < D / 16; ++d) asm volatile("" : "+v"(vf[d]));  // converted here: the rows' registers are free
       if constexpr (KT != KV_BF16) {
-        float top = 0.0f;
+        // The scales' range: in the common step by two instructions a pair, which
+        // see infinities and zeros too; where that finds something, exactly.
+        constexpr float kTop = WIDE ? 0x1p80f : 0x1p7f;
+        float top = 0.0f, low = 0x1p127f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sv[e] = vals.sv[e / 4][e % 4];
+        for (int e = 0; e < 8; e += 2) top = q8_absmax3(top, vals.sv[e / 4][e % 4], vals.sv[e / 4][e % 4 + 1]);
+        if constexpr (!WIDE) {
 #pragma unroll
-        for (int e = 0; e < 8; e += 2) top = q8_absmax3(top, sv[e], sv[e + 1]);
-        if (__any(!(top * iR <= 128.0f))) {
-          top = 0x1p-110f;
+          for (int e = 0; e < 8; e += 2) low = q8_absmin3(low, vals.sv[e / 4][e % 4], vals.sv[e / 4][e % 4 + 1]);
+        }
+        // (bitwise: branches between lanes here cost a copy of acc a step)
+        if (__any((bool)((uint32_t)!(top < R * kTop) | (uint32_t)(!WIDE && low < R * 0x1p-6f)))) {
+          uint32_t least = 0xFFFFFFFFu;  // twice the bits less 2: the sign gone, zero the largest
+          top = 0.0f;
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const float a = fabsf(sv[e]);
+            const float a = fabsf(vals.sv[e / 4][e % 4]);
             top = fmaxf(top, a < __builtin_inff() ? a : 0.0f);
+            least = min(least, (__float_as_uint(a) << 1) - 2);
           }
-          top = fmaxf(q8_max4(top) * 0x1p-6f, R);
-          iR = 1.0f / top;
-          st.scale(R * iR);
-          R = top;
+          auto out = [&] {
+            const uint32_t low2 = (__float_as_uint(R) << 1) - 2 - (6u << 24);
+            return (bool)((uint32_t)!(top < R * kTop) | (uint32_t)(!WIDE && least < low2));
+          };
+          if (__any(out())) {
+            // the largest scale's exponent alone, times 2^-6, in [2^-110, 2^40]
+            const int ex = min(max(uni((int)(__float_as_uint(q8_max4(top)) >> 23)) - 6, 17), 167);
+            const float r = fmaxf(R, __uint_as_float((uint32_t)ex << 23));
+            iR = __uint_as_float(0x7F000000u - __float_as_uint(r));  // 1 / r
+            st.scale(R * iR);
+            R = r;
+            if (!WIDE && __any(out())) end = s;  // (the last step: what it adds is not used)
+          }
         }
+        asm volatile("" : "+s"(end));  // (one way out of the loop, at its end: no copies of acc)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sv[e] *= iR;
+        for (int e = 0; e < 8; ++e) sv[e] = vals.sv[e / 4][e % 4] * iR;
       }
       vals.load(src, k0 + 32 * ds, left(s + ds), lane);
     }
@@ -440,42 +496,61 @@ __device__ __forceinline__ void q8_walk(const Q8Src& src, int first, int s0, int
         }
       }
     }
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-      float p[8];
+    auto weigh = [&](int ct, float (&p)[8]) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         p[e] = q8_ex2(x[ct][e]);
         st.l[ct] += p[e];
+        if constexpr (KT != KV_BF16) p[e] *= sv[e];
       }
-      {
-        if constexpr (KT != KV_BF16) {
+    };
+    if constexpr (WIDE) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) p[e] *= sv[e];
-          const u32x4 w = {q8_pk_f16(p[0], p[1]), q8_pk_f16(p[2], p[3]), q8_pk_f16(p[4], p[5]), q8_pk_f16(p[6], p[7])};
+      for (int ct = 0; ct < CT; ++ct) {
+        if constexpr (KT != KV_BF16) __builtin_amdgcn_sched_barrier(0);  // (a rare path: registers before overlap)
+        float p[8];
+        weigh(ct, p);
+        u32x4 hi, lo;
+        q8_split(p, hi, lo);
 #pragma unroll
-          for (int d = 0; d < D / 16; ++d)
-            st.acc[ct][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, vf[d]),
-                                                                  __builtin_bit_cast(f16x8, w), st.acc[ct][d], 0, 0, 0);
-        } else {
-          u32x4 hi, lo;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t h = kv_pk_bf16(p[2 * e], p[2 * e + 1]);
-            hi[e] = h;
-            lo[e] = kv_pk_bf16(p[2 * e] - __uint_as_float(h << 16), p[2 * e + 1] - __uint_as_float(h & 0xFFFF0000u));
-          }
-#pragma unroll
-          for (int d = 0; d < D / 16; ++d) {
-            const bf16x8 v = __builtin_bit_cast(bf16x8, vf[d]);
-            st.acc[ct][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, __builtin_bit_cast(bf16x8, hi), st.acc[ct][d], 0, 0, 0);
-            st.acc[ct][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, __builtin_bit_cast(bf16x8, lo), st.acc[ct][d], 0, 0, 0);
-          }
+        for (int d = 0; d < D / 16; ++d) {
+          const bf16x8 v = __builtin_bit_cast(bf16x8, vf[d]);
+          st.acc[ct][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, __builtin_bit_cast(bf16x8, hi), st.acc[ct][d], 0, 0, 0);
+          st.acc[ct][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, __builtin_bit_cast(bf16x8, lo), st.acc[ct][d], 0, 0, 0);
         }
+      }
+    } else {
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        float p[8];
+        weigh(ct, p);
+        const u32x4 w = {q8_pk_f16(p[0], p[1]), q8_pk_f16(p[2], p[3]), q8_pk_f16(p[4], p[5]), q8_pk_f16(p[6], p[7])};
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d)
+          st.acc[ct][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, vf[d]),
+                                                                __builtin_bit_cast(f16x8, w), st.acc[ct][d], 0, 0, 0);
       }
     }
   }
-  if constexpr (KT != KV_BF16) st.scale(R);
+  return end != s1;
+}
+
+// The walk from a cleared state; acc absolute afterwards.
+template <int D, int KT, int CT, int KIND, int AUX = 0>
+__device__ __forceinline__ void q8_walk(const Q8Src& src, int first, int s0, int ds, int s1, const Q8Mask<CT>& mk,
+                                        float c, const bf16x8 (&qf)[CT][D / 32], Q8State<CT, D>& st, int lane) {
+  st.clear();
+  if constexpr (KT == KV_BF16) {
+    float R = 1.0f;
+    q8_steps<D, KT, CT, KIND, AUX, true>(src, first, s0, ds, s1, mk, c, qf, st, R, lane);
+  } else {
+    float R = 0.0f;
+    if (q8_steps<D, KT, CT, KIND, AUX, false>(src, first, s0, ds, s1, mk, c, qf, st, R, lane)) {
+      st.clear();
+      q8_steps<D, KT, CT, KIND, AUX, true>(src, first, s0, ds, s1, mk, c, qf, st, R, lane);
+    }
+    st.scale(R);
+  }
 }
 
 // A column's node and query head.
@@ -593,8 +668,12 @@ __device__ __forceinline__ int64_t q8_out_off(const Q8Params& p, int b, int kvh,
 // walks it beside the others, in the last split.  (us, 32 x 7 rows over 617,
 // 128 global rows: 7.8 with that wave, 10.1 walked first; 4 x 512 rows, KW = 2:
 // 18.1 walked first, 26 with the wave and KW = 4.)
+// Waves a SIMD has registers for.
+constexpr int q8_occ(int d, int ct) { return d == 64 && ct <= 2 ? 5 - ct : 2; }
+
 template <int D, int KT, int CT, int KIND, bool SEG2, int KW, int CW, int AUX = 0>
-__global__ __launch_bounds__((KW * CW + (SEG2 && KW >= 4)) * 64, 2) void k_attn8(Q8Params p, Q8Words tw) {
+__global__ __launch_bounds__((KW * CW + (SEG2 && KW >= 4)) * 64,
+                                 KIND == Q8_TREE && CT == 2 ? 2 : q8_occ(D, CT)) void k_attn8(Q8Params p, Q8Words tw) {
   constexpr bool WAVE2 = SEG2 && KW >= 4, LDS2 = SEG2 && KW < 4;
   constexpr int NW = KW * CW + WAVE2, COLS = 16 * CT;
   constexpr int PD = D + 4;                         // row pitch in LDS
@@ -663,7 +742,6 @@ __global__ __launch_bounds__((KW * CW + (SEG2 && KW >= 4)) * 64, 2) void k_attn8
   const float g0 = SEG2 || p.gates ? p.gates[0] : 1.0f;
   const float g1 = SEG2 ? p.gates[1] : 0.0f;
   if constexpr (LDS2) {
-    st.clear();
     q8_walk<D, KV_BF16, CT, Q8_ALL>(t.src2, 0, kw, KW, (p.T2 + 31) / 32, t.mask2(p.T2), p.c, t.qf, st, lane);
     if constexpr (KW > 1) {
       merge([&](int ct, float (&v)[DP], float mx, float sum) {
@@ -680,7 +758,7 @@ __global__ __launch_bounds__((KW * CW + (SEG2 && KW >= 4)) * 64, 2) void k_attn8
       }
     }
   }
-  st.clear();
+  st.clear();  // (for a wave that walks nothing)
   const bool second = WAVE2 && split == p.splits - 1;
   if (!extra) {
     const int per = (t.steps + p.splits - 1) / p.splits;
@@ -817,7 +895,7 @@ float q8_cost(int BH, int d2, bool i8, float last, float mean, float mem, int T2
   const float kConv = i8 ? 3.35f : 2.26f;
   const int cw = q8_cw(kw);
   const float cols = ct * (1.0f + 0.3f * (d2 - 1));
-  const int occ = d2 == 1 ? (ct == 1 ? 4 : ct == 2 ? 3 : 2) : 2;  // waves a SIMD has registers for
+  const int occ = q8_occ(64 * d2, ct);
   const int waves = kw * cw + (T2 > 0 && kw >= 4);
   const int per = occ * 4 / waves > 1 ? occ * 4 / waves : 1;      // workgroups a CU
   const float wgs = (float)BH * groups * S, rounds = wgs / ((float)cus * per);
