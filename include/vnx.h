@@ -881,9 +881,11 @@ int vnx_expert_gemm_bf16_rows(const void* x, int64_t ldx, int64_t sxb, const voi
  *     lens[b] + i, cache_dtype VNX_I8, VNX_E4M3 or VNX_BF16 (the values rounded;
  *     k_scale / v_scale not used).
  * Positions outside [0, cap) (and the tables) are skipped, their q_out rows
- * zero.  Batch rows and heads of the cache must not overlap (a stride 0 is
- * refused; reading takes it).  d in {16, 32, 64, 128, 256}; pointers 16-byte aligned, ldq and strides
- * multiples of 16 bytes.
+ * zero.  Rows that are written must not overlap: each of the batch, head and row
+ * strides (of more than one) steps over all that the smaller ones span, and keys
+ * and values do not meet (else VNX_ERR_INVALID_ARG; what is only read may
+ * overlap, a stride 0 included).  d in {16, 32, 64, 128, 256}; pointers 16-byte
+ * aligned, ldq and strides multiples of 16 bytes.
  * ------------------------------------------------------------------------- */
 typedef struct vnx_kv_write_args {
   const void* qkv;
@@ -912,7 +914,8 @@ int vnx_kv_write(const vnx_kv_write_args* args, void* stream);
 /* vnx_kv_read: k_out / v_out (B, Hkv, rows, d) in out_dtype (VNX_F32, VNX_BF16 or
  * VNX_F16, strides {batch, head, row} in elements, multiples of 16 bytes) = the
  * values that cache rows start[b] + i stand for (start NULL: 0), zeros outside
- * [0, cap).  VNX_I8, VNX_E4M3 or VNX_BF16 caches. */
+ * [0, cap).  VNX_I8, VNX_E4M3 or VNX_BF16 caches.  The outputs must not overlap
+ * (as above). */
 typedef struct vnx_kv_read_args {
   const void* k_cache;
   const void* v_cache;
@@ -951,7 +954,7 @@ int vnx_kv_read(const vnx_kv_read_args* args, void* stream);
  * path and gates, tri_sparse_attn.py:469-495, :585-608).
  * Query head h reads KV head h / (H / Hkv).  q bf16 (B, H, N, d), out VNX_BF16
  * or VNX_F16, strides {batch, head, row} multiples of 8, pointers 16-byte
- * aligned.  d in {64, 128}.  Tp + N <= cap.  Codes of e4m3 NaN must not stand in
+ * aligned, out's rows apart (VNX_ERR_INVALID_ARG).  d in {64, 128}.  Tp + N <= cap.  Codes of e4m3 NaN must not stand in
  * rows below tp_b + N (vnx_kv_write makes none).  One launch, or two when the
  * keys are split over workgroups: the workspace
  * (vnx_tree_attn_q8_workspace(args) bytes, no initialisation) then holds the

@@ -1079,6 +1079,7 @@ int vnx_tree_attn_q8(const vnx_attn_q8_args* a, void* workspace, size_t workspac
       (a->T2 > 0 && (!aligned16(a->k_seg2) || !aligned16(a->v_seg2))) || !aligned_to(a->gates, 4) ||
       !aligned_to(a->k_scale, 4) || !aligned_to(a->v_scale, 4) || !aligned_to(a->lens, 4) || !aligned_to(a->anc, 8))
     return VNX_ERR_UNSUPPORTED;
+  if (!Rows(a->d, a->out_strides, {a->B, a->H, a->N}).apart()) return VNX_ERR_INVALID_ARG;  // rows on one another
   const Q8Plan pl = q8_plan(a);
   Q8Params p{};
   p.slots = 1;

@@ -343,11 +343,6 @@ int vnx_kv_write(const vnx_kv_write_args* a, void* stream) {
   const int64_t HT = (int64_t)a->H + 2 * (int64_t)a->Hkv;
   if (a->ldq < HT * a->d || a->cache_strides[2] < a->d || a->scale_strides[0] < 0 || a->scale_strides[1] < 0)
     return VNX_ERR_INVALID_ARG;
-  // rows written must not lie on one another
-  const bool many = a->B > 1, heads = a->Hkv > 1;
-  if ((many && !a->cache_strides[0]) || (heads && !a->cache_strides[1]) ||
-      (q8 && ((many && !a->scale_strides[0]) || (heads && !a->scale_strides[1]))))
-    return VNX_ERR_INVALID_ARG;
   if (HT > INT_MAX || a->B > INT_MAX / a->n || a->B * a->n > (INT_MAX - 256) / HT) return VNX_ERR_UNSUPPORTED;
   // 16-byte loads and stores
   if (!aligned16(a->qkv) || a->ldq * elem_size(a->dtype) % 16 || !aligned16(a->q_out) || !aligned16(a->k_cache) ||
@@ -355,6 +350,11 @@ int vnx_kv_write(const vnx_kv_write_args* a, void* stream) {
       !aligned16(a->k_norm) || !strides16(a->cache_strides, q8 ? 1 : 2) || !aligned_to(a->lens, 4) ||
       !aligned_to(a->k_scale, 4) || !aligned_to(a->v_scale, 4))
     return VNX_ERR_UNSUPPORTED;
+  // rows written must not lie on one another
+  const Rows rows(a->d, a->cache_strides, {a->B, a->Hkv, a->cap}), scales(a->cap, a->scale_strides, {a->B, a->Hkv});
+  if (!rows.apart() || rows.meet(a->k_cache, a->v_cache, q8 ? 1 : 2) ||
+      (q8 && (!scales.apart() || scales.meet(a->k_scale, a->v_scale, 4))))
+    return VNX_ERR_INVALID_ARG;
   KvWriteParams p{};
   p.qkv = a->qkv; p.ldq = a->ldq; p.lens = a->lens;
   p.cos = a->cos_table; p.sin = a->sin_table; p.qn = a->q_norm; p.kn = a->k_norm;
@@ -389,6 +389,8 @@ int vnx_kv_read(const vnx_kv_read_args* a, void* stream) {
       !strides16(a->cache_strides, q8 ? 1 : 2) || !strides16(a->out_strides, elem_size(a->out_dtype)) ||
       !aligned_to(a->start, 4) || !aligned_to(a->k_scale, 4) || !aligned_to(a->v_scale, 4))
     return VNX_ERR_UNSUPPORTED;
+  const Rows out(a->d, a->out_strides, {a->B, a->Hkv, a->rows});
+  if (!out.apart() || out.meet(a->k_out, a->v_out, elem_size(a->out_dtype))) return VNX_ERR_INVALID_ARG;
   KvReadParams p{};
   p.c[0] = static_cast<const char*>(a->k_cache); p.c[1] = static_cast<const char*>(a->v_cache);
   p.s[0] = a->k_scale; p.s[1] = a->v_scale;

@@ -735,7 +735,8 @@ class HipBackend(DeviceBackend):
         (B, Hkv, cap) fp32) or bfloat16, written in place.  cos / sin (rows, d)
         rotate queries and keys; q_norm / k_norm (d,) norm every query / key
         head before that.  Positions outside the cache (or the tables) are
-        skipped and their queries zero."""
+        skipped and their queries zero.  No row of the caches (and scales) may
+        lie on another."""
         r = self._bind.kv_write(self._index, self._stream(), k_cache, v_cache, k_scale, v_scale, qkv, lens, cos, sin,
                                 q_norm, k_norm, eps)
         if r is not None:      # (None: a call that needs the general path's conversions or errors)
@@ -814,8 +815,8 @@ class HipBackend(DeviceBackend):
         (None: 1) still scales the result.  max_len: a bound of
         lens known to the caller (cap - N by default; longer lens are cut to
         it), from which the launch is sized.  Returns (B, H, N, d) bfloat16 or
-        float16, written into `out` (any strides with unit last stride) when
-        given."""
+        float16, written into `out` when given (rows apart from one another,
+        on 16 bytes, unit last stride)."""
         r = self._bind.tree_attn_q8(self._index, self._stream(), k_cache, v_cache, k_scale, v_scale, q, lens, anc,
                                     scale, seg2, gates, window, max_len, out_dtype, out)
         if r is not None:
