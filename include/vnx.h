@@ -981,6 +981,12 @@ typedef struct vnx_attn_q8_args {
   int B, H, Hkv, Tp, N, d;
   int T2, window, kv_dtype, out_dtype;
   float scale;
+  /* Tuning and tests: force_tiles (1-4 tiles of 16 query columns a wave, at most
+   * 2 for d = 128), force_waves (1, 2, 4 or 8 waves that share a tile's keys; a
+   * tree takes 4 or 8, a second segment at most 4) and force_splits (a power of
+   * two up to 32, for 4 waves and more) pin the launch shape; 0: the plan's
+   * choice.  Another value: VNX_ERR_UNSUPPORTED. */
+  int force_tiles, force_waves, force_splits;
 } vnx_attn_q8_args;
 
 size_t vnx_tree_attn_q8_workspace(const vnx_attn_q8_args* args);

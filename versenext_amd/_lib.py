@@ -212,7 +212,8 @@ class AttnQ8Args(ctypes.Structure):
         ("q_strides", _c_i64 * 3), ("cache_strides", _c_i64 * 3), ("scale_strides", _c_i64 * 2),
         ("out_strides", _c_i64 * 3), ("seg2_strides", _c_i64 * 3), ("anc_batch_stride", _c_i64), ("cap", _c_i64),
         ("B", _int), ("H", _int), ("Hkv", _int), ("Tp", _int), ("N", _int), ("d", _int), ("T2", _int),
-        ("window", _int), ("kv_dtype", _int), ("out_dtype", _int), ("scale", _f32),
+        ("window", _int), ("kv_dtype", _int), ("out_dtype", _int), ("scale", _f32), ("force_tiles", _int),
+        ("force_waves", _int), ("force_splits", _int),
     ]
 
 

@@ -932,17 +932,19 @@ Q8Plan q8_plan(const vnx_attn_q8_args* a) {
   const float mem = BH * (keys < W + a->N ? keys : W + a->N) * 2 * (a->d + 4) / 10.2e6f;
   Q8Plan best{1, 4, tiles, 1};
   float least = 1e30f;
-  const int most = tiles < 4 / d2 ? tiles : 4 / d2;
-  for (int ct = 1; ct <= most; ++ct) {
+  for (int ct = 1; ct <= 4 / d2; ++ct) {
+    if (a->force_tiles ? ct != a->force_tiles : ct > tiles) continue;
     const float span = (float)(16 * ct / rep + 2 < a->N ? 16 * ct / rep + 2 : a->N);  // rows of a tile
     const float end = tree ? (float)a->N : span;
     const float last = keys < W + end ? keys : W + end;
     const float mid = tree ? keys : (float)a->Tp + (a->N + span) / 2;
     const float mean = mid < W + end ? mid : W + end;
     for (int kw = tree ? 4 : 1; kw <= (a->T2 > 0 ? 4 : 8); kw *= 2) {
+      if (a->force_waves && kw != a->force_waves) continue;
       const int groups = (tiles + ct * q8_cw(kw) - 1) / (ct * q8_cw(kw));
       for (int S = 1; S <= (kw < 4 ? 1 : kQ8Split); S *= 2) {
-        if (S > 1 && ((int64_t)BH * groups * S > 6 * cus || last < 32 * S)) break;
+        if (a->force_splits ? S != a->force_splits : S > 1 && ((int64_t)BH * groups * S > 6 * cus || last < 32 * S))
+          continue;
         const float t = q8_cost(BH, d2, a->kv_dtype == VNX_I8, last, mean, mem, a->T2, cus, ct, kw, S, groups);
         if (t < least) {
           least = t;
@@ -979,6 +981,11 @@ int q8_check_sizes(const vnx_attn_q8_args* a) {
   if ((int64_t)a->Tp + a->N > a->cap) return VNX_ERR_INVALID_ARG;
   const bool tree = a->anc || a->anc_host;
   if (tree && (a->N > kQ8MaxN || (a->window > 0 && a->window < a->N))) return VNX_ERR_UNSUPPORTED;
+  // launch shapes that there are
+  const int ft = a->force_tiles, fw = a->force_waves, fs = a->force_splits;
+  if (ft < 0 || ft > 256 / a->d || (fw && fw != 1 && fw != 2 && fw != 4 && fw != 8) || (fw && fw < 4 && tree) ||
+      (fw > 4 && a->T2 > 0) || fs < 0 || fs > kQ8Split || (fs & (fs - 1)) || (fs > 1 && fw && fw < 4))
+    return VNX_ERR_UNSUPPORTED;
   // 32-bit row, column and workgroup numbers
   if (a->cap > INT_MAX - 64 || (int64_t)a->Tp + a->N > INT_MAX - 64 || a->T2 > INT_MAX - 64 ||
       (int64_t)a->H / a->Hkv * a->N > INT_MAX / 2 ||

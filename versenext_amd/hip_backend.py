@@ -803,7 +803,8 @@ class HipBackend(DeviceBackend):
 
     def tree_attention_q8(self, q, k_cache, v_cache, k_scale, v_scale, lens, anc=None, scale: float | None = None,
                           seg2=None, gates=None, window: int = 0, max_len: int | None = None,
-                          out_dtype=torch.bfloat16, out=None) -> torch.Tensor:
+                          out_dtype=torch.bfloat16, out=None, force_tiles: int = 0, force_waves: int = 0,
+                          force_splits: int = 0) -> torch.Tensor:
         """Attention of N new rows of every sequence over its 8-bit cache
         (vnx_tree_attn_q8), the new rows already written at rows lens[b] ..
         lens[b] + N - 1 (kv_write).
@@ -816,17 +817,20 @@ class HipBackend(DeviceBackend):
         lens known to the caller (cap - N by default; longer lens are cut to
         it), from which the launch is sized.  Returns (B, H, N, d) bfloat16 or
         float16, written into `out` when given (rows apart from one another,
-        on 16 bytes, unit last stride)."""
-        r = self._bind.tree_attn_q8(self._index, self._stream(), k_cache, v_cache, k_scale, v_scale, q, lens, anc,
-                                    scale, seg2, gates, window, max_len, out_dtype, out)
-        if r is not None:
-            return self._bound(r, "tree_attention_q8")
+        on 16 bytes, unit last stride).  force_tiles / force_waves /
+        force_splits pin the launch shape (tuning and tests)."""
+        force = (force_tiles, force_waves, force_splits)
+        if not any(force):
+            r = self._bind.tree_attn_q8(self._index, self._stream(), k_cache, v_cache, k_scale, v_scale, q, lens, anc,
+                                        scale, seg2, gates, window, max_len, out_dtype, out)
+            if r is not None:
+                return self._bound(r, "tree_attention_q8")
         with torch.cuda.device(self._index):
             return self._tree_attention_q8(q, k_cache, v_cache, k_scale, v_scale, lens, anc, scale, seg2, gates, window,
-                                           max_len, out_dtype, out)
+                                           max_len, out_dtype, out, force)
 
     def _tree_attention_q8(self, q, k_cache, v_cache, k_scale, v_scale, lens, anc, scale, seg2, gates, window, max_len,
-                           out_dtype, out):
+                           out_dtype, out, force):
         dev = self._torch_device
         B, Hkv, cap, d, code, ss = self._kv_cache(k_cache, v_cache, k_scale, v_scale, self._KV_DTYPES[:2])
         qt = self._heads_bf16(q, "q")
@@ -877,7 +881,7 @@ class HipBackend(DeviceBackend):
             _ptr(k2) or 0, _ptr(v2) or 0, _ptr(g) or 0, *qt.stride()[:3], *k_cache.stride()[:3], *ss,
             *out.stride()[:3], *s2, N if a is not None and a.ndim == 2 else 0, cap, B, H, Hkv, Tp, N, d,
             k2.shape[2] if k2 is not None else 0, int(window), code, _lib.DTYPE_CODES[out.dtype],
-            float(scale) if scale is not None else d ** -0.5)
+            float(scale) if scale is not None else d ** -0.5, *(int(f) for f in force))
         # a workspace of this call's own: a captured graph keeps it in its pool
         need = self._L.vnx_tree_attn_q8_workspace(args)
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 256 else None
