@@ -10,6 +10,7 @@ import ctypes
 import os
 import struct
 import threading
+import warnings
 
 _PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG_DIR, "libvnx_hip.so")
@@ -283,7 +284,8 @@ _bind = None
 
 def bind():
     """The _vnx_bind module (csrc/bind.cpp), pointed at the loaded library's
-    entries (raises RuntimeError if it is not built)."""
+    entries (raises RuntimeError if it is not built, or not for this PyTorch
+    and library)."""
     global _bind
     if _bind is not None:
         return _bind
@@ -293,12 +295,38 @@ def bind():
     except ImportError as e:
         raise RuntimeError(f"vnx binding not found in {_PKG_DIR} ({e}); build it with "
                            "`python -m versenext_amd.build`") from e
+    built = (getattr(_vnx_bind, "torch", None), getattr(_vnx_bind, "sizes", None))
+    here = (_torch.__version__, tuple(ctypes.sizeof(c) for c in (KvWriteArgs, KvReadArgs, AttnQ8Args)))
+    if built != here:
+        raise RuntimeError(f"vnx binding in {_PKG_DIR} was built for {built}, this is {here}; build it again with "
+                           "`python -m versenext_amd.build`")
     with _lock:
         if _bind is None:
             _vnx_bind.init(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
                 L.vnx_kv_write, L.vnx_kv_read, L.vnx_tree_attn_q8_workspace, L.vnx_tree_attn_q8)))
             _bind = _vnx_bind
     return _bind
+
+
+class NoBind:
+    """In the binding's place where there is none: leaves every call to the
+    general path, as the binding leaves those that it does not serve."""
+    @staticmethod
+    def kv_write(*args):
+        return None
+
+    kv_read = tree_attn_q8 = kv_write
+
+
+def bind_or_none():
+    """bind(), or with a RuntimeWarning NoBind: the binding saves host time
+    only, and the library has all that its calls do."""
+    try:
+        return bind()
+    except RuntimeError as e:
+        warnings.warn(f"{e}; kv_write, kv_read and tree_attention_q8 take their checks in Python", RuntimeWarning,
+                      stacklevel=2)
+        return NoBind
 
 
 def check(status: int, what: str = "vnx call") -> None:

@@ -9,6 +9,7 @@ import os
 import shutil
 import subprocess
 import sys
+import warnings
 from concurrent.futures import ThreadPoolExecutor
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
@@ -57,11 +58,15 @@ def build_bind(verbose: bool = False) -> str:
     lib = os.path.join(os.path.dirname(torch.__file__), "lib")
     tmp = BIND_PATH + ".tmp"
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-fvisibility=hidden",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *inc, os.path.join(CSRC, "bind.cpp"),
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f'-DVNX_BIND_TORCH="{torch.__version__}"', *inc, os.path.join(CSRC, "bind.cpp"),
            "-o", tmp, f"-L{lib}", f"-Wl,-rpath,{lib}", "-ltorch_python", "-ltorch_cpu", "-lc10"]
     if verbose:
         print(" ".join(cmd), flush=True)
-    res = subprocess.run(cmd, capture_output=True, text=True)
+    try:
+        res = subprocess.run(cmd, capture_output=True, text=True)
+    except OSError as e:
+        raise RuntimeError(f"the binding's compiler: {e}") from e
     if res.returncode != 0:
         raise RuntimeError(f"the binding did not compile:\n{res.stdout}\n{res.stderr}")
     os.replace(tmp, BIND_PATH)
@@ -70,7 +75,9 @@ def build_bind(verbose: bool = False) -> str:
 
 def build_library(verbose: bool = False, jobs: int | None = None) -> str:
     """Compiles every csrc/*.hip for gfx950 and links LIB_PATH, and the Python
-    binding beside it (build_bind). Returns LIB_PATH."""
+    binding beside it (build_bind). Returns LIB_PATH. Without g++ or the headers
+    of Python and PyTorch the library is built all the same, with a warning:
+    it does not need the binding, and an older one goes."""
     hipcc = _hipcc()
     os.makedirs(OBJ_DIR, exist_ok=True)
     srcs = sources()
@@ -92,13 +99,16 @@ def build_library(verbose: bool = False, jobs: int | None = None) -> str:
         for warn in ex.map(compile_one, zip(srcs, objs)):
             if verbose and warn:
                 print(warn, file=sys.stderr)
-        bind.result()
     tmp = LIB_PATH + ".tmp"
     cmd = [hipcc, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp, *objs]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
     os.replace(tmp, LIB_PATH)
+    if bind.exception() is not None:
+        if os.path.exists(BIND_PATH):
+            os.remove(BIND_PATH)
+        warnings.warn(f"{LIB_NAME} is built, its Python binding is not: {bind.exception()}", RuntimeWarning)
     return LIB_PATH
 
 

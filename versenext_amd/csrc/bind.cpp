@@ -336,4 +336,22 @@ PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_vnx_bind", nullptr, -1, kMethods
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__vnx_bind() { return PyModule_Create(&kModule); }
+// .torch: the PyTorch it was compiled against; .sizes: of the argument blocks
+// that it fills.  Another PyTorch, or another library, must not get them.
+PyMODINIT_FUNC PyInit__vnx_bind() {
+  PyObject* m = PyModule_Create(&kModule);
+  if (!m) return nullptr;
+  PyObject* sizes =
+      Py_BuildValue("(nnn)", (Py_ssize_t)sizeof(vnx_kv_write_args), (Py_ssize_t)sizeof(vnx_kv_read_args),
+                    (Py_ssize_t)sizeof(vnx_attn_q8_args));
+  if (!sizes || PyModule_AddObject(m, "sizes", sizes) < 0) {  // (takes sizes when it succeeds)
+    Py_XDECREF(sizes);
+    Py_DECREF(m);
+    return nullptr;
+  }
+  if (PyModule_AddStringConstant(m, "torch", VNX_BIND_TORCH) < 0) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}

@@ -63,7 +63,7 @@ class HipBackend(DeviceBackend):
         with torch.cuda.device(idx):
             _lib.check(L.vnx_init(idx), "vnx_init")
         self._L = L
-        self._bind = _lib.bind()
+        self._bind = _lib.bind_or_none()
         self._ws = {}
         self._ws_lock = threading.Lock()
 
