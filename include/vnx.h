@@ -884,7 +884,8 @@ int vnx_expert_gemm_bf16_rows(const void* x, int64_t ldx, int64_t sxb, const voi
  * zero.  Rows that are written must not overlap: each of the batch, head and row
  * strides (of more than one) steps over all that the smaller ones span, and keys
  * and values do not meet (else VNX_ERR_INVALID_ARG; what is only read may
- * overlap, a stride 0 included).  d in {16, 32, 64, 128, 256}; pointers 16-byte
+ * overlap, a stride 0 included).  Sizes whose launch would need 2^32 threads
+ * (B * n of 2^26 tokens) are VNX_ERR_UNSUPPORTED, in all three calls.  d in {16, 32, 64, 128, 256}; pointers 16-byte
  * aligned, ldq and strides multiples of 16 bytes.
  * ------------------------------------------------------------------------- */
 typedef struct vnx_kv_write_args {

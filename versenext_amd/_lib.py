@@ -235,7 +235,13 @@ def _packer(cls):
     s = struct.Struct(fmt)
     if s.size != ctypes.sizeof(cls):
         raise AssertionError(f"{cls.__name__}: {s.size} bytes packed, {ctypes.sizeof(cls)} declared")
-    return s.pack
+
+    def pack(*values):
+        try:
+            return s.pack(*values)
+        except struct.error as e:   # (a value that its field does not hold)
+            raise ValueError(f"{cls.__name__}: {e}") from None
+    return pack
 
 
 pack_kv_write = _packer(KvWriteArgs)

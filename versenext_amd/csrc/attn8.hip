@@ -989,7 +989,7 @@ int q8_check_sizes(const vnx_attn_q8_args* a) {
   // 32-bit row, column and workgroup numbers
   if (a->cap > INT_MAX - 64 || (int64_t)a->Tp + a->N > INT_MAX - 64 || a->T2 > INT_MAX - 64 ||
       (int64_t)a->H / a->Hkv * a->N > INT_MAX / 2 ||
-      (int64_t)a->B * a->Hkv * (((int64_t)a->H / a->Hkv * a->N + 15) / 16) * kQ8Split > INT_MAX)
+      (__int128)a->B * a->Hkv * (((int64_t)a->H / a->Hkv * a->N + 15) / 16) * kQ8Split > INT_MAX)
     return VNX_ERR_UNSUPPORTED;
   return VNX_OK;
 }
@@ -1088,6 +1088,10 @@ int vnx_tree_attn_q8(const vnx_attn_q8_args* a, void* workspace, size_t workspac
     return VNX_ERR_UNSUPPORTED;
   if (!Rows(a->d, a->out_strides, {a->B, a->H, a->N}).apart()) return VNX_ERR_INVALID_ARG;  // rows on one another
   const Q8Plan pl = q8_plan(a);
+  const int64_t units = (int64_t)a->B * a->Hkv * pl.groups;
+  if (!launch_fits(units * pl.splits, 64 * (pl.kw * q8_cw(pl.kw) + (a->T2 > 0 && pl.kw >= 4))) ||
+      (pl.splits > 1 && !launch_fits(units * 4 * pl.ct, 256)))
+    return VNX_ERR_UNSUPPORTED;
   Q8Params p{};
   p.slots = 1;
   const size_t need = q8_ws_bytes(a, pl, &p, workspace);

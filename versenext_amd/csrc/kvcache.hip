@@ -305,8 +305,9 @@ int kv_write_launch(KvWriteParams p, int d, hipStream_t st) {
     p.per = (int64_t)p.tokens * groups <= 16 * (int64_t)device_cus() ? 1 : groups;
     p.chunks = (groups + p.per - 1) / p.per;
     p.past = (int64_t)p.tokens * p.H * d * 2 >= (64 << 20);
-    const unsigned grid = (unsigned)(((int64_t)p.tokens * p.chunks + 3) / 4);
-    hipLaunchKernelGGL((k_kv_write<TS, KT, L>), dim3(grid), dim3(256), 0, st, p);
+    const int64_t grid = ((int64_t)p.tokens * p.chunks + 3) / 4;
+    if (!launch_fits(grid, 256)) return (int)VNX_ERR_UNSUPPORTED;
+    hipLaunchKernelGGL((k_kv_write<TS, KT, L>), dim3((unsigned)grid), dim3(256), 0, st, p);
     VNX_LAUNCH_CHECK();
     return (int)VNX_OK;
   });
@@ -406,8 +407,9 @@ int vnx_kv_read(const vnx_kv_read_args* a, void* stream) {
     constexpr int KT = decltype(kt)::value;
     return by_lanes<2, 32>(a->d / 8, [&](auto l) {
       constexpr int L = decltype(l)::value;
-      const unsigned gx = (unsigned)(((int64_t)p.rows + 256 / L - 1) / (256 / L));
-      hipLaunchKernelGGL((k_kv_read<TO, KT, L>), dim3(gx, (unsigned)(p.BH < 65535 ? p.BH : 65535), 2), dim3(256), 0,
+      const int64_t gx = ((int64_t)p.rows + 256 / L - 1) / (256 / L);
+      if (!launch_fits(gx, 256)) return (int)VNX_ERR_UNSUPPORTED;
+      hipLaunchKernelGGL((k_kv_read<TO, KT, L>), dim3((unsigned)gx, (unsigned)(p.BH < 65535 ? p.BH : 65535), 2), dim3(256), 0,
                          st, p);
       VNX_LAUNCH_CHECK();
       return (int)VNX_OK;

@@ -71,6 +71,9 @@ struct Carve {
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// A launch of `wgs` workgroups of `threads`: HIP takes fewer than 2^32 threads.
+inline bool launch_fits(int64_t wgs, int threads) { return wgs <= UINT32_MAX / threads; }
+
 inline int elem_size(int dtype) { return dtype == VNX_F32 ? 4 : 2; }
 
 // Zeroes n arrival counters on `st` (a kernel, not a memset, so the call
