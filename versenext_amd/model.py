@@ -670,7 +670,8 @@ class CometSparkGPU:
             gv = (g @ wv_g.t()).reshape(G, cfg.n_kv_head, d).permute(1, 0, 2).unsqueeze(0)
             L = _Layer(kind=kind, norm1=W[p + "norm1.weight"], norm2=W[p + "norm2.weight"],
                        wqkv=_Linear(_cat([wq, wk, wv]), dtype, hip, int4,
-                                    rope_head_dim=d if dtype == torch.bfloat16 and int4 else 0),
+                                    # (for the GEMVs that write bf16 cache rows: not with an 8-bit cache)
+                                    rope_head_dim=d if dtype == torch.bfloat16 and int4 and kv_dtype is None else 0),
                        proj=_Linear(W[p + "attn.proj.weight"], dtype, hip, int4),
                        gk=gk.to(dtype).contiguous(), gv=gv.to(dtype).contiguous(),
                        gates=torch.sigmoid(W[p + "attn.gate_logits"].float()).contiguous())
@@ -1120,7 +1121,8 @@ class CometSparkGPU:
                           (L.ffn["gu"].wp is not None and L.ffn["gu"].swiglu and L.ffn["down"].wp is not None)))
             norm_in = fused and M <= _Linear.GEMM_MAX_M and D <= 2048
             # the INT4 draft's decode: the same fusions on its GEMVs
-            qfused = (not fused and L.kind == "trisparse" and L.wqkv.wq_rope is not None and L.proj.int4
+            qfused = (not fused and L.kind == "trisparse"
+                      and (L.wqkv.int4 if kv8 else L.wqkv.wq_rope is not None) and L.proj.int4
                       and L.ffn["gu"].int4 and L.ffn["gu"].swiglu and L.ffn["down"].int4 and M <= 64
                       and pending is None)
             h = None
