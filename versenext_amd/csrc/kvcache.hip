@@ -17,7 +17,7 @@
 // and the maximum one reduction over the head's lanes.
 // vnx_kv_read: codes * scale of a range of rows.
 // Both are bound by HBM where the rows are many (on the GPU: 16,384 tokens x 48
-// heads of 128 with norms, int8, 73 us for 371 MB, 5.1 TB/s; 131,072 rows x 8
+// heads of 128 with norms, int8, 71 us for 371 MB, 5.2 TB/s; 131,072 rows x 8
 // heads of 128 from e4m3, 151 us, 5.4 TB/s; a large copy runs at 5.3) and by the
 // launch elsewhere (one token: 2.8 us and 2.9).
 #include <climits>
@@ -47,7 +47,6 @@ struct KvWriteParams {
   int64_t cap;               // rows below cap (and the tables') are written
   uint32_t tokens;           // B * n
   int chunks, per;           // waves a token, head groups a wave
-  int past;                  // queries past the caches
   int n, H, Hkv;
   float eps;
 };
@@ -59,7 +58,10 @@ __device__ __forceinline__ void kv_ld8(const T* p, float (&v)[8]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
   } else {
-    const u32x4 a = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));  // (read once)
+    // 16-bit rows are read once (past the caches 71.1 us, else 77.1 for 16,384
+    // tokens x 48 heads of 128; fp32 rows come through the loads of the tables
+    // and norms, which are read again)
+    const u32x4 a = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if constexpr (__is_same(T, _Float16)) {
@@ -181,13 +183,8 @@ __global__ __launch_bounds__(256) void k_kv_write(KvWriteParams p) {
       uint16_t* o = p.q + (((int64_t)b * p.H + head) * p.n + i) * D + lane * 8;
       u32x4 x = kv_bf16x8(lo), y = kv_bf16x8(hi);
       if (!in) x = y = u32x4{0, 0, 0, 0};  // a position outside the cache: zeros
-      if (p.past) {
-        __builtin_nontemporal_store(x, reinterpret_cast<u32x4*>(o));
-        __builtin_nontemporal_store(y, reinterpret_cast<u32x4*>(o + HD));
-      } else {
-        *reinterpret_cast<u32x4*>(o) = x;
-        *reinterpret_cast<u32x4*>(o + HD) = y;
-      }
+      *reinterpret_cast<u32x4*>(o) = x;
+      *reinterpret_cast<u32x4*>(o + HD) = y;
       continue;
     }
     const int kvh = head - p.H - (is_v ? p.Hkv : 0);
@@ -298,13 +295,10 @@ int kv_write_launch(KvWriteParams p, int d, hipStream_t st) {
   return by_lanes<1, 16>(d / 16, [&](auto l) {
     constexpr int L = decltype(l)::value;
     // a wave a head group while that leaves the chip room (16 waves a CU), else a
-    // token's all (us, 16,384 tokens x 48 heads of 128 with norms: 83 / 81).
-    // Queries that no cache will hold until they are read go past it (81 / 77
-    // together with the inputs, which are read once and always do).
+    // token's all (us, 16,384 tokens x 48 heads of 128 with norms: 82.7 / 71.1)
     const int groups = (p.H + 2 * p.Hkv + 64 / L - 1) / (64 / L);
     p.per = (int64_t)p.tokens * groups <= 16 * (int64_t)device_cus() ? 1 : groups;
     p.chunks = (groups + p.per - 1) / p.per;
-    p.past = (int64_t)p.tokens * p.H * d * 2 >= (64 << 20);
     const int64_t grid = ((int64_t)p.tokens * p.chunks + 3) / 4;
     if (!launch_fits(grid, 256)) return (int)VNX_ERR_UNSUPPORTED;
     hipLaunchKernelGGL((k_kv_write<TS, KT, L>), dim3((unsigned)grid), dim3(256), 0, st, p);
