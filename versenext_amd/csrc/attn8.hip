@@ -30,10 +30,10 @@
 // and no rescaling.
 //
 // Long caches with few rows are bound by HBM (8 x 5 rows over 16,000 keys, heads
-// of 128: 46.8 us for 269 MB, 5.7 TB/s, and 4.7 for the join), prompts by the
-// vector ALU's issue rate beside the products (2,048 rows over 8,192: 109-112 us,
+// of 128: 46.8 us for 269 MB, 5.7 TB/s, and 4.8 for the join), prompts by the
+// vector ALU's issue rate beside the products (2,048 rows over 8,192: 110-112 us,
 // 0.7 PFLOP/s of the 1.17 of a large bf16 product), small steps by launch,
-// prologue and merge (32 x 7 rows over 617: 7.4 us, 5 of them with no key).
+// prologue and merge (32 x 7 rows over 617: 7.9 us).
 #include <climits>
 
 #include "kvcache.h"
@@ -666,8 +666,9 @@ __device__ __forceinline__ int64_t q8_out_off(const Q8Params& p, int b, int kvh,
 // weighted result kept in LDS meanwhile (KW = 1: by the lane, else by the
 // thread that adds it again); for KW >= 4 (few steps a wave) a wave of its own
 // walks it beside the others, in the last split.  (us, 32 x 7 rows over 617,
-// 128 global rows: 7.8 with that wave, 10.1 walked first; 4 x 512 rows, KW = 2:
-// 18.1 walked first, 26 with the wave and KW = 4.)
+// 128 global rows: 8.2 with that wave at KW = 4, 13.2 walked first at KW = 2; the
+// same KW both ways on an earlier build 7.8 and 10.1.  4 x 512 rows: 17.0 walked first at
+// KW = 2, 23.9 with the wave at KW = 4, 4 tiles.)
 // Waves a SIMD has registers for.
 constexpr int q8_occ(int d, int ct) { return d == 64 && ct <= 2 ? 5 - ct : 2; }
 
@@ -885,9 +886,12 @@ constexpr int q8_cw(int kw) { return kw == 1 ? 4 : kw == 2 ? 2 : 1; }
 // second launch joins splits.  The constants are fitted to 1,700 timings of 70
 // shapes (1-64 sequences, 1-1,500 new rows, 1-16,000 keys, both head sizes); of 67
 // others it picks the fastest launch shape within 2% on average and 21% at
-// worst.  us, 16 trees of 40 nodes over 2,048 rows: ct 3 x 8 waves 18.8, ct 1 x 4
-// waves 23.5; 4 prompts of 512: ct 2 x 2 waves 18.1, ct 4 x 4 waves 24.6; 8 x 5 rows
-// over 16,000, heads of 128: ct 2 x 4 splits 55.6, no split 139, ct 1 x 4 splits 76.
+// worst.  The constants stand for nothing but that fit (mem's 10.2 TB/s is no rate
+// of the memory), and the kernel has gained a test a step since; what is measured
+// on it, us: 16 trees of 40 nodes over 2,048 rows ct 3 x 8 waves 18.9, ct 3 x 4 20.5,
+// ct 1 x 4 21.5, ct 2 x 8 25.8; 4 prompts of 512 ct 2 x 2 waves 17.0, ct 4 x 2 21.2, ct 4 x 4
+// 23.9; 8 x 5 rows over 16,000, heads of 128, ct 2 x 4 splits 50.1, no split 130,
+// ct 1 x 4 splits 72.9; 2,048 rows over 8,192 ct 4 x 4 waves 111.4, ct 3 x 4 132, ct 4 x 1 287.
 float q8_cost(int BH, int d2, bool i8, float last, float mean, float mem, int T2, int cus, int ct, int kw, int S,
               int groups) {
   constexpr float kMerge = 0.813f, kLone = 1.66f, kJoin = 1.09f, kPart = 5.9e-3f, kStep = 0.078f, kCol = 0.252f,
@@ -1003,7 +1007,7 @@ inline bool q8_strides(const int64_t* s, int n, int64_t unit) {
 template <int D, int KT, int CT, int KIND, bool SEG2>
 void q8_launch(const Q8Params& p, const Q8Words& tw, const Q8Plan& pl, hipStream_t st) {
   const dim3 grid((unsigned)(p.B * p.Hkv * pl.groups * pl.splits));
-  if constexpr (KIND == Q8_CHAIN) {  // (a tree's 64 nodes make few columns)
+  if constexpr (KIND == Q8_CHAIN) {  // (a tree's walk is no shorter in its first column groups: 4 waves and more)
     if (pl.kw == 1) {
       hipLaunchKernelGGL((k_attn8<D, KT, CT, KIND, SEG2, 1, 4>), grid, dim3(256), 0, st, p, tw);
       return;
@@ -1025,7 +1029,7 @@ void q8_launch(const Q8Params& p, const Q8Words& tw, const Q8Plan& pl, hipStream
   };
   // Rows that one column group reads go past the caches from 192 MiB on, where
   // the next layer's rows push them out before they are read again.  us past /
-  // cached, 5 rows a sequence, heads of 128, two caches read in turn: 125 MiB
+  // cached (before q8_steps tested the scales), 5 rows a sequence, heads of 128, two caches read in turn: 125 MiB
   // 32.3 / 29.7, 156 51.1 / 49.1, 188 49.1 / 49.0, 219 49.8 / 51.3, 250 51.8 /
   // 56.1, 500 (heads of 64) 93.1 / 101.7.  A single cache read again at once
   // keeps more: 250 MiB 51.4 / 48.2.  Rows that several groups read lose (16
