@@ -175,3 +175,14 @@ def test_refusals(hip):
                dict(force_waves=2, anc=[1]), dict(force_waves=8, seg2=(s2, s2), gates=[1.0, 1.0])):
         with pytest.raises(ValueError):
             hip.tree_attention_q8(q, kc, kc, ks, ks, [3], **kw)
+
+
+@pytest.mark.parametrize("dtype", [I8, E4], ids=["int8", "e4m3"])
+@pytest.mark.parametrize("d,H,Hkv,N,lens,tree,window,G", [
+    (64, 40, 1, 3, [90, 0], None, 0, 0), (128, 33, 1, 1, [200, 31], None, 17, 3), (64, 34, 2, 70, [5, 64], None, 33, 40),
+    (64, 24, 1, 0, [100, 3], (4, 3, 2), 40, 0), (128, 32, 2, 0, [64, 0], (2, 2, 2, 2), 30, 9)])
+def test_many_query_heads_to_a_kv_head(hip, d, H, Hkv, N, lens, tree, window, G, dtype):
+    """17 to 40 query heads a KV head, so a column tile holds one node or a part of one; trees with the smallest window."""
+    words = [int(w) for w in VT.ancestor_words(VT.tree_from_branching(list(tree)))] if tree else None
+    _case(hip, d, dtype, H, Hkv, len(words) if tree else N, lens, words, window, G,
+          [(0, 0, 0), (1, 4, 1), (2, 4, 4)] + ([] if tree else [(1, 1, 1), (2, 2, 1)]), H)
