@@ -993,6 +993,67 @@ typedef struct vnx_attn_q8_args {
 size_t vnx_tree_attn_q8_workspace(const vnx_attn_q8_args* args);
 int vnx_tree_attn_q8(const vnx_attn_q8_args* args, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Products in 8-bit integers.  A row t of K values is held as K int8 codes and
+ * one fp32 scale,
+ *   a = max|t|,  code = rint(t * RN(127 / a)),  scale = RN(a / 127)
+ * (nearest, ties to even), and stands for code * scale.  A row whose maximum is
+ * below 2^-100 has codes and scale 0; one with an infinity or a NaN has codes 0
+ * and scale NaN.  Matrices row-major with the given row pitches (elements).
+ * The weight-only INT8 of quantize.py:187-214 holds its weights this way; the
+ * reference has no counterpart that quantises the activations.
+ *
+ * vnx_q8_quantize: codes and scales of rows x (M, K), VNX_F32 / VNX_BF16 /
+ * VNX_F16.
+ *
+ * vnx_q8_rmsnorm: s = x + res (fp32, rounded to x's dtype; res in its own
+ * dtype, NULL: s = x), written to sum (x's dtype; NULL: not; it may be the very
+ * rows of x or of res), then the codes of t = s * w and
+ *   scale = RN(a / 127) / sqrt(mean(s^2) + eps),  a = max|t|:
+ * RMSNorm (packages/verse_torch/verse_torch/vnnn.py:593-615) of the residual
+ * stream, its factor in the scale alone.  A row whose squares sum past fp32's
+ * range has scale NaN.
+ *
+ * vnx_q8_dequantize: out (M, K) in out_dtype = code * scale.
+ * No output may share bytes with an input but as said (VNX_ERR_INVALID_ARG).
+ * ------------------------------------------------------------------------- */
+int vnx_q8_quantize(const void* x, int dtype, int64_t ldx, int64_t M, int64_t K, int8_t* codes, int64_t ldc,
+                    float* scale, void* stream);
+
+int vnx_q8_rmsnorm(const void* x, int dtype, int64_t ldx, const void* res, int res_dtype, int64_t ldr, const float* w,
+                   float eps, int64_t M, int64_t K, void* sum, int64_t lds, int8_t* codes, int64_t ldc, float* scale,
+                   void* stream);
+
+int vnx_q8_dequantize(const int8_t* codes, int64_t ldc, const float* scale, int64_t M, int64_t K, void* out,
+                      int out_dtype, int64_t ldo, void* stream);
+
+/* vnx_q8_linear: of rows x (M, K) and W (N, K) of such codes, with
+ *   acc[m, n] = sum_k x[m, k] * W[n, k]   (exact in 32 bits: K <= 131,071)
+ *   v[m, n] = acc[m, n] * x_scale[m] * w_scale[n] (+ bias[n])   (fp32)
+ * VNX_EPI_NONE: y (M, N) = v (+ res[m, n], in its own dtype, added in fp32; res
+ * may be y itself).  VNX_EPI_SWIGLU: W holds N / 2 gate rows, then N / 2 up rows
+ * in the same order; y (M, N / 2) = silu(v[m, n]) * v[m, N / 2 + n] (SwiGLUMLP,
+ * vnnn.py:779-807), no res.  y and res VNX_F32, VNX_BF16 or VNX_F16, rounded
+ * once.  x and W on 16 bytes with pitches a multiple of 16 (below 2^22); bytes
+ * of a row between K and its pitch are not used, whatever they hold.  y must not
+ * share bytes with what is read but as said.  Codes may be -128.  force_shape
+ * (tuning and tests): 1 + the index of a launch shape; 0: the plan's choice,
+ * another value VNX_ERR_UNSUPPORTED. */
+typedef struct vnx_q8_linear_args {
+  const int8_t* x;
+  const float* x_scale;
+  const int8_t* w;
+  const float* w_scale;
+  const float* bias;
+  const void* res;
+  void* y;
+  int64_t ldx, ldw, ldr, ldy;
+  int64_t M, N, K;
+  int res_dtype, y_dtype, epilogue, force_shape;
+} vnx_q8_linear_args;
+
+int vnx_q8_linear(const vnx_q8_linear_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

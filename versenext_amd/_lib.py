@@ -218,7 +218,21 @@ class AttnQ8Args(ctypes.Structure):
     ]
 
 
+class Q8LinearArgs(ctypes.Structure):
+    """vnx_q8_linear_args (include/vnx.h)."""
+    _fields_ = [
+        ("x", _vp), ("x_scale", _vp), ("w", _vp), ("w_scale", _vp), ("bias", _vp), ("res", _vp), ("y", _vp),
+        ("ldx", _c_i64), ("ldw", _c_i64), ("ldr", _c_i64), ("ldy", _c_i64), ("M", _c_i64), ("N", _c_i64),
+        ("K", _c_i64), ("res_dtype", _int), ("y_dtype", _int), ("epilogue", _int), ("force_shape", _int),
+    ]
+
+
 SIGNATURES.update({
+    "vnx_q8_quantize": (_int, [_vp, _int, _c_i64, _c_i64, _c_i64, _vp, _c_i64, _vp, _vp]),
+    "vnx_q8_rmsnorm": (_int, [_vp, _int, _c_i64, _vp, _int, _c_i64, _vp, _f32, _c_i64, _c_i64, _vp, _c_i64, _vp,
+                              _c_i64, _vp, _vp]),
+    "vnx_q8_dequantize": (_int, [_vp, _c_i64, _vp, _c_i64, _c_i64, _vp, _int, _c_i64, _vp]),
+    "vnx_q8_linear": (_int, [_vp, _vp]),
     "vnx_kv_write": (_int, [_vp, _vp]),
     "vnx_kv_read": (_int, [_vp, _vp]),
     "vnx_tree_attn_q8_workspace": (_c_sz, [_vp]),
@@ -247,6 +261,7 @@ def _packer(cls):
 pack_kv_write = _packer(KvWriteArgs)
 pack_kv_read = _packer(KvReadArgs)
 pack_attn_q8 = _packer(AttnQ8Args)
+pack_q8_linear = _packer(Q8LinearArgs)
 
 
 def stream_handle(index: int) -> int:
@@ -301,8 +316,9 @@ def bind():
     except ImportError as e:
         raise RuntimeError(f"vnx binding not found in {_PKG_DIR} ({e}); build it with "
                            "`python -m versenext_amd.build`") from e
-    built = (getattr(_vnx_bind, "torch", None), getattr(_vnx_bind, "sizes", None))
-    here = (_torch.__version__, tuple(ctypes.sizeof(c) for c in (KvWriteArgs, KvReadArgs, AttnQ8Args)))
+    built = tuple(getattr(_vnx_bind, a, None) for a in ("torch", "sizes", "q8_size"))
+    here = (_torch.__version__, tuple(ctypes.sizeof(c) for c in (KvWriteArgs, KvReadArgs, AttnQ8Args)),
+            ctypes.sizeof(Q8LinearArgs))
     if built != here:
         raise RuntimeError(f"vnx binding in {_PKG_DIR} was built for {built}, this is {here}; build it again with "
                            "`python -m versenext_amd.build`")
@@ -310,6 +326,8 @@ def bind():
         if _bind is None:
             _vnx_bind.init(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
                 L.vnx_kv_write, L.vnx_kv_read, L.vnx_tree_attn_q8_workspace, L.vnx_tree_attn_q8)))
+            _vnx_bind.init_q8(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
+                L.vnx_q8_quantize, L.vnx_q8_rmsnorm, L.vnx_q8_dequantize, L.vnx_q8_linear)))
             _bind = _vnx_bind
     return _bind
 
@@ -321,7 +339,7 @@ class NoBind:
     def kv_write(*args):
         return None
 
-    kv_read = tree_attn_q8 = kv_write
+    kv_read = tree_attn_q8 = q8_quantize = q8_rmsnorm = q8_dequantize = q8_linear = kv_write
 
 
 def bind_or_none():
@@ -330,7 +348,7 @@ def bind_or_none():
     try:
         return bind()
     except RuntimeError as e:
-        warnings.warn(f"{e}; kv_write, kv_read and tree_attention_q8 take their checks in Python", RuntimeWarning,
+        warnings.warn(f"{e}; the calls of the 8-bit cache and of 8-bit rows take their checks in Python", RuntimeWarning,
                       stacklevel=2)
         return NoBind
 

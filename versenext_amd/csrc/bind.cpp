@@ -1,6 +1,7 @@
-// Python binding of the 8-bit KV cache's entries: _vnx_bind.kv_write, kv_read
-// and tree_attn_q8 take tensors, check them, allocate the results and call the
-// C entries of vnx.h, in 1-2 us of host time a call beside the launch's
+// Python binding of the 8-bit KV cache's entries and of the products in 8-bit
+// integers: _vnx_bind.kv_write, kv_read, tree_attn_q8, q8_quantize, q8_rmsnorm,
+// q8_dequantize and q8_linear take tensors, check them, allocate the results and
+// call the C entries of vnx.h, in 1-2 us of host time a call beside the launch's
 // 3.5, where the same checks in Python take 7-13 (a decode step's kernels take 3-9 us).
 //
 // Each function serves the call whose arguments the kernels read as they are.
@@ -16,6 +17,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <climits>
 #include <cmath>
 
@@ -307,18 +309,230 @@ PyObject* tree_attn_q8(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- products in 8-bit integers ----
+
+decltype(&vnx_q8_quantize) g_quantize;
+decltype(&vnx_q8_rmsnorm) g_rmsnorm;
+decltype(&vnx_q8_dequantize) g_dequantize;
+decltype(&vnx_q8_linear) g_linear;
+
+// (rows, K) with unit last stride and rows that follow each other: its pitch in
+// elements, 0 where it is not.
+int64_t pitch_of(const at::Tensor& t) {
+  if (t.dim() != 2 || t.size(1) < 1 || (t.size(1) > 1 && t.stride(1) != 1)) return 0;
+  return t.size(0) <= 1 ? std::max(t.size(1), t.stride(0)) : t.stride(0) >= t.size(1) ? t.stride(0) : 0;
+}
+
+int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
+
+// (rows, K) codes, rows on 16 bytes.
+at::Tensor new_codes(const at::Tensor& like, int64_t M, int64_t K) {
+  return at::empty_strided({M, K}, {up16(K), 1}, like.options().dtype(at::kChar));
+}
+
+// Codes (rows, K) as vnx_q8_linear reads them; their pitch, 0 where they are not.
+int64_t codes_of(const at::Tensor* t) {
+  if (!t || t->scalar_type() != at::kChar || !aligned(t->data_ptr(), 16)) return 0;
+  int64_t ld = pitch_of(*t);
+  if (t->dim() == 2 && t->size(0) <= 1) ld = up16(ld);
+  return ld % 16 ? 0 : ld;
+}
+
+// A contiguous fp32 vector of n values (a (n, 1) tensor is one too).
+const at::Tensor* f32_vec(PyObject* o, int dev, int64_t n) {
+  const at::Tensor* t = tensor(o, dev);
+  return t && t->scalar_type() == at::kFloat && t->numel() == n && t->is_contiguous() &&
+                 (t->dim() == 1 || (t->dim() == 2 && t->size(1) == 1))
+             ? t
+             : nullptr;
+}
+
+PyObject* pack2(at::Tensor a, at::Tensor b, PyObject* c = nullptr) {
+  PyObject* r = PyTuple_New(c ? 3 : 2);
+  if (!r) return nullptr;
+  PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(std::move(a)));
+  PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(std::move(b)));
+  if (c) PyTuple_SET_ITEM(r, 2, c);
+  return r;
+}
+
+// q8_quantize(device, stream, x)
+PyObject* q8_quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  int64_t dev;
+  void* st;
+  if (n != 3 || !stream_of(a[0], a[1], &dev, &st)) Py_RETURN_NONE;
+  const at::Tensor* x = tensor(a[2], (int)dev);
+  if (!x) Py_RETURN_NONE;
+  const int dt = code_of(x->scalar_type());
+  const int64_t ld = pitch_of(*x);
+  if (dt < 0 || !ld) Py_RETURN_NONE;
+  const int64_t M = x->size(0), K = x->size(1);
+  const c10::DeviceGuard guard(x->device());  // (the null stream is the current device's)
+  at::Tensor codes = new_codes(*x, M, K), scale = at::empty({M}, x->options().dtype(at::kFloat));
+  const int rc = g_quantize(x->data_ptr(), dt, ld, M, K, static_cast<int8_t*>(codes.data_ptr()), up16(K),
+                            static_cast<float*>(scale.data_ptr()), st);
+  return rc == VNX_OK ? pack2(std::move(codes), std::move(scale)) : status(rc);
+  END_HANDLE_TH_ERRORS
+}
+
+// q8_rmsnorm(device, stream, x, weight, eps, residual, sum_out)
+PyObject* q8_rmsnorm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  int64_t dev, ldr = 0, lds = 0;
+  void* st;
+  double eps;
+  if (n != 7 || !stream_of(a[0], a[1], &dev, &st) || !float_of(a[4], &eps)) Py_RETURN_NONE;
+  const at::Tensor *x = tensor(a[2], (int)dev), *res = nullptr, *sum = nullptr;
+  if (!x) Py_RETURN_NONE;
+  const int dt = code_of(x->scalar_type());
+  const int64_t ld = pitch_of(*x);
+  if (dt < 0 || !ld) Py_RETURN_NONE;
+  const int64_t M = x->size(0), K = x->size(1);
+  const at::Tensor* w = f32_vec(a[3], (int)dev, K);
+  if (!w || w->dim() != 1) Py_RETURN_NONE;
+  if (a[5] != Py_None) {
+    res = tensor(a[5], (int)dev);
+    if (!res || res->sizes() != x->sizes() || code_of(res->scalar_type()) < 0 || !(ldr = pitch_of(*res)))
+      Py_RETURN_NONE;
+  }
+  if (a[6] != Py_None) {
+    sum = tensor(a[6], (int)dev);
+    if (!sum || sum->sizes() != x->sizes() || sum->scalar_type() != x->scalar_type() || !(lds = pitch_of(*sum)))
+      Py_RETURN_NONE;
+  }
+  const c10::DeviceGuard guard(x->device());
+  at::Tensor fresh;
+  if (res && !sum) {
+    fresh = at::empty({M, K}, x->options());
+    sum = &fresh, lds = K;
+  }
+  at::Tensor codes = new_codes(*x, M, K), scale = at::empty({M}, x->options().dtype(at::kFloat));
+  const int rc =
+      g_rmsnorm(x->data_ptr(), dt, ld, res ? res->data_ptr() : nullptr, res ? code_of(res->scalar_type()) : VNX_F32,
+                ldr, static_cast<const float*>(w->data_ptr()), (float)eps, M, K, sum ? sum->data_ptr() : nullptr, lds,
+                static_cast<int8_t*>(codes.data_ptr()), up16(K), static_cast<float*>(scale.data_ptr()), st);
+  if (rc != VNX_OK) return status(rc);
+  PyObject* s = a[6] != Py_None ? a[6] : a[2];
+  if (fresh.defined()) s = THPVariable_Wrap(std::move(fresh));
+  else Py_INCREF(s);
+  return pack2(std::move(codes), std::move(scale), s);
+  END_HANDLE_TH_ERRORS
+}
+
+// q8_dequantize(device, stream, codes, scale, out_dtype)
+PyObject* q8_dequantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  int64_t dev;
+  void* st;
+  if (n != 5 || !stream_of(a[0], a[1], &dev, &st) || !THPDtype_Check(a[4])) Py_RETURN_NONE;
+  const at::Tensor* c = tensor(a[2], (int)dev);
+  const auto t = reinterpret_cast<THPDtype*>(a[4])->scalar_type;
+  if (!c || c->scalar_type() != at::kChar || code_of(t) < 0) Py_RETURN_NONE;
+  const int64_t ld = pitch_of(*c);
+  if (!ld) Py_RETURN_NONE;
+  const at::Tensor* s = f32_vec(a[3], (int)dev, c->size(0));
+  if (!s) Py_RETURN_NONE;
+  const c10::DeviceGuard guard(c->device());
+  at::Tensor out = at::empty({c->size(0), c->size(1)}, c->options().dtype(t));
+  const int rc = g_dequantize(static_cast<const int8_t*>(c->data_ptr()), ld, static_cast<const float*>(s->data_ptr()),
+                              c->size(0), c->size(1), out.data_ptr(), code_of(t), c->size(1), st);
+  return rc == VNX_OK ? THPVariable_Wrap(std::move(out)) : status(rc);
+  END_HANDLE_TH_ERRORS
+}
+
+// q8_linear(device, stream, codes, scale, wq, w_scale, bias, residual, swiglu, out_dtype, out)
+PyObject* q8_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  int64_t dev;
+  void* st;
+  vnx_q8_linear_args p{};
+  if (n != 11 || !stream_of(a[0], a[1], &dev, &st) || !PyBool_Check(a[8])) Py_RETURN_NONE;
+  const at::Tensor *x = tensor(a[2], (int)dev), *w = tensor(a[4], (int)dev);
+  p.ldx = codes_of(x), p.ldw = codes_of(w);
+  if (!p.ldx || !p.ldw || x->size(1) != w->size(1)) Py_RETURN_NONE;
+  p.M = x->size(0), p.N = w->size(0), p.K = x->size(1);
+  const bool sw = a[8] == Py_True;
+  const int64_t cols = sw ? p.N / 2 : p.N;
+  const at::Tensor *xs = f32_vec(a[3], (int)dev, p.M), *ws = f32_vec(a[5], (int)dev, p.N);
+  if (!xs || !ws) Py_RETURN_NONE;
+  if (a[6] != Py_None) {
+    const at::Tensor* b = f32_vec(a[6], (int)dev, p.N);
+    if (!b || b->dim() != 1) Py_RETURN_NONE;
+    p.bias = static_cast<const float*>(b->data_ptr());
+  }
+  if (a[7] != Py_None) {
+    const at::Tensor* r = tensor(a[7], (int)dev);
+    if (!r || (p.res_dtype = code_of(r->scalar_type())) < 0 || !(p.ldr = pitch_of(*r)) || r->size(0) != p.M ||
+        r->size(1) != cols)
+      Py_RETURN_NONE;
+    p.res = r->data_ptr();
+  }
+  const c10::DeviceGuard guard(x->device());
+  at::Tensor fresh;
+  const at::Tensor* out;
+  if (a[10] == Py_None) {
+    if (!THPDtype_Check(a[9])) Py_RETURN_NONE;
+    const auto t = reinterpret_cast<THPDtype*>(a[9])->scalar_type;
+    if (code_of(t) < 0) Py_RETURN_NONE;
+    fresh = at::empty({p.M, cols}, x->options().dtype(t));
+    out = &fresh;
+    p.ldy = cols;
+  } else {
+    out = tensor(a[10], (int)dev);
+    if (!out || code_of(out->scalar_type()) < 0 || !(p.ldy = pitch_of(*out)) || out->size(0) != p.M ||
+        out->size(1) != cols)
+      Py_RETURN_NONE;
+  }
+  p.x = static_cast<const int8_t*>(x->data_ptr()), p.w = static_cast<const int8_t*>(w->data_ptr());
+  p.x_scale = static_cast<const float*>(xs->data_ptr()), p.w_scale = static_cast<const float*>(ws->data_ptr());
+  p.y = out->data_ptr(), p.y_dtype = code_of(out->scalar_type());
+  p.epilogue = sw ? VNX_EPI_SWIGLU : VNX_EPI_NONE;
+  const int rc = g_linear(&p, st);
+  if (rc != VNX_OK) return status(rc);
+  if (a[10] != Py_None) {
+    Py_INCREF(a[10]);
+    return a[10];
+  }
+  return THPVariable_Wrap(std::move(fresh));
+  END_HANDLE_TH_ERRORS
+}
+
+// Reads n addresses into f; an exception is set where it fails.
+bool addresses(PyObject* const* a, Py_ssize_t got, int want, void** f) {
+  if (got != want) {
+    PyErr_Format(PyExc_TypeError, "init takes %d addresses", want);
+    return false;
+  }
+  for (int i = 0; i < want; ++i) {
+    f[i] = PyLong_AsVoidPtr(a[i]);
+    if (!f[i]) {
+      if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "a null address");
+      return false;
+    }
+  }
+  return true;
+}
+
 // init(address of vnx_kv_write, vnx_kv_read, vnx_tree_attn_q8_workspace, vnx_tree_attn_q8)
 PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t n) {
   void* f[4];
-  if (n != 4) return PyErr_Format(PyExc_TypeError, "init takes four addresses");
-  for (int i = 0; i < 4; ++i) {
-    f[i] = PyLong_AsVoidPtr(a[i]);
-    if (!f[i]) return PyErr_Occurred() ? nullptr : PyErr_Format(PyExc_ValueError, "a null address");
-  }
+  if (!addresses(a, n, 4, f)) return nullptr;
   g_write = reinterpret_cast<decltype(g_write)>(f[0]);
   g_read = reinterpret_cast<decltype(g_read)>(f[1]);
   g_attn_ws = reinterpret_cast<decltype(g_attn_ws)>(f[2]);
   g_attn = reinterpret_cast<decltype(g_attn)>(f[3]);
+  Py_RETURN_NONE;
+}
+
+// init_q8(address of vnx_q8_quantize, vnx_q8_rmsnorm, vnx_q8_dequantize, vnx_q8_linear)
+PyObject* init_q8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  void* f[4];
+  if (!addresses(a, n, 4, f)) return nullptr;
+  g_quantize = reinterpret_cast<decltype(g_quantize)>(f[0]);
+  g_rmsnorm = reinterpret_cast<decltype(g_rmsnorm)>(f[1]);
+  g_dequantize = reinterpret_cast<decltype(g_dequantize)>(f[2]);
+  g_linear = reinterpret_cast<decltype(g_linear)>(f[3]);
   Py_RETURN_NONE;
 }
 
@@ -328,16 +542,21 @@ PyCFunction fast() {
 }
 
 PyMethodDef kMethods[] = {{"init", fast<init>(), METH_FASTCALL, nullptr},
+                          {"init_q8", fast<init_q8>(), METH_FASTCALL, nullptr},
                           {"kv_write", fast<kv_write>(), METH_FASTCALL, nullptr},
                           {"kv_read", fast<kv_read>(), METH_FASTCALL, nullptr},
                           {"tree_attn_q8", fast<tree_attn_q8>(), METH_FASTCALL, nullptr},
+                          {"q8_quantize", fast<q8_quantize>(), METH_FASTCALL, nullptr},
+                          {"q8_rmsnorm", fast<q8_rmsnorm>(), METH_FASTCALL, nullptr},
+                          {"q8_dequantize", fast<q8_dequantize>(), METH_FASTCALL, nullptr},
+                          {"q8_linear", fast<q8_linear>(), METH_FASTCALL, nullptr},
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_vnx_bind", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
 
-// .torch: the PyTorch it was compiled against; .sizes: of the argument blocks
-// that it fills.  Another PyTorch, or another library, must not get them.
+// .torch: the PyTorch it was compiled against; .sizes, .q8_size: of the argument
+// blocks that it fills.  Another PyTorch, or another library, must not get them.
 PyMODINIT_FUNC PyInit__vnx_bind() {
   PyObject* m = PyModule_Create(&kModule);
   if (!m) return nullptr;
@@ -349,7 +568,8 @@ PyMODINIT_FUNC PyInit__vnx_bind() {
     Py_DECREF(m);
     return nullptr;
   }
-  if (PyModule_AddStringConstant(m, "torch", VNX_BIND_TORCH) < 0) {
+  if (PyModule_AddIntConstant(m, "q8_size", (long)sizeof(vnx_q8_linear_args)) < 0 ||
+      PyModule_AddStringConstant(m, "torch", VNX_BIND_TORCH) < 0) {
     Py_DECREF(m);
     return nullptr;
   }

@@ -889,6 +889,188 @@ class HipBackend(DeviceBackend):
                    "tree_attention_q8")
         return out
 
+    # ---- products in 8-bit integers ------------------------------------------
+    def _rows_of(self, x, what: str, dtypes=None):
+        """(lead shape, (rows, K) view with unit last stride) of a tensor of
+        the given types (copied where its rows do not follow each other)."""
+        t = _to_tensor(x, self._torch_device)
+        if t.is_neg():
+            t = t.resolve_neg()
+        if t.dtype not in (dtypes or _lib.DTYPE_CODES):
+            raise ValueError(f"{what} must be {', '.join(str(d) for d in dtypes or _lib.DTYPE_CODES)}, got {t.dtype}")
+        if t.dim() < 1 or t.shape[-1] < 1:
+            raise ValueError(f"{what} must be (..., K) with K >= 1, got {tuple(t.shape)}")
+        lead, K = tuple(t.shape[:-1]), t.shape[-1]
+        t2 = t if t.dim() == 2 else t.reshape(-1, K)
+        if (K > 1 and t2.stride(1) != 1) or (t2.shape[0] > 1 and t2.stride(0) < K):
+            t2 = t2.contiguous()
+        return lead, t2
+
+    @staticmethod
+    def _pitch(t2: torch.Tensor) -> int:
+        return max(t2.shape[1], t2.stride(0))
+
+    def _code_rows(self, x, what: str):
+        """int8 rows as vnx_q8_linear reads them: on 16 bytes (padded where
+        they are not), and their pitch."""
+        lead, t = self._rows_of(x, what, (torch.int8,))
+        if t.data_ptr() % 16 or (t.shape[0] > 1 and t.stride(0) % 16):
+            ld = (t.shape[1] + 15) // 16 * 16
+            p = torch.empty((t.shape[0], ld), dtype=torch.int8, device=t.device)[:, :t.shape[1]]
+            p.copy_(t)
+            t = p
+        return lead, t, (self._pitch(t) + 15) // 16 * 16
+
+    def _scales(self, s, n: int, what: str) -> torch.Tensor:
+        t = _to_tensor(s, self._torch_device, torch.float32)
+        if t.numel() != n:
+            raise ValueError(f"{what} must have {n} entries, got {tuple(t.shape)}")
+        return t.reshape(-1).contiguous().resolve_neg()
+
+    def _new_codes(self, M: int, K: int):
+        """((M, K) int8 with rows on 16 bytes, its pitch, (M,) fp32)."""
+        ld = (K + 15) // 16 * 16
+        return (torch.empty_strided((M, K), (ld, 1), dtype=torch.int8, device=self._torch_device), ld,
+                torch.empty(M, dtype=torch.float32, device=self._torch_device))
+
+    def _out_rows(self, out, shape, dtypes, what: str) -> torch.Tensor:
+        """`out` as (rows, K) rows written in place: checked, never copied."""
+        if not isinstance(out, torch.Tensor) or out.device != self._torch_device or tuple(out.shape) != shape \
+                or out.dtype not in dtypes:
+            raise ValueError(f"{what} must be a {shape} tensor of {', '.join(str(d) for d in dtypes)} on "
+                             f"{self._torch_device}")
+        K = shape[-1]
+        o = out if out.dim() == 2 else out.view(-1, K)
+        if (K > 1 and o.stride(1) != 1) or (o.shape[0] > 1 and o.stride(0) < K) or o.is_neg():
+            raise ValueError(f"{what} needs unit last stride and rows that do not overlap")
+        return o
+
+    def quantize_rows(self, x):
+        """Rows (..., K) fp32, bf16 or fp16 as 8-bit integers
+        (vnx_q8_quantize): (codes (..., K) int8, scale (...) fp32), scale =
+        max|x| / 127 and code = rint(x * (127 / max|x|)) of each row.  The
+        codes' rows start on 16 bytes, as linear_q8 reads them.  A row with an
+        infinity or a NaN has codes 0 and scale NaN."""
+        r = self._bind.q8_quantize(self._index, self._stream(), x)
+        if r is not None:      # (None: a call that needs the general path's conversions or errors)
+            return self._bound(r, "quantize_rows")
+        with torch.cuda.device(self._index):
+            lead, t = self._rows_of(x, "x")
+            M, K = t.shape
+            codes, ld, scale = self._new_codes(M, K)
+            _lib.check(self._L.vnx_q8_quantize(t.data_ptr(), _lib.DTYPE_CODES[t.dtype], self._pitch(t), M, K,
+                                               codes.data_ptr(), ld, scale.data_ptr(), self._stream()),
+                       "quantize_rows")
+            return codes.view(*lead, K), scale.view(lead)
+
+    def dequantize_rows(self, codes, scale, out_dtype=torch.float32) -> torch.Tensor:
+        """The values (..., K) in out_dtype that codes (..., K) int8 with a
+        scale a row stand for (vnx_q8_dequantize)."""
+        r = self._bind.q8_dequantize(self._index, self._stream(), codes, scale, out_dtype)
+        if r is not None:
+            return self._bound(r, "dequantize_rows")
+        with torch.cuda.device(self._index):
+            if out_dtype not in _lib.DTYPE_CODES:
+                raise ValueError("out_dtype must be torch.float32, torch.bfloat16 or torch.float16")
+            lead, c = self._rows_of(codes, "codes", (torch.int8,))
+            M, K = c.shape
+            sc = self._scales(scale, M, "scale")
+            out = torch.empty((M, K), dtype=out_dtype, device=self._torch_device)
+            _lib.check(self._L.vnx_q8_dequantize(c.data_ptr(), self._pitch(c), sc.data_ptr(), M, K, out.data_ptr(),
+                                                 _lib.DTYPE_CODES[out_dtype], K, self._stream()), "dequantize_rows")
+            return out.view(*lead, K)
+
+    def rmsnorm_q8(self, x, weight, eps: float = 1e-6, residual=None, sum_out=None):
+        """RMS norm of a residual stream, as 8-bit rows (vnx_q8_rmsnorm).
+
+        x (..., D) fp32, bf16 or fp16; residual (same shape, any of these
+        types) is added first: s = x + residual in x's type (s = x without
+        one).  Returns (codes (..., D) int8, scale (...) fp32, s): codes and
+        scales of s / sqrt(mean(s^2) + eps) * weight, and s, written into
+        sum_out when given (x's shape and type; x or residual itself for a sum
+        in place), else a new tensor (x itself without a residual)."""
+        r = self._bind.q8_rmsnorm(self._index, self._stream(), x, weight, eps, residual, sum_out)
+        if r is not None:
+            return self._bound(r, "rmsnorm_q8")
+        with torch.cuda.device(self._index):
+            lead, t = self._rows_of(x, "x")
+            M, D = t.shape
+            w = self._scales(weight, D, "weight")
+            rt = None
+            if residual is not None:
+                rlead, rt = self._rows_of(residual, "residual")
+                if rlead != lead or rt.shape[1] != D:
+                    raise ValueError(f"residual must be {(*lead, D)}, got {(*rlead, rt.shape[1])}")
+            s = st = None
+            if sum_out is not None:
+                s = sum_out
+                st = self._out_rows(s, (*lead, D), (t.dtype,), "sum_out")
+            elif rt is not None:
+                st = torch.empty((M, D), dtype=t.dtype, device=self._torch_device)
+                s = st.view(*lead, D)
+            codes, ld, scale = self._new_codes(M, D)
+            _lib.check(self._L.vnx_q8_rmsnorm(
+                t.data_ptr(), _lib.DTYPE_CODES[t.dtype], self._pitch(t), _ptr(rt),
+                _lib.DTYPE_CODES[rt.dtype] if rt is not None else _lib.VNX_F32, self._pitch(rt) if rt is not None else 0,
+                w.data_ptr(), float(eps), M, D, _ptr(st), self._pitch(st) if st is not None else 0, codes.data_ptr(),
+                ld, scale.data_ptr(), self._stream()), "rmsnorm_q8")
+            return codes.view(*lead, D), scale.view(lead), s if s is not None else t.view(*lead, D)
+
+    def linear_q8(self, codes, scale, wq, w_scale, bias=None, residual=None, swiglu: bool = False,
+                  out_dtype=torch.bfloat16, out=None, force_shape: int = 0) -> torch.Tensor:
+        """The product of 8-bit rows with an INT8 weight (vnx_q8_linear).
+
+        codes (..., K) int8 with scale (...) fp32 (quantize_rows, rmsnorm_q8);
+        wq (N, K) int8 with w_scale (N,) or (N, 1) fp32 (quant.quantize_int8).
+        Returns (..., N) in out_dtype (fp32, bf16 or fp16): the exact integer
+        sums times both scales, + bias (N,) and + residual (..., N) when given
+        (added in fp32, rounded once).  swiglu: wq holds N / 2 gate rows, then
+        N / 2 up rows, and the result is silu(gate) * up (..., N / 2), without
+        a residual.  out: written into (residual itself for a sum in place).
+        Codes or weights whose rows are not on 16 bytes are copied every call.
+        force_shape pins the launch shape (tuning and tests)."""
+        if not force_shape:
+            r = self._bind.q8_linear(self._index, self._stream(), codes, scale, wq, w_scale, bias, residual, swiglu,
+                                     out_dtype, out)
+            if r is not None:
+                return self._bound(r, "linear_q8")
+        with torch.cuda.device(self._index):
+            return self._linear_q8(codes, scale, wq, w_scale, bias, residual, swiglu, out_dtype, out, force_shape)
+
+    def _linear_q8(self, codes, scale, wq, w_scale, bias, residual, swiglu, out_dtype, out, force_shape):
+        lead, c, ldx = self._code_rows(codes, "codes")
+        wlead, w, ldw = self._code_rows(wq, "wq")
+        M, K = c.shape
+        if len(wlead) != 1 or w.shape[1] != K:
+            raise ValueError(f"wq must be (N, {K}), got {(*wlead, w.shape[1])}")
+        N = w.shape[0]
+        if swiglu and N % 2:
+            raise ValueError(f"a SwiGLU weight has as many up rows as gate rows, got {N} rows")
+        cols = N // 2 if swiglu else N
+        xs, ws = self._scales(scale, M, "scale"), self._scales(w_scale, N, "w_scale")
+        b = None if bias is None else self._scales(bias, N, "bias")
+        rt = None
+        if residual is not None:
+            if swiglu:
+                raise ValueError("SwiGLU takes no residual")
+            rlead, rt = self._rows_of(residual, "residual")
+            if rlead != lead or rt.shape[1] != cols:
+                raise ValueError(f"residual must be {(*lead, cols)}, got {(*rlead, rt.shape[1])}")
+        if out is None:
+            if out_dtype not in _lib.DTYPE_CODES:
+                raise ValueError("out_dtype must be torch.float32, torch.bfloat16 or torch.float16")
+            y = torch.empty((M, cols), dtype=out_dtype, device=self._torch_device)
+            out = y.view(*lead, cols)
+        else:
+            y = self._out_rows(out, (*lead, cols), tuple(_lib.DTYPE_CODES), "out")
+        args = _lib.pack_q8_linear(
+            c.data_ptr(), xs.data_ptr(), w.data_ptr(), ws.data_ptr(), _ptr(b) or 0, _ptr(rt) or 0, y.data_ptr(),
+            ldx, ldw, self._pitch(rt) if rt is not None else 0, self._pitch(y), M, N, K,
+            _lib.DTYPE_CODES[rt.dtype] if rt is not None else _lib.VNX_F32, _lib.DTYPE_CODES[y.dtype],
+            _lib.VNX_EPI_SWIGLU if swiglu else _lib.VNX_EPI_NONE, int(force_shape))
+        _lib.check(self._L.vnx_q8_linear(args, self._stream()), "linear_q8")
+        return out
+
     def attention(self, q, k, v, mask=None):
         """DeviceBackend.attention (device.py:260-270; TorchBackend's SDPA call,
         backend_torch.py:356-379).  bf16 (B, H, Nq, d) queries over (B, Hkv, T, d)
