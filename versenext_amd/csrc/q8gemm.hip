@@ -265,14 +265,273 @@ int q8_direct(Q8LinParams p, hipStream_t st) {
   return VNX_OK;
 }
 
-constexpr int kQ8Shapes = 2;
+// ---------------------------------------------------------------------------
+// k_q8_tile: many rows.  BM x BN tiles of y, WM x WN waves, slabs of 64 bytes of
+// k in a ring of NS buffers in LDS.
+//
+// The slabs come by direct copies from memory to LDS (1 KB an instruction: 16
+// rows of 64 bytes, lane l's 16 bytes at 16 l), so the tile's layout is made by
+// which piece of its row a lane asks for: piece c of row R lies at c ^ (R / 2 %
+// 4), and the eight lanes that LDS serves at once read eight different 16-byte
+// columns of its 128.  A wave holds two sets of operands: it reads slab c + 1
+// while the products of slab c run, and slab c + NS comes into the buffer that
+// slab c has left, so one barrier a slab does.
+// ---------------------------------------------------------------------------
+constexpr int kQ8Slab = 64;
+
+__device__ __forceinline__ uint32_t lds_addr(const void* p) {
+  return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
+}
+
+// Lane l's 16 bytes at base + off to LDS at `to` + 16 l (counted by vmcnt).
+__device__ __forceinline__ void copy_to_lds(uint32_t to, uint32_t off, const int8_t* base) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+               :
+               : "s"(to), "v"(off), "s"(base)
+               : "memory", "m0");
+}
+
+// Waits until at most N of this wave's copies are under way.
+template <int N>
+__device__ __forceinline__ void wait_copies() {
+  asm volatile("s_waitcnt vmcnt(%0)" : : "i"(N) : "memory");
+}
+
+// Every wave's LDS reads so far are done, and every wave is here.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0), in a form that the compiler counts with
+  asm volatile("s_barrier" : : : "memory");
+}
+
+template <int BM, int BN, int WM, int WN, int NS, int OCC, bool SW>
+__global__ __launch_bounds__(64 * WM * WN, OCC) void k_q8_tile(Q8LinParams p) {
+  using F = Mfma<32>;
+  constexpr int NW = WM * WN, RT = BM / WM / 32, CT = BN / WN / 32;
+  constexpr int STAGE = (BM + BN) * kQ8Slab, PW = (BM + BN) / 16 / NW;
+  static_assert((BM + BN) / 16 % NW == 0 && (NS - 1) * PW < 64 && (!SW || CT % 2 == 0), "");
+  constexpr int WCOLS = CT * 32, WOUT = SW ? WCOLS / 2 : WCOLS, OC = SW ? BN / 2 : BN;
+  constexpr int TP = WOUT + 4;                       // row pitch (floats) of a wave's output strip
+  constexpr int EPI = NW * 32 * TP * 4 + BM * 4;
+  constexpr int SM = NS * STAGE > EPI ? NS * STAGE : EPI;
+  __shared__ __attribute__((aligned(128))) char smem[SM];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+  // Each XCD takes a run of tiles, in blocks of eight rows of tiles: the tiles
+  // that run at once on it share rows of x and of W in its L2.
+  int mi, ni;
+  {
+    const int total = p.mt * p.nt, run = (total + kQ8Xcds - 1) / kQ8Xcds;
+    const int at = blockIdx.x / kQ8Xcds, i = blockIdx.x % kQ8Xcds * run + at;
+    if (at >= run || i >= total) return;             // uniform over the workgroup
+    const int blk = i / (8 * p.nt), in = i - blk * 8 * p.nt, h = min(8, p.mt - blk * 8);
+    mi = blk * 8 + in % h;
+    ni = in / h;
+  }
+  const int m0 = mi * BM, o0 = ni * OC;              // first row and column of y
+  const int nsl = (p.K + kQ8Slab - 1) / kQ8Slab;
+  const uint32_t lds0 = lds_addr(smem);
+
+  // this wave's copies of a slab: rows 16 (wave PW + q) + lane / 4 of [x tile; W tile]
+  const int piece = (lane & 3) ^ (lane >> 3 & 3);    // of the row's four in a slab
+  uint32_t off[PW];
+  const int8_t* base[PW];                            // uniform
+#pragma unroll
+  for (int q = 0; q < PW; ++q) {
+    const int r0 = (wave * PW + q) * 16;
+    if (r0 < BM) {
+      base[q] = p.x + (int64_t)m0 * p.ldx;
+      off[q] = (uint32_t)min(r0 + (lane >> 2), p.M - 1 - m0) * (uint32_t)p.ldx + piece * 16;
+    } else {
+      const int w0 = r0 - BM, up = SW ? w0 / 32 & 1 : 0, row = SW ? w0 / 64 * 32 + w0 % 32 : w0;
+      base[q] = p.w + (int64_t)(up ? p.cols + o0 : o0) * p.ldw;
+      off[q] = (uint32_t)min(row + (lane >> 2), p.cols - 1 - o0) * (uint32_t)p.ldw + piece * 16;
+    }
+  }
+  auto fetch = [&](int c) {
+    const uint32_t to = lds0 + c % NS * STAGE + wave * PW * 1024;
+    const int64_t k = (int64_t)c * kQ8Slab;
+    // a piece past the row's end: the slab's first instead
+    const uint32_t back = c * kQ8Slab + piece * 16 < p.K ? 0u : piece * 16u;
+#pragma unroll
+    for (int q = 0; q < PW; ++q) copy_to_lds(to + q * 1024, off[q] - back, base[q] + k);
+  };
+  // bytes of x at or past K count as 0, in the pieces that this lane copied
+  auto clear = [&](int c) {
+    const int left = p.K - c * kQ8Slab - piece * 16;
+    if (left < 16) {
+#pragma unroll
+      for (int q = 0; q < PW; ++q) {
+        if ((wave * PW + q) * 16 >= BM) continue;
+        u32x4* d = reinterpret_cast<u32x4*>(smem + c % NS * STAGE + (wave * PW + q) * 1024 + lane * 16);
+        u32x4 v = *d;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int n = left - 4 * e;
+          v[e] = n >= 4 ? v[e] : n <= 0 ? 0u : v[e] & ((1u << (8 * n)) - 1u);
+        }
+        *d = v;
+      }
+    }
+  };
+
+  typename F::Acc acc[RT][CT];
+#pragma unroll
+  for (int i = 0; i < RT; ++i)
+#pragma unroll
+    for (int t = 0; t < CT; ++t)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][t][e] = 0;
+  const int r = lane & 31, h = lane >> 5;
+  int xo[2], wo[2];
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const int col = ((2 * s + h) ^ (r >> 1 & 3)) * 16;
+    xo[s] = (wm * RT * 32 + r) * kQ8Slab + col;
+    wo[s] = (BM + wn * CT * 32 + r) * kQ8Slab + col;
+  }
+  struct Set { u32x4 x[2][RT], w[2][CT]; };
+  auto read = [&](int c, Set& q) {
+    const char* b = smem + c % NS * STAGE;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+#pragma unroll
+      for (int i = 0; i < RT; ++i) q.x[s][i] = *reinterpret_cast<const u32x4*>(b + xo[s] + i * 32 * kQ8Slab);
+#pragma unroll
+      for (int t = 0; t < CT; ++t) q.w[s][t] = *reinterpret_cast<const u32x4*>(b + wo[s] + t * 32 * kQ8Slab);
+    }
+  };
+  // STEADY: slab c + NS is one more to fetch
+  auto step = [&](auto steady, int c, const Set& cur, Set& nxt) {
+    if constexpr (decltype(steady)::value) {
+      wait_copies<(NS - 2) * PW>();
+      lds_barrier();
+      fetch(c + NS);
+      read(c + 1, nxt);
+    } else if (c + 1 < nsl) {                        // uniform
+      wait_copies<0>();
+      if (c + 2 == nsl && p.K % kQ8Slab) clear(c + 1);
+      lds_barrier();
+      read(c + 1, nxt);
+    }
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int t = 0; t < CT; ++t)
+#pragma unroll
+        for (int i = 0; i < RT; ++i) acc[i][t] = F::mma(cur.x[s][i], cur.w[s][t], acc[i][t]);
+  };
+  for (int c = 0; c < NS && c < nsl; ++c) fetch(c);
+  if (nsl >= NS) wait_copies<(NS - 1) * PW>();
+  else wait_copies<0>();
+  if (nsl == 1 && p.K % kQ8Slab) clear(0);
+  lds_barrier();
+  Set a, b;
+  read(0, a);
+  int c = 0;
+  for (; c + 1 + NS < nsl; c += 2) {
+    step(BoolC<true>{}, c, a, b);
+    step(BoolC<true>{}, c + 1, b, a);
+  }
+  if (c + NS < nsl) {                                // an odd one: the sets change places
+    step(BoolC<true>{}, c, a, b);
+    a = b;
+    ++c;
+  }
+  for (; c < nsl; c += 2) {
+    step(BoolC<false>{}, c, a, b);
+    if (c + 1 < nsl) step(BoolC<false>{}, c + 1, b, a);
+  }
+
+  // A strip of 32 rows at a time leaves through this wave's part of LDS: lane (r,
+  // h) writes its column of each tile, then holds 8 columns of a row.
+  lds_barrier();
+  float* xs = reinterpret_cast<float*>(smem + NW * 32 * TP * 4);
+  for (int i = tid; i < BM; i += 64 * NW) xs[i] = p.xs[min(m0 + i, p.M - 1)];
+  float ws[CT], bias[CT];
+#pragma unroll
+  for (int t = 0; t < CT; ++t) {
+    const int n = SW ? (t & 1) * p.cols + min(o0 + wn * WOUT + t / 2 * 32 + r, p.cols - 1)
+                     : min(o0 + wn * WOUT + t * 32 + r, p.cols - 1);
+    ws[t] = p.ws[n];
+    bias[t] = p.bias ? p.bias[n] : 0.0f;
+  }
+  __syncthreads();
+  float* tr = reinterpret_cast<float*>(smem) + wave * 32 * TP;
+#pragma unroll
+  for (int i = 0; i < RT; ++i) {
+    const int row0 = wm * RT * 32 + i * 32;          // of the tile
+    if (m0 + row0 >= p.M) break;                     // uniform
+#pragma unroll
+    for (int ii = 0; ii < 4; ++ii) {
+      const f32x4 sx = *reinterpret_cast<const f32x4*>(xs + row0 + 8 * ii + 4 * h);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float* d = tr + (8 * ii + 4 * h + e) * TP + r;
+        auto val = [&](int t) {
+          const float v = (float)acc[i][t][4 * ii + e] * sx[e] * ws[t];
+          return p.bias ? v + bias[t] : v;
+        };
+        if constexpr (SW) {
+#pragma unroll
+          for (int t = 0; t < CT; t += 2) d[t / 2 * 32] = q8_swiglu(val(t), val(t + 1));
+        } else {
+#pragma unroll
+          for (int t = 0; t < CT; ++t) d[t * 32] = val(t);
+        }
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    constexpr int LR = WOUT / 8, RP = 64 / LR;       // lanes a row, rows a pass
+#pragma unroll 1
+    for (int q = 0; q < 32 / RP; ++q) {
+      const int row = q * RP + lane / LR, col = lane % LR * 8;
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const f32x4 f = *reinterpret_cast<const f32x4*>(tr + row * TP + col + 4 * e);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[4 * e + j] = f[j];
+      }
+      const int m = m0 + row0 + row, n = o0 + wn * WOUT + col;
+      if (m < p.M && n < p.cols) q8_out8(p, m, n, v);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  }
+}
+
+template <int BM, int BN, int WM, int WN, int NS, int OCC, bool SW>
+int q8_tile(Q8LinParams p, hipStream_t st) {
+  constexpr int OC = SW ? BN / 2 : BN;
+  p.mt = (p.M + BM - 1) / BM;
+  p.nt = (p.cols + OC - 1) / OC;
+  const int64_t total = (int64_t)p.mt * p.nt;
+  if (total >= INT_MAX - 64 || (int64_t)8 * p.nt >= INT_MAX || !launch_fits(total + 8, 64 * WM * WN))
+    return VNX_ERR_UNSUPPORTED;
+  const unsigned wgs = (unsigned)((total + kQ8Xcds - 1) / kQ8Xcds * kQ8Xcds);
+  hipLaunchKernelGGL((k_q8_tile<BM, BN, WM, WN, NS, OCC, SW>), dim3(wgs), dim3(64 * WM * WN), 0, st, p);
+  VNX_LAUNCH_CHECK();
+  return VNX_OK;
+}
+
+constexpr int kQ8Shapes = 4;
 
 template <bool SW>
 int q8_linear(const Q8LinParams& p, int force, hipStream_t st) {
-  const int shape = force ? force - 1 : p.M <= 16 ? 0 : 1;
+  auto tiles = [&](int bm, int bn) {
+    const int oc = SW ? bn / 2 : bn;
+    return (int64_t)((p.M + bm - 1) / bm) * ((p.cols + oc - 1) / oc);
+  };
+  int shape = p.M <= 16 ? 0 : tiles(256, 256) >= 2 * device_cus() && p.M > 256 ? 3 : p.M > 128 ? 2 : 1;
+  if (force) shape = force - 1;
   switch (shape) {
     case 0: return q8_direct<16, 1, 2, 4, 1, SW>(p, st);
-    default: return q8_direct<32, 2, 2, 2, 1, SW>(p, st);
+    case 1: return q8_direct<32, 2, 2, 2, 1, SW>(p, st);
+    case 2: return q8_tile<128, 128, 2, 2, 4, 2, SW>(p, st);
+    default: return q8_tile<256, 256, 2, 2, 4, 1, SW>(p, st);
   }
 }
 
