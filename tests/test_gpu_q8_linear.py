@@ -7,7 +7,7 @@ import q8_ref as R
 
 pytestmark = pytest.mark.gpu
 
-SHAPES = range(0, 5)     # 0: the plan's choice
+SHAPES = range(0, 9)     # 0: the plan's choice
 
 
 def check(hip, shape, M, N, K, out=torch.bfloat16, bias=False, residual=None, swiglu=False, low=-127, fill=77, seed=0):

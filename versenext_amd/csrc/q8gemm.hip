@@ -271,9 +271,9 @@ int q8_direct(Q8LinParams p, hipStream_t st) {
 //
 // The slabs come by direct copies from memory to LDS (1 KB an instruction: 16
 // rows of 64 bytes, lane l's 16 bytes at 16 l), so the tile's layout is made by
-// which piece of its row a lane asks for: piece c of row R lies at c ^ (R / 2 %
-// 4), and the eight lanes that LDS serves at once read eight different 16-byte
-// columns of its 128.  A wave holds two sets of operands: it reads slab c + 1
+// which piece of its row a lane asks for: piece c of row R lies at c ^ (R / 4 %
+// 4), and the sixteen lanes that LDS serves together, four runs of four rows,
+// read sixteen different 16-byte columns of its 256.  A wave holds two sets of operands: it reads slab c + 1
 // while the products of slab c run, and slab c + NS comes into the buffer that
 // slab c has left, so one barrier a slab does.
 // ---------------------------------------------------------------------------
@@ -303,15 +303,15 @@ __device__ __forceinline__ void lds_barrier() {
   asm volatile("s_barrier" : : : "memory");
 }
 
-template <int BM, int BN, int WM, int WN, int NS, int OCC, bool SW>
+template <int S, int BM, int BN, int WM, int WN, int NS, int OCC, bool SW>
 __global__ __launch_bounds__(64 * WM * WN, OCC) void k_q8_tile(Q8LinParams p) {
-  using F = Mfma<32>;
-  constexpr int NW = WM * WN, RT = BM / WM / 32, CT = BN / WN / 32;
+  using F = Mfma<S>;
+  constexpr int NW = WM * WN, RT = BM / WM / S, CT = BN / WN / S, KT = S / 16;
   constexpr int STAGE = (BM + BN) * kQ8Slab, PW = (BM + BN) / 16 / NW;
   static_assert((BM + BN) / 16 % NW == 0 && (NS - 1) * PW < 64 && (!SW || CT % 2 == 0), "");
-  constexpr int WCOLS = CT * 32, WOUT = SW ? WCOLS / 2 : WCOLS, OC = SW ? BN / 2 : BN;
+  constexpr int ACC = S * S / 64, WCOLS = CT * S, WOUT = SW ? WCOLS / 2 : WCOLS, OC = SW ? BN / 2 : BN;
   constexpr int TP = WOUT + 4;                       // row pitch (floats) of a wave's output strip
-  constexpr int EPI = NW * 32 * TP * 4 + BM * 4;
+  constexpr int EPI = NW * S * TP * 4 + BM * 4;
   constexpr int SM = NS * STAGE > EPI ? NS * STAGE : EPI;
   __shared__ __attribute__((aligned(128))) char smem[SM];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -332,7 +332,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void k_q8_tile(Q8LinParams p) {
   const uint32_t lds0 = lds_addr(smem);
 
   // this wave's copies of a slab: rows 16 (wave PW + q) + lane / 4 of [x tile; W tile]
-  const int piece = (lane & 3) ^ (lane >> 3 & 3);    // of the row's four in a slab
+  const int piece = (lane & 3) ^ (-(lane >> 4) & 3);    // of the row's four in a slab
   uint32_t off[PW];
   const int8_t* base[PW];                            // uniform
 #pragma unroll
@@ -342,18 +342,20 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void k_q8_tile(Q8LinParams p) {
       base[q] = p.x + (int64_t)m0 * p.ldx;
       off[q] = (uint32_t)min(r0 + (lane >> 2), p.M - 1 - m0) * (uint32_t)p.ldx + piece * 16;
     } else {
-      const int w0 = r0 - BM, up = SW ? w0 / 32 & 1 : 0, row = SW ? w0 / 64 * 32 + w0 % 32 : w0;
+      const int w0 = r0 - BM, up = SW ? w0 / S & 1 : 0, row = SW ? w0 / (2 * S) * S + w0 % S : w0;
       base[q] = p.w + (int64_t)(up ? p.cols + o0 : o0) * p.ldw;
       off[q] = (uint32_t)min(row + (lane >> 2), p.cols - 1 - o0) * (uint32_t)p.ldw + piece * 16;
     }
   }
-  auto fetch = [&](int c) {
-    const uint32_t to = lds0 + c % NS * STAGE + wave * PW * 1024;
-    const int64_t k = (int64_t)c * kQ8Slab;
-    // a piece past the row's end: the slab's first instead
+  // copy q of slab c
+  auto copy = [&](int c, int q) {
+    // (a piece past the row's end: the slab's first instead)
     const uint32_t back = c * kQ8Slab + piece * 16 < p.K ? 0u : piece * 16u;
+    copy_to_lds(lds0 + c % NS * STAGE + (wave * PW + q) * 1024, off[q] - back, base[q] + (int64_t)c * kQ8Slab);
+  };
+  auto fetch = [&](int c) {
 #pragma unroll
-    for (int q = 0; q < PW; ++q) copy_to_lds(to + q * 1024, off[q] - back, base[q] + k);
+    for (int q = 0; q < PW; ++q) copy(c, q);
   };
   // bytes of x at or past K count as 0, in the pieces that this lane copied
   auto clear = [&](int c) {
@@ -380,45 +382,61 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void k_q8_tile(Q8LinParams p) {
 #pragma unroll
     for (int t = 0; t < CT; ++t)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) acc[i][t][e] = 0;
-  const int r = lane & 31, h = lane >> 5;
-  int xo[2], wo[2];
+      for (int e = 0; e < ACC; ++e) acc[i][t][e] = 0;
+  const int r = lane % S, g = lane / S;
+  int xo[KT], wo[KT];
 #pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    const int col = ((2 * s + h) ^ (r >> 1 & 3)) * 16;
-    xo[s] = (wm * RT * 32 + r) * kQ8Slab + col;
-    wo[s] = (BM + wn * CT * 32 + r) * kQ8Slab + col;
+  for (int s = 0; s < KT; ++s) {
+    const int col = ((64 / S * s + g) ^ (-(r >> 2) & 3)) * 16;
+    xo[s] = (wm * RT * S + r) * kQ8Slab + col;
+    wo[s] = (BM + wn * CT * S + r) * kQ8Slab + col;
   }
-  struct Set { u32x4 x[2][RT], w[2][CT]; };
-  auto read = [&](int c, Set& q) {
-    const char* b = smem + c % NS * STAGE;
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-#pragma unroll
-      for (int i = 0; i < RT; ++i) q.x[s][i] = *reinterpret_cast<const u32x4*>(b + xo[s] + i * 32 * kQ8Slab);
-#pragma unroll
-      for (int t = 0; t < CT; ++t) q.w[s][t] = *reinterpret_cast<const u32x4*>(b + wo[s] + t * 32 * kQ8Slab);
-    }
+  struct Set { u32x4 x[KT][RT], w[KT][CT]; };
+  // operand j of slab c, in the products' order of k, x before W
+  constexpr int OPS = KT * (RT + CT);
+  auto read1 = [&](const char* b, int j, Set& q) {
+    const int s = j / (RT + CT), i = j % (RT + CT);
+    if (i < RT) q.x[s][i] = *reinterpret_cast<const u32x4*>(b + xo[s] + i * S * kQ8Slab);
+    else q.w[s][i - RT] = *reinterpret_cast<const u32x4*>(b + wo[s] + (i - RT) * S * kQ8Slab);
   };
-  // STEADY: slab c + NS is one more to fetch
+  auto read = [&](int c, Set& q) {
+#pragma unroll
+    for (int j = 0; j < OPS; ++j) read1(smem + c % NS * STAGE, j, q);
+  };
+  auto product = [&](const Set& q, int j) {
+    const int s = j / (RT * CT), t = j / RT % CT, i = j % RT;
+    acc[i][t] = F::mma(q.x[s][i], q.w[s][t], acc[i][t]);
+  };
+  // Slab c's products; STEADY: slab c + NS is one more to fetch.  Its copies and
+  // the reads of slab c + 1 are spread over the products, the reads early.
   auto step = [&](auto steady, int c, const Set& cur, Set& nxt) {
+    constexpr int PROD = KT * RT * CT, G = PROD < 8 ? PROD : 8, PG = PROD / G, RG = (OPS + G * 3 / 4 - 1) / (G * 3 / 4);
     if constexpr (decltype(steady)::value) {
       wait_copies<(NS - 2) * PW>();
       lds_barrier();
-      fetch(c + NS);
-      read(c + 1, nxt);
-    } else if (c + 1 < nsl) {                        // uniform
+      const char* b = smem + (c + 1) % NS * STAGE;
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+#pragma unroll
+        for (int q = g * PW / G; q < (g + 1) * PW / G; ++q) copy(c + NS, q);
+#pragma unroll
+        for (int j = 0; j < RG; ++j)
+          if (g * RG + j < OPS) read1(b, g * RG + j, nxt);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < PG; ++j) product(cur, g * PG + j);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      return;
+    }
+    if (c + 1 < nsl) {                               // uniform
       wait_copies<0>();
       if (c + 2 == nsl && p.K % kQ8Slab) clear(c + 1);
       lds_barrier();
       read(c + 1, nxt);
     }
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int t = 0; t < CT; ++t)
-#pragma unroll
-        for (int i = 0; i < RT; ++i) acc[i][t] = F::mma(cur.x[s][i], cur.w[s][t], acc[i][t]);
+    for (int j = 0; j < KT * RT * CT; ++j) product(cur, j);
   };
   for (int c = 0; c < NS && c < nsl; ++c) fetch(c);
   if (nsl >= NS) wait_copies<(NS - 1) * PW>();
@@ -442,41 +460,41 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void k_q8_tile(Q8LinParams p) {
     if (c + 1 < nsl) step(BoolC<false>{}, c + 1, b, a);
   }
 
-  // A strip of 32 rows at a time leaves through this wave's part of LDS: lane (r,
-  // h) writes its column of each tile, then holds 8 columns of a row.
+  // A strip of S rows at a time leaves through this wave's part of LDS: lane (r,
+  // g) writes its column of each tile, then holds 8 columns of a row.
   lds_barrier();
-  float* xs = reinterpret_cast<float*>(smem + NW * 32 * TP * 4);
+  float* xs = reinterpret_cast<float*>(smem + NW * S * TP * 4);
   for (int i = tid; i < BM; i += 64 * NW) xs[i] = p.xs[min(m0 + i, p.M - 1)];
   float ws[CT], bias[CT];
 #pragma unroll
   for (int t = 0; t < CT; ++t) {
-    const int n = SW ? (t & 1) * p.cols + min(o0 + wn * WOUT + t / 2 * 32 + r, p.cols - 1)
-                     : min(o0 + wn * WOUT + t * 32 + r, p.cols - 1);
+    const int n = SW ? (t & 1) * p.cols + min(o0 + wn * WOUT + t / 2 * S + r, p.cols - 1)
+                     : min(o0 + wn * WOUT + t * S + r, p.cols - 1);
     ws[t] = p.ws[n];
     bias[t] = p.bias ? p.bias[n] : 0.0f;
   }
   __syncthreads();
-  float* tr = reinterpret_cast<float*>(smem) + wave * 32 * TP;
+  float* tr = reinterpret_cast<float*>(smem) + wave * S * TP;
 #pragma unroll
   for (int i = 0; i < RT; ++i) {
-    const int row0 = wm * RT * 32 + i * 32;          // of the tile
+    const int row0 = (wm * RT + i) * S;          // of the tile
     if (m0 + row0 >= p.M) break;                     // uniform
 #pragma unroll
-    for (int ii = 0; ii < 4; ++ii) {
-      const f32x4 sx = *reinterpret_cast<const f32x4*>(xs + row0 + 8 * ii + 4 * h);
+    for (int ii = 0; ii < ACC / 4; ++ii) {
+      const f32x4 sx = *reinterpret_cast<const f32x4*>(xs + row0 + F::row(g, 4 * ii));
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        float* d = tr + (8 * ii + 4 * h + e) * TP + r;
+        float* d = tr + F::row(g, 4 * ii + e) * TP + r;
         auto val = [&](int t) {
           const float v = (float)acc[i][t][4 * ii + e] * sx[e] * ws[t];
           return p.bias ? v + bias[t] : v;
         };
         if constexpr (SW) {
 #pragma unroll
-          for (int t = 0; t < CT; t += 2) d[t / 2 * 32] = q8_swiglu(val(t), val(t + 1));
+          for (int t = 0; t < CT; t += 2) d[t / 2 * S] = q8_swiglu(val(t), val(t + 1));
         } else {
 #pragma unroll
-          for (int t = 0; t < CT; ++t) d[t * 32] = val(t);
+          for (int t = 0; t < CT; ++t) d[t * S] = val(t);
         }
       }
     }
@@ -485,7 +503,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void k_q8_tile(Q8LinParams p) {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     constexpr int LR = WOUT / 8, RP = 64 / LR;       // lanes a row, rows a pass
 #pragma unroll 1
-    for (int q = 0; q < 32 / RP; ++q) {
+    for (int q = 0; q < S / RP; ++q) {
       const int row = q * RP + lane / LR, col = lane % LR * 8;
       float v[8];
 #pragma unroll
@@ -503,7 +521,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void k_q8_tile(Q8LinParams p) {
   }
 }
 
-template <int BM, int BN, int WM, int WN, int NS, int OCC, bool SW>
+template <int S, int BM, int BN, int WM, int WN, int NS, int OCC, bool SW>
 int q8_tile(Q8LinParams p, hipStream_t st) {
   constexpr int OC = SW ? BN / 2 : BN;
   p.mt = (p.M + BM - 1) / BM;
@@ -512,12 +530,12 @@ int q8_tile(Q8LinParams p, hipStream_t st) {
   if (total >= INT_MAX - 64 || (int64_t)8 * p.nt >= INT_MAX || !launch_fits(total + 8, 64 * WM * WN))
     return VNX_ERR_UNSUPPORTED;
   const unsigned wgs = (unsigned)((total + kQ8Xcds - 1) / kQ8Xcds * kQ8Xcds);
-  hipLaunchKernelGGL((k_q8_tile<BM, BN, WM, WN, NS, OCC, SW>), dim3(wgs), dim3(64 * WM * WN), 0, st, p);
+  hipLaunchKernelGGL((k_q8_tile<S, BM, BN, WM, WN, NS, OCC, SW>), dim3(wgs), dim3(64 * WM * WN), 0, st, p);
   VNX_LAUNCH_CHECK();
   return VNX_OK;
 }
 
-constexpr int kQ8Shapes = 4;
+constexpr int kQ8Shapes = 8;
 
 template <bool SW>
 int q8_linear(const Q8LinParams& p, int force, hipStream_t st) {
@@ -530,8 +548,12 @@ int q8_linear(const Q8LinParams& p, int force, hipStream_t st) {
   switch (shape) {
     case 0: return q8_direct<16, 1, 2, 4, 1, SW>(p, st);
     case 1: return q8_direct<32, 2, 2, 2, 1, SW>(p, st);
-    case 2: return q8_tile<128, 128, 2, 2, 4, 2, SW>(p, st);
-    default: return q8_tile<256, 256, 2, 2, 4, 1, SW>(p, st);
+    case 2: return q8_tile<32, 128, 128, 2, 2, 4, 2, SW>(p, st);
+    case 3: return q8_tile<16, 256, 256, 2, 2, 4, 1, SW>(p, st);
+    case 4: return q8_tile<32, 256, 256, 2, 4, 4, 1, SW>(p, st);
+    case 5: return q8_tile<16, 256, 256, 2, 4, 4, 1, SW>(p, st);
+    case 6: return q8_tile<16, 128, 128, 2, 2, 4, 2, SW>(p, st);
+    default: return q8_tile<16, 256, 256, 2, 4, 5, 1, SW>(p, st);
   }
 }
 
