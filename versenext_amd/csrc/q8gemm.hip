@@ -4,12 +4,8 @@
 //   y[m, n] = acc * x_scale[m] * w_scale[n] (+ bias[n]) (+ residual[m, n])
 // or, of gate rows and up rows, silu(gate) * up.  The sums are whole numbers, so
 // how K is split never changes a result.
-//
-// k_q8_direct: operands straight from global memory to the matrix cores (the
-// order of k inside a product is free as long as both operands have the same,
-// so each lane loads whole pieces of its row), the K pieces of a tile shared by
-// KW waves whose sums meet in LDS.
 #include <climits>
+#include <utility>
 
 #include "q8.h"
 
@@ -36,6 +32,7 @@ struct Q8LinParams {
   int cols;        // columns of y: N, or N / 2
   int mt, nt;      // tiles
   int res_dtype, y_dtype;
+  int y_vec;       // rows of y lie on 16 bytes
 };
 
 // Up to eight columns n.. of row m: y = v (already scaled, with bias or SwiGLU
@@ -88,197 +85,140 @@ __device__ __forceinline__ void q8_scale8(const Q8LinParams& p, float xs, int r,
 #pragma unroll
     for (int i = 0; i < 8; ++i) s[i] = p.ws[min(r + i, rows - 1)];
   }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = (float)a[i] * xs * s[i];
+  float b[8] = {0, 0, 0, 0, 0, 0, 0, 0};
   if (p.bias) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] += p.bias[min(r + i, rows - 1)];
+    for (int i = 0; i < 8; ++i) b[i] = p.bias[min(r + i, rows - 1)];
   }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = fmaf((float)a[i] * xs, s[i], b[i]);
 }
 
-template <int S>
-struct Mfma;
-template <>
-struct Mfma<16> {
-  typedef i32x4 Acc;
-  static constexpr int P = 2;          // 16-byte pieces of a lane's row a chunk
-  __device__ __forceinline__ static Acc mma(u32x4 a, u32x4 b, Acc c) {
-    return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
-  }
-  // row of the tile that register e of lane group g holds
-  __device__ __forceinline__ static int row(int g, int e) { return 4 * g + e; }
-};
-template <>
-struct Mfma<32> {
-  typedef i32x16 Acc;
-  static constexpr int P = 4;
-  __device__ __forceinline__ static Acc mma(u32x4 a, u32x4 b, Acc c) {
-    return __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
-  }
-  __device__ __forceinline__ static int row(int g, int e) { return 8 * (e >> 2) + 4 * g + (e & 3); }
-};
+__device__ __forceinline__ i32x4 q8_mma(u32x4 a, u32x4 b, i32x4 c) {
+  return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
+}
 
-// A workgroup: MT x S rows of x by NW waves' NT x S rows of W each; SW: a wave's
-// tiles are gate and up rows in turn.
-template <int S, int MT, int NT, int KW, int NW, bool SW>
-__global__ __launch_bounds__(64 * KW * NW) void k_q8_direct(Q8LinParams p) {
-  using F = Mfma<S>;
-  constexpr int P = F::P, ACC = S * S / 64;
-  constexpr int ROWS = S * MT, WCOLS = S * NT, PITCH = WCOLS + 4;
-  constexpr int OCOLS = SW ? WCOLS / 2 : WCOLS;    // columns of y a wave
-  __shared__ __attribute__((aligned(16))) int red[KW * NW * ROWS * PITCH];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int kw = wave % KW, nw = wave / KW;
-  const int r = lane % S, g = lane / S;
+// ---------------------------------------------------------------------------
+// k_q8_direct: few rows of y.  A workgroup owns 16 rows of x and 16 of W; its KW
+// waves take chunks of 128 bytes of k in turn, operands straight from memory to
+// the matrix cores, and their sums meet in LDS.  The order of k inside a product
+// is free as long as both operands have the same, so a lane loads two 16-byte
+// pieces side by side of its row (lane (r, g): row r, bytes 32 g .. + 32), whole
+// lines over the wave.
+// ---------------------------------------------------------------------------
+template <int KW>
+__global__ __launch_bounds__(64 * KW) void k_q8_direct(Q8LinParams p) {
+  constexpr int PITCH = 20;                          // of a row of sums
+  __shared__ __attribute__((aligned(16))) int red[KW * 16 * PITCH];
+  const int tid = threadIdx.x, lane = tid & 63, kw = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = lane & 15, g = lane >> 4;
   // the row tiles that share W rows follow each other on one XCD
   const int xcd = blockIdx.x % kQ8Xcds, at = blockIdx.x / kQ8Xcds;
-  const int mi = at % p.mt, ni = at / p.mt * kQ8Xcds + xcd;
-  if (ni >= p.nt) return;  // uniform over the workgroup
-  const int m0 = mi * ROWS, o0 = (ni * NW + nw) * OCOLS;   // first row and column of y
-  const int8_t *xp[MT], *wp[NT];
+  const int m0 = at % p.mt * 16, n0 = (at / p.mt * kQ8Xcds + xcd) * 16;
+  if (n0 >= p.N) return;                             // uniform over the workgroup
+  const int8_t* xp = p.x + (int64_t)min(m0 + r, p.M - 1) * p.ldx + g * 32;
+  const int8_t* wp = p.w + (int64_t)min(n0 + r, p.N - 1) * p.ldw + g * 32;
+  i32x4 acc = {0, 0, 0, 0};
+  struct Set { u32x4 x[2], w[2]; };
+  const int nf = p.K / kQ8Chunk, mine = nf > kw ? (nf - kw + KW - 1) / KW : 0;  // whole chunks, and this wave's
+  auto load = [&](int i, Set& q) {                   // this wave's chunk i
+    const int64_t k = (int64_t)(kw + i * KW) * kQ8Chunk;
 #pragma unroll
-  for (int i = 0; i < MT; ++i) xp[i] = p.x + (int64_t)min(m0 + i * S + r, p.M - 1) * p.ldx + g * (16 * P);
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const int row = SW ? min(o0 + t / 2 * S + r, p.cols - 1) + (t & 1) * p.cols : min(o0 + t * S + r, p.N - 1);
-    wp[t] = p.w + (int64_t)row * p.ldw + g * (16 * P);
-  }
-  typename F::Acc acc[MT][NT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int e = 0; e < ACC; ++e) acc[i][t][e] = 0;
-
-  struct Set { u32x4 x[MT][P], w[NT][P]; };
-  const int nf = p.K / kQ8Chunk;
-  auto load = [&](int c, Set& q) {
-    const int64_t k = (int64_t)c * kQ8Chunk;
-#pragma unroll
-    for (int s = 0; s < P; ++s) {
-#pragma unroll
-      for (int t = 0; t < NT; ++t) q.w[t][s] = *reinterpret_cast<const u32x4*>(wp[t] + k + s * 16);
-#pragma unroll
-      for (int i = 0; i < MT; ++i) q.x[i][s] = *reinterpret_cast<const u32x4*>(xp[i] + k + s * 16);
+    for (int s = 0; s < 2; ++s) {
+      q.w[s] = *reinterpret_cast<const u32x4*>(wp + k + s * 16);
+      q.x[s] = *reinterpret_cast<const u32x4*>(xp + k + s * 16);
     }
   };
   auto mma = [&](const Set& q) {
 #pragma unroll
-    for (int s = 0; s < P; ++s)
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int i = 0; i < MT; ++i) acc[i][t] = F::mma(q.x[i][s], q.w[t][s], acc[i][t]);
+    for (int s = 0; s < 2; ++s) acc = q8_mma(q.x[s], q.w[s], acc);
   };
-  if (kw < nf) {
+  // two chunks under way, none of them loaded twice (a short row has no time for that)
+  if (mine == 1) {                                   // uniform, as the others
+    Set a;
+    load(0, a);
+    mma(a);
+  } else if (mine > 1) {
     Set a, b;
-    const int last = kw + (nf - 1 - kw) / KW * KW;   // this wave's last chunk
-    load(kw, a);
-    for (int c = kw; c < nf; c += 2 * KW) {
-      load(min(c + KW, last), b);
+    load(0, a);
+    load(1, b);
+    int i = 0;
+    for (; i + 3 < mine; i += 2) {
       mma(a);
-      load(min(c + 2 * KW, last), a);
-      if (c + KW < nf) mma(b);                       // uniform
+      load(i + 2, a);
+      mma(b);
+      load(i + 3, b);
     }
+    mma(a);
+    if (i + 2 < mine) load(i + 2, a);
+    mma(b);
+    if (i + 2 < mine) mma(a);
   }
   if (p.K % kQ8Chunk && kw == nf % KW) {
     // The last chunk's pieces: those past the row's end come from its start, and
     // every byte of x at or past K counts as 0 (of W there may be anything).
     Set q;
 #pragma unroll
-    for (int s = 0; s < P; ++s) {
+    for (int s = 0; s < 2; ++s) {
       const int64_t k = (int64_t)nf * kQ8Chunk + s * 16;
-      const int left = p.K - (int)k - g * (16 * P);  // bytes of this piece inside the row
-      const int64_t o = left > 0 ? k : -g * (16 * P);
+      const int left = p.K - (int)k - g * 32;        // bytes of this piece inside the row
+      const int64_t o = left > 0 ? k : -g * 32;
+      q.w[s] = *reinterpret_cast<const u32x4*>(wp + o);
+      u32x4 v = *reinterpret_cast<const u32x4*>(xp + o);
 #pragma unroll
-      for (int t = 0; t < NT; ++t) q.w[t][s] = *reinterpret_cast<const u32x4*>(wp[t] + o);
-#pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        u32x4 v = *reinterpret_cast<const u32x4*>(xp[i] + o);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int n = left - 4 * e;                // bytes of this word inside the row
-          v[e] = n >= 4 ? v[e] : n <= 0 ? 0u : v[e] & ((1u << (8 * n)) - 1u);
-        }
-        q.x[i][s] = v;
+      for (int e = 0; e < 4; ++e) {
+        const int n = left - 4 * e;                  // bytes of this word inside the row
+        v[e] = n >= 4 ? v[e] : n <= 0 ? 0u : v[e] & ((1u << (8 * n)) - 1u);
       }
+      q.x[s] = v;
     }
     mma(q);
   }
-
-  int* mine = red + wave * ROWS * PITCH;
 #pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int e = 0; e < ACC; ++e) mine[(i * S + F::row(g, e)) * PITCH + t * S + r] = acc[i][t][e];
+  for (int e = 0; e < 4; ++e) red[(kw * 16 + 4 * g + e) * PITCH + r] = acc[e];
   __syncthreads();
-  constexpr int GR = OCOLS / 8;                      // pieces of 8 columns a row and wave
-  for (int j = tid; j < ROWS * GR * NW; j += 64 * KW * NW) {
-    const int c = j % (GR * NW), row = j / (GR * NW), m = m0 + row;
-    const int w = c / GR, o = c % GR * 8;            // (OCOLS of each wave follow each other)
-    const int n = (ni * NW + w) * OCOLS + o;
-    if (m >= p.M || n >= p.cols) continue;
-    const int* src = red + w * KW * ROWS * PITCH + row * PITCH;
-    const float xs = p.xs[m];
-    auto sum8 = [&](int col, int (&a)[8]) {
+  if (tid >= 32) return;
+  const int row = tid >> 1, m = m0 + row, n = n0 + (tid & 1) * 8;
+  if (m >= p.M || n >= p.N) return;
+  int a[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) a[i] = 0;
+  for (int k = 0; k < KW; ++k) {
+    const int* src = red + (k * 16 + row) * PITCH + (tid & 1) * 8;
+    const i32x4 lo = *reinterpret_cast<const i32x4*>(src), hi = *reinterpret_cast<const i32x4*>(src + 4);
 #pragma unroll
-      for (int k = 0; k < KW; ++k) {
-        const i32x4 lo = *reinterpret_cast<const i32x4*>(src + k * ROWS * PITCH + col),
-                    hi = *reinterpret_cast<const i32x4*>(src + k * ROWS * PITCH + col + 4);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { a[i] += lo[i]; a[4 + i] += hi[i]; }
-      }
-    };
-    int a[8];
-    float v[8];
-    if constexpr (SW) {
-      float u[8];
-      const int col = o / S * 2 * S + o % S;         // the gate's; the up's is S further on
-      sum8(col, a);
-      q8_scale8(p, xs, n, p.cols, a, v);
-      sum8(col + S, a);
-      q8_scale8(p, xs, p.cols + n, p.N, a, u);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = q8_swiglu(v[i], u[i]);
-    } else {
-      sum8(o, a);
-      q8_scale8(p, xs, n, p.N, a, v);
-    }
-    q8_out8(p, m, n, v);
+    for (int i = 0; i < 4; ++i) { a[i] += lo[i]; a[4 + i] += hi[i]; }
   }
+  float v[8];
+  q8_scale8(p, p.xs[m], n, p.N, a, v);
+  q8_out8(p, m, n, v);
 }
 
-template <int S, int MT, int NT, int KW, int NW, bool SW>
+template <int KW>
 int q8_direct(Q8LinParams p, hipStream_t st) {
-  constexpr int OC = NW * S * NT / (SW ? 2 : 1);
-  p.mt = (p.M + S * MT - 1) / (S * MT);
-  p.nt = (p.cols + OC - 1) / OC;
+  p.mt = (p.M + 15) / 16;
+  p.nt = (p.N + 15) / 16;
   const int64_t wgs = (int64_t)p.mt * ((p.nt + kQ8Xcds - 1) / kQ8Xcds * kQ8Xcds);
-  if (wgs >= INT_MAX || !launch_fits(wgs, 64 * KW * NW)) return VNX_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL((k_q8_direct<S, MT, NT, KW, NW, SW>), dim3((unsigned)wgs), dim3(64 * KW * NW), 0, st, p);
+  if (wgs >= INT_MAX || !launch_fits(wgs, 64 * KW)) return VNX_ERR_UNSUPPORTED;
+  hipLaunchKernelGGL((k_q8_direct<KW>), dim3((unsigned)wgs), dim3(64 * KW), 0, st, p);
   VNX_LAUNCH_CHECK();
   return VNX_OK;
 }
 
 // ---------------------------------------------------------------------------
-// k_q8_tile: many rows.  BM x BN tiles of y, WM x WN waves, slabs of 64 bytes of
-// k in a ring of NS buffers in LDS.
+// k_q8_tile: BM x BN tiles of y, WM x WN waves, slabs of KS parts of 64 bytes of k
+// in a ring of NS buffers in LDS, a tile a workgroup.
 //
 // The slabs come by direct copies from memory to LDS (1 KB an instruction: 16
 // rows of 64 bytes, lane l's 16 bytes at 16 l), so the tile's layout is made by
-// which piece of its row a lane asks for: piece c of row R lies at c ^ (R / 4 %
+// which piece of its row a lane asks for: piece c of row R lies at c ^ (-R / 4 %
 // 4), and the sixteen lanes that LDS serves together, four runs of four rows,
-// read sixteen different 16-byte columns of its 256.  A wave holds two sets of operands: it reads slab c + 1
-// while the products of slab c run, and slab c + NS comes into the buffer that
-// slab c has left, so one barrier a slab does.
+// read sixteen different 16-byte columns of its 256.  A wave holds two sets of
+// operands: it reads slab g + 1 while the products of slab g run, and slab g + NS
+// comes into the buffer that slab g has left, so one barrier a slab does.
+//
+// W is the products' first operand: lane (r, g) then holds four columns of y of
+// row r, which it stores itself.
 // ---------------------------------------------------------------------------
-constexpr int kQ8Slab = 64;
-
 __device__ __forceinline__ uint32_t lds_addr(const void* p) {
   return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
 }
@@ -288,7 +228,12 @@ __device__ __forceinline__ void copy_to_lds(uint32_t to, uint32_t off, const int
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                :
                : "s"(to), "v"(off), "s"(base)
-               : "memory", "m0");
+               : "memory");
+}
+
+// Lane l's value at p to LDS at `to` + 4 l.
+__device__ __forceinline__ void copy_to_lds(uint32_t to, const float* p) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" : : "s"(to), "v"(p) : "memory");
 }
 
 // Waits until at most N of this wave's copies are under way.
@@ -297,42 +242,93 @@ __device__ __forceinline__ void wait_copies() {
   asm volatile("s_waitcnt vmcnt(%0)" : : "i"(N) : "memory");
 }
 
-// Every wave's LDS reads so far are done, and every wave is here.
+// Every wave's LDS reads and writes so far are done, and every wave is here.
 __device__ __forceinline__ void lds_barrier() {
   __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0), in a form that the compiler counts with
   asm volatile("s_barrier" : : : "memory");
 }
 
-template <int S, int BM, int BN, int WM, int WN, int NS, int OCC, bool SW>
+template <typename F, int... J>
+__device__ __forceinline__ void each(F&& f, std::integer_sequence<int, J...>) {
+  (f(IntC<J>{}), ...);
+}
+
+// Four values rounded to TY at p (on its own size only).
+template <typename TY>
+__device__ __forceinline__ void q8_st4(TY* p, const float (&v)[4]) {
+  if constexpr (sizeof(TY) == 4) {
+    const f32x4 a = {v[0], v[1], v[2], v[3]};
+    __builtin_memcpy(p, &a, 16);
+  } else {
+    u32x2 o;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if constexpr (__is_same(TY, _Float16))
+        o[i] = __builtin_bit_cast(uint32_t, f16x2{(_Float16)v[2 * i], (_Float16)v[2 * i + 1]});
+      else o[i] = kv_pk_bf16(v[2 * i], v[2 * i + 1]);
+    }
+    __builtin_memcpy(p, &o, 8);
+  }
+}
+
+// v += the residual's four values from element o on.
+__device__ __forceinline__ void q8_add4(const Q8LinParams& p, int64_t o, float (&v)[4]) {
+  if (p.res_dtype == VNX_F32) {  // uniform
+    f32x4 a;
+    __builtin_memcpy(&a, static_cast<const float*>(p.res) + o, 16);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] += a[i];
+  } else {
+    u32x2 a;
+    __builtin_memcpy(&a, static_cast<const uint16_t*>(p.res) + o, 8);
+    const bool bf = p.res_dtype == VNX_BF16;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t w = a[i / 2];
+      const float x = __uint_as_float(i & 1 ? w & 0xFFFF0000u : w << 16), y = (float)__builtin_bit_cast(f16x2, w)[i & 1];
+      v[i] += bf ? x : y;
+    }
+  }
+}
+
+__device__ __forceinline__ float q8_res1(const Q8LinParams& p, int64_t o) {
+  return p.res_dtype == VNX_F32    ? q8_ld1(static_cast<const float*>(p.res) + o)
+         : p.res_dtype == VNX_BF16 ? q8_ld1(static_cast<const uint16_t*>(p.res) + o)
+                                   : q8_ld1(static_cast<const _Float16*>(p.res) + o);
+}
+
+template <typename TY, bool RES, bool SW, int BM, int BN, int WM, int WN, int KS, int NS, int OCC>
 __global__ __launch_bounds__(64 * WM * WN, OCC) void k_q8_tile(Q8LinParams p) {
-  using F = Mfma<S>;
-  constexpr int NW = WM * WN, RT = BM / WM / S, CT = BN / WN / S, KT = S / 16;
-  constexpr int STAGE = (BM + BN) * kQ8Slab, PW = (BM + BN) / 16 / NW;
-  static_assert((BM + BN) / 16 % NW == 0 && (NS - 1) * PW < 64 && (!SW || CT % 2 == 0), "");
-  constexpr int ACC = S * S / 64, WCOLS = CT * S, WOUT = SW ? WCOLS / 2 : WCOLS, OC = SW ? BN / 2 : BN;
-  constexpr int TP = WOUT + 4;                       // row pitch (floats) of a wave's output strip
-  constexpr int EPI = NW * S * TP * 4 + BM * 4;
-  constexpr int SM = NS * STAGE > EPI ? NS * STAGE : EPI;
-  __shared__ __attribute__((aligned(128))) char smem[SM];
+  constexpr int NW = WM * WN, RT = BM / WM / 16, CT = BN / WN / 16;
+  constexpr int SLAB = 64 * KS, PART = (BM + BN) * 64, STAGE = KS * PART, OC = SW ? BN / 2 : BN;
+  constexpr int PW = (BM + BN) / 16 / NW, CW = PW * KS;  // a wave's copies of a part, and of a slab
+  static_assert((BM + BN) / 16 % NW == 0 && (NS - 1) * CW < 64 && NS % 2 == 0 && (!SW || CT % 2 == 0) && BM % 64 == 0 &&
+                    BN % 64 == 0, "");
+  __shared__ __attribute__((aligned(256))) char smem[NS * STAGE];
+  __shared__ __attribute__((aligned(256))) float scales[BM + 2 * BN];  // of x, of W, the bias
+  // results: tiles of a row (CTO, ST in a strip), values in 16 bytes, lanes a row, pitch
+  constexpr int CTO = SW ? CT / 2 : CT, VE = 16 / sizeof(TY), ST = CTO < 8 / (int)sizeof(TY) ? CTO : 8 / (int)sizeof(TY);
+  constexpr int LR = ST * 16 / VE, SP = ST * 16 * (int)sizeof(TY) + 16;
+  static_assert(CTO % ST == 0, "");
+  static_assert(NW * 16 * SP <= NS * STAGE, "");     // (the ring is free by then)
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = wave / WN, wn = wave % WN;
+  const int wm = wave / WN, wn = wave % WN, r = lane & 15, g4 = lane >> 4;
   // Each XCD takes a run of tiles, in blocks of eight rows of tiles: the tiles
   // that run at once on it share rows of x and of W in its L2.
-  int mi, ni;
+  int m0, o0;                                        // first row and column of y
   {
-    const int total = p.mt * p.nt, run = (total + kQ8Xcds - 1) / kQ8Xcds;
-    const int at = blockIdx.x / kQ8Xcds, i = blockIdx.x % kQ8Xcds * run + at;
+    const int total = p.mt * p.nt, run = (total + kQ8Xcds - 1) / kQ8Xcds, at = blockIdx.x / kQ8Xcds;
+    const int i = blockIdx.x % kQ8Xcds * run + at;
     if (at >= run || i >= total) return;             // uniform over the workgroup
-    const int blk = i / (8 * p.nt), in = i - blk * 8 * p.nt, h = min(8, p.mt - blk * 8);
-    mi = blk * 8 + in % h;
-    ni = in / h;
+    const int blk = i / (8 * p.nt), in = i - blk * 8 * p.nt, h = min(8, p.mt - blk * 8), ni = in / h;
+    m0 = (blk * 8 + in - ni * h) * BM;
+    o0 = ni * OC;
   }
-  const int m0 = mi * BM, o0 = ni * OC;              // first row and column of y
-  const int nsl = (p.K + kQ8Slab - 1) / kQ8Slab;
+  const int nsl = (p.K + 2 * SLAB - 1) / (2 * SLAB) * 2;  // an even number: the last may be all zeros
   const uint32_t lds0 = lds_addr(smem);
 
-  // this wave's copies of a slab: rows 16 (wave PW + q) + lane / 4 of [x tile; W tile]
-  const int piece = (lane & 3) ^ (-(lane >> 4) & 3);    // of the row's four in a slab
+  // this wave's copies of a part: rows 16 (wave PW + q) + lane / 4 of [x tile; W tile]
+  const int piece = (lane & 3) ^ (-(lane >> 4) & 3); // of the row's four in a part
   uint32_t off[PW];
   const int8_t* base[PW];                            // uniform
 #pragma unroll
@@ -342,218 +338,293 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void k_q8_tile(Q8LinParams p) {
       base[q] = p.x + (int64_t)m0 * p.ldx;
       off[q] = (uint32_t)min(r0 + (lane >> 2), p.M - 1 - m0) * (uint32_t)p.ldx + piece * 16;
     } else {
-      const int w0 = r0 - BM, up = SW ? w0 / S & 1 : 0, row = SW ? w0 / (2 * S) * S + w0 % S : w0;
+      const int w0 = r0 - BM, up = SW ? w0 / 16 & 1 : 0, row = SW ? w0 / 32 * 16 : w0;
       base[q] = p.w + (int64_t)(up ? p.cols + o0 : o0) * p.ldw;
       off[q] = (uint32_t)min(row + (lane >> 2), p.cols - 1 - o0) * (uint32_t)p.ldw + piece * 16;
     }
   }
-  // copy q of slab c
-  auto copy = [&](int c, int q) {
-    // (a piece past the row's end: the slab's first instead)
-    const uint32_t back = c * kQ8Slab + piece * 16 < p.K ? 0u : piece * 16u;
-    copy_to_lds(lds0 + c % NS * STAGE + (wave * PW + q) * 1024, off[q] - back, base[q] + (int64_t)c * kQ8Slab);
+  // copy j of slab c (a piece past the row's end: its first instead)
+  auto copy = [&](int c, int j) {
+    const int part = j / PW, q = j % PW, k = c * SLAB + part * 64;
+    const uint32_t back = k + piece * 16 < p.K ? 0u : piece * 16u;
+    const uint32_t to = lds0 + c % NS * STAGE + part * PART + (wave * PW + q) * 1024;
+    copy_to_lds(__builtin_amdgcn_readfirstlane(to), off[q] - back, base[q] + (k < p.K ? k : 0));
   };
-  auto fetch = [&](int c) {
-#pragma unroll
-    for (int q = 0; q < PW; ++q) copy(c, q);
-  };
-  // bytes of x at or past K count as 0, in the pieces that this lane copied
+  // bytes of x at or past K count as 0, in the pieces of slab c that this lane copied
   auto clear = [&](int c) {
-    const int left = p.K - c * kQ8Slab - piece * 16;
-    if (left < 16) {
 #pragma unroll
-      for (int q = 0; q < PW; ++q) {
-        if ((wave * PW + q) * 16 >= BM) continue;
-        u32x4* d = reinterpret_cast<u32x4*>(smem + c % NS * STAGE + (wave * PW + q) * 1024 + lane * 16);
-        u32x4 v = *d;
+    for (int j = 0; j < CW; ++j) {
+      const int part = j / PW, q = j % PW, in = p.K - c * SLAB - part * 64 - piece * 16;
+      if ((wave * PW + q) * 16 >= BM || in >= 16) continue;
+      u32x4* d = reinterpret_cast<u32x4*>(smem + c % NS * STAGE + part * PART + (wave * PW + q) * 1024 + lane * 16);
+      u32x4 v = *d;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int n = left - 4 * e;
-          v[e] = n >= 4 ? v[e] : n <= 0 ? 0u : v[e] & ((1u << (8 * n)) - 1u);
-        }
-        *d = v;
+      for (int e = 0; e < 4; ++e) {
+        const int n = in - 4 * e;
+        v[e] = n >= 4 ? v[e] : n <= 0 ? 0u : v[e] & ((1u << (8 * n)) - 1u);
       }
+      *d = v;
     }
   };
 
-  typename F::Acc acc[RT][CT];
+  // ---- operands and products ----
+  i32x4 acc[RT][CT];
+  const int col = (g4 ^ (-(r >> 2) & 3)) * 16;
+  const int xo = (wm * RT * 16 + r) * 64 + col, wo = (BM + wn * CT * 16 + r) * 64 + col;
+  struct Set { u32x4 x[KS][RT], w[KS][CT]; };
+  constexpr int OPS = KS * (RT + CT), PROD = KS * RT * CT;
+  auto read1 = [&](const char* b, int j, Set& q) {
+    const int part = j / (RT + CT), i = j % (RT + CT);
+    b += part * PART;
+    if (i < CT) q.w[part][i] = *reinterpret_cast<const u32x4*>(b + wo + i * 1024);
+    else q.x[part][i - CT] = *reinterpret_cast<const u32x4*>(b + xo + (i - CT) * 1024);
+  };
+  auto product = [&](const Set& q, int j) {
+    const int part = j / (RT * CT), i = j / CT % RT, t = i & 1 ? CT - 1 - j % CT : j % CT;
+    acc[i][t] = q8_mma(q.w[part][t], q.x[part][i], acc[i][t]);
+  };
+  // Slab c's products.  The copies of slab c + NS (COPY) and the reads of slab c + 1
+  // (unless LAST) are spread over them, the reads early.  left: of the slabs behind
+  // c + 1, how many are under way.
+  auto step = [&](auto left, auto copies, auto last, int c, const Set& cur, Set& nxt) {
+    constexpr bool COPY = decltype(copies)::value, LAST = decltype(last)::value;
+    constexpr int G = PROD < 8 ? PROD : 8, PG = PROD / G, RG = (OPS + G * 3 / 4 - 1) / (G * 3 / 4);
+    static_assert(PROD % G == 0, "");
+    if constexpr (!LAST) {
+      wait_copies<decltype(left)::value * CW>();
+      if ((c + 2) * SLAB > p.K) clear(c + 1);     // uniform
+      lds_barrier();
+    }
+    const char* b = smem + (c + 1) % NS * STAGE;
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+#pragma unroll
+      for (int j = 0; j < PG; ++j) product(cur, g * PG + j);
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (COPY)
+#pragma unroll
+        for (int q = g * CW / G; q < (g + 1) * CW / G; ++q) copy(c + NS, q);
+      if constexpr (!LAST)
+#pragma unroll
+        for (int j = 0; j < RG; ++j)
+          if (g * RG + j < OPS) read1(b, g * RG + j, nxt);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+
+  // the scales, 64 a copy
+  for (int u = wave; u < (BM + (p.bias ? 2 : 1) * BN) / 64; u += NW) {
+    const int j = u * 64 + lane;
+    const float* src;
+    if (u * 64 < BM) {
+      src = p.xs + m0 + min(j, p.M - 1 - m0);
+    } else {
+      const int w = j < BM + BN ? j - BM : j - BM - BN, up = SW ? w / 16 & 1 : 0, row = SW ? w / 32 * 16 + w % 16 : w;
+      src = (j < BM + BN ? p.ws : p.bias) + (int64_t)up * p.cols + min(o0 + row, p.cols - 1);
+    }
+    copy_to_lds(lds_addr(scales) + u * 256, src);
+  }
+  if (!p.bias)
+    for (int i = tid; i < BN; i += 64 * NW) scales[BM + BN + i] = 0.0f;
+#pragma unroll 1
+  for (int c = 0; c < NS; ++c)                       // (of fewer slabs: the first again, not read)
+#pragma unroll
+    for (int j = 0; j < CW; ++j) copy(c, j);
 #pragma unroll
   for (int i = 0; i < RT; ++i)
 #pragma unroll
     for (int t = 0; t < CT; ++t)
 #pragma unroll
-      for (int e = 0; e < ACC; ++e) acc[i][t][e] = 0;
-  const int r = lane % S, g = lane / S;
-  int xo[KT], wo[KT];
-#pragma unroll
-  for (int s = 0; s < KT; ++s) {
-    const int col = ((64 / S * s + g) ^ (-(r >> 2) & 3)) * 16;
-    xo[s] = (wm * RT * S + r) * kQ8Slab + col;
-    wo[s] = (BM + wn * CT * S + r) * kQ8Slab + col;
-  }
-  struct Set { u32x4 x[KT][RT], w[KT][CT]; };
-  // operand j of slab c, in the products' order of k, x before W
-  constexpr int OPS = KT * (RT + CT);
-  auto read1 = [&](const char* b, int j, Set& q) {
-    const int s = j / (RT + CT), i = j % (RT + CT);
-    if (i < RT) q.x[s][i] = *reinterpret_cast<const u32x4*>(b + xo[s] + i * S * kQ8Slab);
-    else q.w[s][i - RT] = *reinterpret_cast<const u32x4*>(b + wo[s] + (i - RT) * S * kQ8Slab);
-  };
-  auto read = [&](int c, Set& q) {
-#pragma unroll
-    for (int j = 0; j < OPS; ++j) read1(smem + c % NS * STAGE, j, q);
-  };
-  auto product = [&](const Set& q, int j) {
-    const int s = j / (RT * CT), t = j / RT % CT, i = j % RT;
-    acc[i][t] = F::mma(q.x[s][i], q.w[s][t], acc[i][t]);
-  };
-  // Slab c's products; STEADY: slab c + NS is one more to fetch.  Its copies and
-  // the reads of slab c + 1 are spread over the products, the reads early.
-  auto step = [&](auto steady, int c, const Set& cur, Set& nxt) {
-    constexpr int PROD = KT * RT * CT, G = PROD < 8 ? PROD : 8, PG = PROD / G, RG = (OPS + G * 3 / 4 - 1) / (G * 3 / 4);
-    if constexpr (decltype(steady)::value) {
-      wait_copies<(NS - 2) * PW>();
-      lds_barrier();
-      const char* b = smem + (c + 1) % NS * STAGE;
-#pragma unroll
-      for (int g = 0; g < G; ++g) {
-#pragma unroll
-        for (int q = g * PW / G; q < (g + 1) * PW / G; ++q) copy(c + NS, q);
-#pragma unroll
-        for (int j = 0; j < RG; ++j)
-          if (g * RG + j < OPS) read1(b, g * RG + j, nxt);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int j = 0; j < PG; ++j) product(cur, g * PG + j);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      return;
-    }
-    if (c + 1 < nsl) {                               // uniform
-      wait_copies<0>();
-      if (c + 2 == nsl && p.K % kQ8Slab) clear(c + 1);
-      lds_barrier();
-      read(c + 1, nxt);
-    }
-#pragma unroll
-    for (int j = 0; j < KT * RT * CT; ++j) product(cur, j);
-  };
-  for (int c = 0; c < NS && c < nsl; ++c) fetch(c);
-  if (nsl >= NS) wait_copies<(NS - 1) * PW>();
-  else wait_copies<0>();
-  if (nsl == 1 && p.K % kQ8Slab) clear(0);
+      for (int e = 0; e < 4; ++e) acc[i][t][e] = 0;
+  wait_copies<(NS - 1) * CW>();
+  if (SLAB > p.K) clear(0);
   lds_barrier();
   Set a, b;
-  read(0, a);
+#pragma unroll
+  for (int j = 0; j < OPS; ++j) read1(smem, j, a);
+  constexpr auto yes = BoolC<true>{};
+  constexpr auto no = BoolC<false>{};
   int c = 0;
-  for (; c + 1 + NS < nsl; c += 2) {
-    step(BoolC<true>{}, c, a, b);
-    step(BoolC<true>{}, c + 1, b, a);
-  }
-  if (c + NS < nsl) {                                // an odd one: the sets change places
-    step(BoolC<true>{}, c, a, b);
-    a = b;
-    ++c;
-  }
-  for (; c < nsl; c += 2) {
-    step(BoolC<false>{}, c, a, b);
-    if (c + 1 < nsl) step(BoolC<false>{}, c + 1, b, a);
-  }
-
-  // A strip of S rows at a time leaves through this wave's part of LDS: lane (r,
-  // g) writes its column of each tile, then holds 8 columns of a row.
-  lds_barrier();
-  float* xs = reinterpret_cast<float*>(smem + NW * S * TP * 4);
-  for (int i = tid; i < BM; i += 64 * NW) xs[i] = p.xs[min(m0 + i, p.M - 1)];
-  float ws[CT], bias[CT];
-#pragma unroll
-  for (int t = 0; t < CT; ++t) {
-    const int n = SW ? (t & 1) * p.cols + min(o0 + wn * WOUT + t / 2 * S + r, p.cols - 1)
-                     : min(o0 + wn * WOUT + t * S + r, p.cols - 1);
-    ws[t] = p.ws[n];
-    bias[t] = p.bias ? p.bias[n] : 0.0f;
-  }
-  __syncthreads();
-  float* tr = reinterpret_cast<float*>(smem) + wave * S * TP;
-#pragma unroll
-  for (int i = 0; i < RT; ++i) {
-    const int row0 = (wm * RT + i) * S;          // of the tile
-    if (m0 + row0 >= p.M) break;                     // uniform
-#pragma unroll
-    for (int ii = 0; ii < ACC / 4; ++ii) {
-      const f32x4 sx = *reinterpret_cast<const f32x4*>(xs + row0 + F::row(g, 4 * ii));
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float* d = tr + F::row(g, 4 * ii + e) * TP + r;
-        auto val = [&](int t) {
-          const float v = (float)acc[i][t][4 * ii + e] * sx[e] * ws[t];
-          return p.bias ? v + bias[t] : v;
-        };
-        if constexpr (SW) {
-#pragma unroll
-          for (int t = 0; t < CT; t += 2) d[t / 2 * S] = q8_swiglu(val(t), val(t + 1));
-        } else {
-#pragma unroll
-          for (int t = 0; t < CT; ++t) d[t * S] = val(t);
-        }
-      }
-    }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    constexpr int LR = WOUT / 8, RP = 64 / LR;       // lanes a row, rows a pass
 #pragma unroll 1
-    for (int q = 0; q < S / RP; ++q) {
-      const int row = q * RP + lane / LR, col = lane % LR * 8;
-      float v[8];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const f32x4 f = *reinterpret_cast<const f32x4*>(tr + row * TP + col + 4 * e);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[4 * e + j] = f[j];
-      }
-      const int m = m0 + row0 + row, n = o0 + wn * WOUT + col;
-      if (m < p.M && n < p.cols) q8_out8(p, m, n, v);
-    }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  for (; c + NS < nsl; c += 2) {
+    step(IntC<NS - 2>{}, yes, no, c, a, b);
+    step(IntC<NS - 2>{}, yes, no, c + 1, b, a);
   }
+  // the last NS slabs, or all of fewer (of which the last reads a slab for nothing)
+  auto tail = [&](auto at) {
+    constexpr int J = decltype(at)::value;
+    if (c + J >= nsl) return;                        // uniform
+    if constexpr (J % 2 == 0) step(IntC<NS - 2 - J>{}, no, no, c + J, a, b);
+    else if constexpr (J + 1 < NS) step(IntC<NS - 2 - J>{}, no, no, c + J, b, a);
+    else step(IntC<0>{}, no, yes, c + J, b, a);
+  };
+  each(tail, std::make_integer_sequence<int, NS>{});
+  wait_copies<0>();
+  lds_barrier();                                     // every wave has its operands: the ring is free
+
+  // Sixteen rows of up to 128 bytes at a time leave through a part of LDS of the
+  // wave's own, so that each store takes whole runs of a row; past the caches,
+  // which would hold the stores up (the 248,320 head at 224 rows: 105 us through
+  // them, 79 past, 74 with no stores at all).
+  auto leave = [&](auto edge) {
+    constexpr bool EDGE = decltype(edge)::value;
+    constexpr bool LATE = RES && sizeof(TY) == 4;  // the residual is added behind LDS, which holds fp32
+    const float* sw = scales + BM + wn * CT * 16 + 4 * g4;  // of this lane's W rows (read again and again: registers are few)
+    const int n0 = o0 + wn * CTO * 16;
+    char* mine = smem + wave * 16 * SP;
+    const int lr = lane / LR, lc = lane % LR * VE; // row and first column of this lane's 16 bytes
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      const int rl = (wm * RT + i) * 16;
+      const float sx = scales[rl + r];
+#pragma unroll
+      for (int q = 0; q < CTO; q += ST) {
+#pragma unroll
+        for (int u = 0; u < ST; ++u) {
+          const int t = (q + u) * (SW ? 2 : 1);
+          float v[4];
+          auto val = [&](int at, float (&d)[4]) {
+            const f32x4 w = *reinterpret_cast<const f32x4*>(sw + at * 16), c = *reinterpret_cast<const f32x4*>(sw + BN + at * 16);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) d[e] = fmaf((float)acc[i][at][e] * sx, w[e], c[e]);
+          };
+          val(t, v);
+          if constexpr (SW) {
+            float up[4];
+            val(t + 1, up);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = q8_swiglu(v[e], up[e]);
+          }
+          if constexpr (RES && !LATE) {
+            const int m = m0 + rl + r, n = n0 + (q + u) * 16 + 4 * g4;
+            const int64_t o = (int64_t)m * p.ldr + n;
+            if (!EDGE || (m < p.M && n + 4 <= p.cols)) {
+              q8_add4(p, o, v);
+            } else if (m < p.M) {
+#pragma unroll
+              for (int e = 0; e < 3; ++e)
+                if (n + e < p.cols) v[e] += q8_res1(p, o + e);
+            }
+          }
+          q8_st4(static_cast<TY*>(__builtin_assume_aligned(mine + r * SP + (u * 16 + 4 * g4) * (int)sizeof(TY), 4 * sizeof(TY))), v);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+        for (int h = 0; h < 16; h += 64 / LR) {
+          if (64 / LR > 16 && lr >= 16) break;
+          const int m = m0 + rl + h + lr, n = n0 + q * 16 + lc;
+          u32x4 d = *reinterpret_cast<const u32x4*>(mine + (h + lr) * SP + lane % LR * 16);
+          TY* y = static_cast<TY*>(p.y) + (int64_t)m * p.ldy + n;
+          if (!EDGE || (m < p.M && n + VE <= p.cols)) {
+            if constexpr (LATE) {
+              float v[4];
+              __builtin_memcpy(v, &d, 16);
+              q8_add4(p, (int64_t)m * p.ldr + n, v);
+              __builtin_memcpy(&d, v, 16);
+            }
+            if (p.y_vec) __builtin_nontemporal_store(d, reinterpret_cast<u32x4*>(y));
+            else __builtin_memcpy(y, &d, 16);
+          } else if (m < p.M) {
+            TY v[VE];
+            __builtin_memcpy(v, &d, 16);
+#pragma unroll
+            for (int e = 0; e < VE - 1; ++e) {
+              if (n + e >= p.cols) break;
+              if constexpr (LATE) v[e] += q8_res1(p, (int64_t)m * p.ldr + n + e);
+              y[e] = v[e];
+            }
+          }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+      }
+    }
+  };
+  if (m0 + BM <= p.M && o0 + OC <= p.cols) leave(BoolC<false>{});
+  else leave(BoolC<true>{});
 }
 
-template <int S, int BM, int BN, int WM, int WN, int NS, int OCC, bool SW>
+template <bool SW, int BM, int BN, int WM, int WN, int KS, int NS, int OCC>
 int q8_tile(Q8LinParams p, hipStream_t st) {
   constexpr int OC = SW ? BN / 2 : BN;
   p.mt = (p.M + BM - 1) / BM;
   p.nt = (p.cols + OC - 1) / OC;
   const int64_t total = (int64_t)p.mt * p.nt;
-  if (total >= INT_MAX - 64 || (int64_t)8 * p.nt >= INT_MAX || !launch_fits(total + 8, 64 * WM * WN))
-    return VNX_ERR_UNSUPPORTED;
-  const unsigned wgs = (unsigned)((total + kQ8Xcds - 1) / kQ8Xcds * kQ8Xcds);
-  hipLaunchKernelGGL((k_q8_tile<S, BM, BN, WM, WN, NS, OCC, SW>), dim3(wgs), dim3(64 * WM * WN), 0, st, p);
-  VNX_LAUNCH_CHECK();
-  return VNX_OK;
+  if (total >= INT_MAX / 2 || (int64_t)8 * p.nt >= INT_MAX) return VNX_ERR_UNSUPPORTED;
+  const int64_t wgs64 = (total + kQ8Xcds - 1) / kQ8Xcds * kQ8Xcds;
+  if (!launch_fits(wgs64, 64 * WM * WN)) return VNX_ERR_UNSUPPORTED;
+  const unsigned wgs = (unsigned)wgs64;
+  const int ey = elem_size(p.y_dtype);
+  p.y_vec = aligned16(p.y) && p.ldy * ey % 16 == 0;
+  return q8_by_type(p.y_dtype, [&](auto ty) -> int {
+    using TY = decltype(ty);
+    if constexpr (!SW) {
+      if (p.res) {
+        hipLaunchKernelGGL((k_q8_tile<TY, true, SW, BM, BN, WM, WN, KS, NS, OCC>), dim3(wgs), dim3(64 * WM * WN), 0, st, p);
+        VNX_LAUNCH_CHECK();
+        return VNX_OK;
+      }
+    }
+    hipLaunchKernelGGL((k_q8_tile<TY, false, SW, BM, BN, WM, WN, KS, NS, OCC>), dim3(wgs), dim3(64 * WM * WN), 0, st, p);
+    VNX_LAUNCH_CHECK();
+    return VNX_OK;
+  });
 }
 
-constexpr int kQ8Shapes = 8;
+// ---------------------------------------------------------------------------
+// Launch shapes, and the choice between them by an estimate of their time: n =
+// workgroups a CU, each of them `slab` us per 64 bytes of k (`alone` where less
+// than half of the CUs has one) and `rest` us besides.  Fitted to 60 sizes; us by
+// the estimate / measured (M x N x K; the shape taken first, then the others in
+// the order below):
+//   2,048 x 2,048 x 1,024    128^2 7.7 / 8.8; 256^2 16 / 16, 64 x 128 9.9 / 9.9, 64^2 12 / 11
+//   2,048 x 1,024 x 2,752    64 x 128 12 / 12.5; 256^2 34 / 33, 128^2 14 / 17, 64^2 15 / 14
+//   224 x 1,024 x 2,752      64^2 7.0 / 6.9; 128^2 14 / 14, 64 x 128 9.9 / 10, direct 11 / 8.6
+//   64 x 1,024 x 4,096       direct 5.5 / 5.7; 64^2 9.3 / 8.5
+//   1 x 248,320 x 1,024      direct 40 / 40; 64 x 128 29 / 47, which HBM holds up (51 in the estimate)
+// ---------------------------------------------------------------------------
+constexpr int kQ8Shapes = 5;
+struct Q8Shape { int bm, bn; double slab, alone, rest; };
+constexpr Q8Shape kQ8Tiles[4] = {
+    {256, 256, 0.85, 0.68, 3.0}, {128, 128, 0.32, 0.27, 0.6}, {64, 128, 0.23, 0.17, 0.4}, {64, 64, 0.14, 0.11, 0.25}};
+
+template <bool SW>
+int q8_plan(const Q8LinParams& p) {
+  const int64_t cus = device_cus();
+  const double slabs = (p.K + 63) / 64;
+  const double hbm = ((double)p.M * p.K + (double)p.N * p.K + (double)p.M * p.cols * elem_size(p.y_dtype)) / 5e6;
+  int best = 0;
+  double least = 1e300;
+  for (int i = 0; i < 4; ++i) {
+    const Q8Shape& s = kQ8Tiles[i];
+    const int oc = SW ? s.bn / 2 : s.bn;
+    const int64_t tiles = (int64_t)((p.M + s.bm - 1) / s.bm) * ((p.cols + oc - 1) / oc);
+    const double t = (double)((tiles + cus - 1) / cus) * (slabs * (2 * tiles <= cus ? s.alone : s.slab) + s.rest);
+    const double us = t > hbm ? t : hbm + 0.01 * t;
+    if (us < least) least = us, best = i;
+  }
+  if (!SW) {
+    // 16 x 16 of y a workgroup; rows of x that are one and the same line cost less
+    const int64_t wgs = (int64_t)((p.M + 15) / 16) * ((p.N + 15) / 16);
+    const double us = (double)(wgs > cus ? wgs : cus) / cus * slabs * (p.M <= 4 ? 0.039 : 0.055);
+    if (us < least) best = 4;
+  }
+  return best;
+}
 
 template <bool SW>
 int q8_linear(const Q8LinParams& p, int force, hipStream_t st) {
-  auto tiles = [&](int bm, int bn) {
-    const int oc = SW ? bn / 2 : bn;
-    return (int64_t)((p.M + bm - 1) / bm) * ((p.cols + oc - 1) / oc);
-  };
-  int shape = p.M <= 16 ? 0 : tiles(256, 256) >= 2 * device_cus() && p.M > 256 ? 3 : p.M > 128 ? 2 : 1;
-  if (force) shape = force - 1;
-  switch (shape) {
-    case 0: return q8_direct<16, 1, 2, 4, 1, SW>(p, st);
-    case 1: return q8_direct<32, 2, 2, 2, 1, SW>(p, st);
-    case 2: return q8_tile<32, 128, 128, 2, 2, 4, 2, SW>(p, st);
-    case 3: return q8_tile<16, 256, 256, 2, 2, 4, 1, SW>(p, st);
-    case 4: return q8_tile<32, 256, 256, 2, 4, 4, 1, SW>(p, st);
-    case 5: return q8_tile<16, 256, 256, 2, 4, 4, 1, SW>(p, st);
-    case 6: return q8_tile<16, 128, 128, 2, 2, 4, 2, SW>(p, st);
-    default: return q8_tile<16, 256, 256, 2, 4, 5, 1, SW>(p, st);
+  switch (force ? force - 1 : q8_plan<SW>(p)) {
+    case 0: return q8_tile<SW, 256, 256, 2, 4, 1, 4, 1>(p, st);
+    case 1: return q8_tile<SW, 128, 128, 2, 2, 1, 4, 2>(p, st);
+    case 2: return q8_tile<SW, 64, 128, 2, 2, 1, 4, 3>(p, st);
+    case 3: return q8_tile<SW, 64, 64, 2, 2, 2, 4, 2>(p, st);
+    default:
+      if constexpr (!SW) return q8_direct<4>(p, st);
+      return VNX_ERR_UNSUPPORTED;
   }
 }
 
