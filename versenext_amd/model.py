@@ -43,6 +43,11 @@ With kv_dtype (int8 or e4m3) the caches hold 8-bit codes and a scale a row and
 head: vnx_kv_write rotates, quantises and writes the new rows, vnx_tree_attn_q8
 attends over them (chunks of any length; vnx_kv_read and PyTorch where it does
 not apply).
+With w8a8 the dense products (q|k|v, output, SwiGLU FFN, LM head) take 8-bit
+integers on both sides: vnx_q8_rmsnorm norms the residual rows into codes and a
+scale a row, vnx_q8_quantize does so with the attention's and the activation's
+rows, vnx_q8_linear multiplies (SwiGLU and the residual's addition in it).  The
+MoD layers' routing and experts stay as they are.
 Prefill-size forwards (more rows than one verify round) take the same calls
 with the norms apart (vnx_rmsnorm) and, for the MoD layers, the row lists
 built first (vnx_mod_lists, vnx_expert_gemm_bf16_rows); INT4 models run their
@@ -295,6 +300,12 @@ def _deq_int4(w, hip) -> torch.Tensor:
     return hip.dequant_w4(wq, sc, w.shape[1], 128)
 
 
+def _deq_int8(w, hip) -> torch.Tensor:
+    """fp32 q * s of w quantized to INT8 with a scale a row (exact)."""
+    q, s = VQ.quantize_int8(w.float())
+    return hip.dequant_w8(q, s.reshape(-1))
+
+
 def _cat(ws):
     """Row concatenation of dense tensors or of Int4Weights (per-row groups,
     so the packed rows and scales concatenate as they are)."""
@@ -351,8 +362,9 @@ class _Linear:
     M <= 64 rows and a dequantized copy (bit-exact q * s) for larger M
     (prefill)."""
 
-    def __init__(self, w, dtype, hip, int4: bool, swiglu: bool = False, rope_head_dim: int = 0):
+    def __init__(self, w, dtype, hip, int4: bool, swiglu: bool = False, rope_head_dim: int = 0, w8a8: bool = False):
         self.N, self.K = w.shape
+        self.w8a8 = bool(w8a8)
         self.wq_rope = None
         self.wt = None
         self.dtype = dtype
@@ -361,7 +373,16 @@ class _Linear:
         self.int4 = pre or (bool(int4) and self.K % 128 == 0)
         self.wp = None
         self.swiglu = bool(swiglu) and self.N % 32 == 0
-        if self.int4:
+        if self.w8a8:
+            # INT8, a scale a row, rows on 16 bytes; in row blocks, so that no
+            # temporary of a large matrix (the head) is larger than 64 MB
+            self.q = hip._rows16(torch.empty((self.N, self.K), dtype=torch.int8, device=hip.torch_device))
+            self.qs = torch.empty(self.N, dtype=torch.float32, device=hip.torch_device)
+            rb = max(1, (16 << 20) // self.K)
+            for r0 in range(0, self.N, rb):
+                q, s = VQ.quantize_int8(w[r0:r0 + rb].float())
+                self.q[r0:r0 + rb], self.qs[r0:r0 + rb] = q, s.reshape(-1)
+        elif self.int4:
             wq, sc = (w.wq, w.sc) if pre else VQ.quantize_int4_g(w.float(), 128)
             self.wq, self.sc = wq.contiguous(), sc.contiguous()
             if self.swiglu:
@@ -416,6 +437,10 @@ class _Linear:
     GEMM_MAX_M = 256
     # rows from which an INT4 weight also keeps the tiled copy (the LM head)
     TILES_MIN_N = 32768
+
+    def q8(self, codes: torch.Tensor, scale: torch.Tensor, **kw) -> torch.Tensor:
+        """linear_q8 of 8-bit rows with this INT8 weight (w8a8)."""
+        return self.hip.linear_q8(codes, scale, self.q, self.qs, **kw)
 
     def gemm(self, x: torch.Tensor, epilogue: int = 0, out_dtype=None) -> Optional[torch.Tensor]:
         """vnx_gemm_bf16 of the packed weight for x (bf16 rows): (M, N), or
@@ -561,8 +586,11 @@ class _Linear:
     def __call__(self, x: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """x (M, K); returns (M, N) in the compute dtype (dense) or fp32
         (INT4 GEMV, written into `out` when given: an (M, N) view with unit
-        column stride, fp32, or bf16 for the tiled large-N product)."""
+        column stride, fp32, or bf16 for the tiled large-N product; w8a8: in
+        the compute dtype, or into `out`)."""
         M = x.shape[0]
+        if self.w8a8:
+            return self.q8(*self.hip.quantize_rows(x), out_dtype=self.dtype, out=out)
         if self.int4 and M <= 64:
             x16 = x.to(torch.float16).contiguous()
             y = out if out is not None else torch.empty((M, self.N), dtype=torch.float32, device=x.device)
@@ -605,10 +633,18 @@ class CometSparkGPU:
 
     kv_dtype torch.int8 or torch.float8_e4m3fn: the cache in 8 bits (half its
     bytes, to hold and to read; heads of 16 to 256, a power of two; dtype
-    bfloat16).  None: in dtype."""
+    bfloat16).  None: in dtype.
+
+    w8a8: dense products in 8-bit integers, weights with a scale a row and
+    activations with a scale a token (half the weights' bytes of a bfloat16
+    model; dtype bfloat16, not with int4)."""
 
     def __init__(self, cfg: ModelConfig, weights: Dict[str, torch.Tensor], hip, batch: int, capacity: int,
-                 dtype=torch.bfloat16, int4: bool = False, kv_dtype: Optional[torch.dtype] = None):
+                 dtype=torch.bfloat16, int4: bool = False, kv_dtype: Optional[torch.dtype] = None,
+                 w8a8: bool = False):
+        if w8a8 and (int4 or dtype != torch.bfloat16):
+            raise ValueError("w8a8 needs dtype bfloat16 and int4 False")
+        self.w8a8 = bool(w8a8)
         if kv_dtype is not None:
             if kv_dtype not in (torch.int8, torch.float8_e4m3fn):
                 raise ValueError(f"kv_dtype must be torch.int8 or torch.float8_e4m3fn, got {kv_dtype}")
@@ -649,9 +685,9 @@ class CometSparkGPU:
                 raise ValueError(f"head.weight has shape {tuple(Hw.shape)}, expected {(cfg.vocab_size, D)}")
             if isinstance(Hw, Int4Weight) and not int4:
                 raise ValueError("an INT4 head needs int4=True")
-        self.head = _Linear(Hw, dtype, hip, int4) if int4 else None
+        self.head = _Linear(Hw, dtype, hip, int4, w8a8=w8a8) if int4 or w8a8 else None
         # the dense head matrix of the bf16 / fp32 logits path
-        self.head_w = None if int4 else (self.emb if cfg.tie_weights else Hw.to(dtype).contiguous())
+        self.head_w = None if int4 or w8a8 else (self.emb if cfg.tie_weights else Hw.to(dtype).contiguous())
         # its packed copy for vnx_gemm_bf16 (224 rows x 248,320: 143 us against
         # vnx_lm_head's 172 on the row layout, 4 rows 84 against 101, the same
         # sums; 2 V D bytes beside a table the embedding needs as it is)
@@ -664,21 +700,23 @@ class CometSparkGPU:
             g = W[p + "attn.global_tokens.weight"]
             G = g.shape[0]
             # the global sinks go through the same k / v weights as the tokens:
-            # with INT4 weights, their exact dequantization q * s
-            wk_g, wv_g = (wk, wv) if not (int4 and D % 128 == 0) else (_deq_int4(wk, hip), _deq_int4(wv, hip))
+            # with INT4 or INT8 weights, their exact dequantization q * s
+            deq = _deq_int4 if int4 and D % 128 == 0 else _deq_int8 if w8a8 else lambda w, hip: w
+            wk_g, wv_g = deq(wk, hip), deq(wv, hip)
             gk = (g @ wk_g.t()).reshape(G, cfg.n_kv_head, d).permute(1, 0, 2).unsqueeze(0)
             gv = (g @ wv_g.t()).reshape(G, cfg.n_kv_head, d).permute(1, 0, 2).unsqueeze(0)
             L = _Layer(kind=kind, norm1=W[p + "norm1.weight"], norm2=W[p + "norm2.weight"],
                        wqkv=_Linear(_cat([wq, wk, wv]), dtype, hip, int4,
                                     # (for the GEMVs that write bf16 cache rows: not with an 8-bit cache)
-                                    rope_head_dim=d if dtype == torch.bfloat16 and int4 and kv_dtype is None else 0),
-                       proj=_Linear(W[p + "attn.proj.weight"], dtype, hip, int4),
+                                    rope_head_dim=d if dtype == torch.bfloat16 and int4 and kv_dtype is None else 0,
+                                    w8a8=w8a8),
+                       proj=_Linear(W[p + "attn.proj.weight"], dtype, hip, int4, w8a8=w8a8),
                        gk=gk.to(dtype).contiguous(), gv=gv.to(dtype).contiguous(),
                        gates=torch.sigmoid(W[p + "attn.gate_logits"].float()).contiguous())
             if kind == "trisparse":
                 L.ffn["gu"] = _Linear(_cat([W[p + "ffn.w_gate.weight"], W[p + "ffn.w_up.weight"]]),
-                                      dtype, hip, int4, swiglu=True)
-                L.ffn["down"] = _Linear(W[p + "ffn.w_down.weight"], dtype, hip, int4)
+                                      dtype, hip, int4, swiglu=True, w8a8=w8a8)
+                L.ffn["down"] = _Linear(W[p + "ffn.w_down.weight"], dtype, hip, int4, w8a8=w8a8)
             else:
                 P, E = cfg.num_dense_parts, cfg.num_experts_per_part
                 # routing logits [part router | expert routers, part-major] in
@@ -739,7 +777,7 @@ class CometSparkGPU:
     @classmethod
     def from_vn(cls, path: str, hip, batch: int, capacity: int, dtype=torch.bfloat16, int4: bool = True,
                 chunk_bytes: int = 64 << 20, cfg: Optional[ModelConfig] = None,
-                kv_dtype: Optional[torch.dtype] = None) -> "CometSparkGPU":
+                kv_dtype: Optional[torch.dtype] = None, w8a8: bool = False) -> "CometSparkGPU":
         """The model saved in a .vn file (CometSparkNexLM.save_vn /
         CometSparkV05LM.save_vn, cometspark.py:1014-1060; loaded by the
         reference through VNFileReader, spark/mate/model/model.py:271-285),
@@ -759,7 +797,7 @@ class CometSparkGPU:
                                 chunk_bytes=chunk_bytes, skip=lambda n: tied and n == "head.weight")
         if cfg is None:
             cfg = config_from_vn(conf, W, name=f"{path} (.vn)")
-        return cls(cfg, W, hip, batch, capacity, dtype, int4, kv_dtype)
+        return cls(cfg, W, hip, batch, capacity, dtype, int4, kv_dtype, w8a8)
 
     # ---- pieces ---------------------------------------------------------
     def _st(self) -> int:
@@ -1140,6 +1178,13 @@ class CometSparkGPU:
             elif li == 0 and norm_in and self.embed_fold and (qkv := L.wqkv.gemm_norm_embed(
                     tok, self.emb, self.emb_scale, x, L.norm1, cfg.eps)) is not None:
                 pass                                       # embedding, norm and q|k|v: one call
+            elif self.w8a8:
+                if li == 0:                                # x = emb[tok] * scale (its norm's rows are not used)
+                    self._embed_rms(tok, L.norm1, x, torch.empty((M, D), dtype=self.act_dtype, device=self.dev))
+                codes, sc, _ = self.hip.rmsnorm_q8(x, L.norm1, cfg.eps, residual=pending,
+                                                     sum_out=x if pending is not None else None)
+                pending = None
+                qkv = L.wqkv.q8(codes, sc)
             elif li == 0:
                 h = torch.empty((M, D), dtype=self.act_dtype, device=self.dev)
                 self._embed_rms(tok, L.norm1, x, h)        # token embedding folded into the first norm
@@ -1200,7 +1245,19 @@ class CometSparkGPU:
                 if act is None or not L.ffn["down"].gemv_residual(act, x):
                     raise RuntimeError("fused INT4 FFN path unavailable for this layer")
                 continue
-            a = L.proj(o)
+            if self.w8a8:
+                L.proj.q8(*self.hip.quantize_rows(o), residual=x, out=x)
+                if L.kind == "trisparse":
+                    codes, sc, _ = self.hip.rmsnorm_q8(x, L.norm2, cfg.eps)
+                    act = L.ffn["gu"].q8(codes, sc, swiglu=True)
+                    L.ffn["down"].q8(*self.hip.quantize_rows(act), residual=x, out=x)
+                    continue
+                if "w1p" in L.ffn:
+                    self._mod_routed(L, x, L.norm2, x, True)
+                    continue
+                a = None                                   # (x holds it already)
+            else:
+                a = L.proj(o)
             # MoD layers route on fp32 rows, as the reference does
             h2 = torch.empty((M, D), dtype=torch.float32 if L.kind == "mod" else self.act_dtype, device=self.dev)
             self._rms(x, a, L.norm2, h2)
@@ -1211,8 +1268,8 @@ class CometSparkGPU:
 
     def head_writes_bf16(self) -> bool:
         """Whether logits(out=<bf16 tensor>) is written by the head itself:
-        the bf16 LM head (vnx_gemm_bf16 on its packed copy), or an INT4 head on
-        its tiled copy (vnx_gemv_w4_tiles_out)."""
+        the bf16 LM head (vnx_gemm_bf16 on its packed copy), an INT4 head on
+        its tiled copy (vnx_gemv_w4_tiles_out), or a w8a8 one (vnx_q8_linear)."""
         if self.head is not None:
             return self.head.wt is not None if self.head.int4 else self.dtype == torch.bfloat16
         return self.dtype == torch.bfloat16
@@ -1221,7 +1278,8 @@ class CometSparkGPU:
         """(B, n, V) logits of the LM head (the tied embedding, or
         head.weight when untied), fp32 or in out's dtype (bf16 where
         head_writes_bf16()): vnx_gemm_bf16 (bf16, matrix cores) on the packed
-        head, vnx_gemv_w4 for an INT4 draft, F.linear for an fp32 model."""
+        head, vnx_gemv_w4 for an INT4 draft, vnx_q8_linear for a w8a8 model,
+        F.linear for an fp32 model."""
         B, n, D = hidden.shape
         V = self.cfg.vocab_size
         if D != self.cfg.dim:
@@ -1231,6 +1289,8 @@ class CometSparkGPU:
             if out is not None:
                 self.head(h2, out=out.view(B * n, V))
                 return out
+            if self.w8a8:
+                return self.head.q8(*self.hip.quantize_rows(h2), out_dtype=torch.float32).view(B, n, V)
             return self.head(h2).view(B, n, V)
         if self.head_p is not None:
             x = h2.to(self.dev, torch.bfloat16).contiguous()

@@ -12,7 +12,9 @@ device) follow packages/verse_torch/verse_torch/quantize.py:
 
 `QuantizedLinear` mirrors the reference class (quantize.py:382-582): it holds
 the packed weight and scales on the GPU and runs `forward` on the gfx950
-dequant-GEMV kernels (vnx_linear_w4 / vnx_linear_w8), y = x @ W^T (+ bias).
+dequant-GEMV kernels (vnx_linear_w4 / vnx_linear_w8), y = x @ W^T (+ bias).  With
+act_bits=8 an INT8 weight meets activations in 8 bits too, quantised row by row
+(vnx_q8_quantize, vnx_q8_linear).
 """
 from __future__ import annotations
 
@@ -22,7 +24,9 @@ import numpy as np
 import torch
 from torch.autograd import forward_ad
 
+from ._lib import DTYPE_CODES
 from .device import get_backend
+from .hip_backend import _to_tensor
 
 
 def _div(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
@@ -116,14 +120,18 @@ class QuantizedLinear:
 
     qtype "int8": per-channel int8; "int4": per-channel int4 with fp32 scales
     (the reference's format); "int4_g128": group-128 int4 with fp16 scales.
-    forward(x) takes (..., in) activations (rounded to fp16, as the kernels read)
-    and returns (..., out) fp32."""
+    forward(x) takes (..., in) activations (rounded to fp16, as the kernels read;
+    with act_bits=8, for qtype "int8", to 8-bit integers with a scale a row) and
+    returns (..., out) fp32."""
 
     QTYPES = ("int8", "int4", "int4_g128")
 
-    def __init__(self, weight, bias=None, qtype: str = "int4_g128", device: str = "rocm"):
+    def __init__(self, weight, bias=None, qtype: str = "int4_g128", device: str = "rocm", act_bits: int = 16):
         if qtype not in self.QTYPES:
             raise ValueError(f"qtype must be one of {self.QTYPES}, got {qtype!r}")
+        if act_bits not in (8, 16) or (act_bits == 8 and qtype != "int8"):
+            raise ValueError(f"act_bits is 16, or 8 for qtype 'int8': got {act_bits} for {qtype!r}")
+        self.act_bits = act_bits
         self.backend = get_backend(device)
         dev = self.backend.torch_device
         w = _f32(weight).to(dev)
@@ -134,6 +142,8 @@ class QuantizedLinear:
         if qtype == "int8":
             q, s = quantize_int8(w)
             self.wq, self.scale = q.contiguous(), s.reshape(-1).contiguous()
+            if act_bits == 8:
+                self.wq = self.backend._rows16(self.wq)    # (rows on 16 bytes, once)
         elif qtype == "int4":
             q, s = quantize_int4(w)
             self.wq, self.scale = q.contiguous(), s.reshape(-1, 1).contiguous()
@@ -167,6 +177,10 @@ class QuantizedLinear:
                 and (forward_ad._current_level < 0 or forward_ad.unpack_dual(b).tangent is None))
 
     def _product(self, x, bias) -> torch.Tensor:
+        if self.act_bits == 8:
+            t = _to_tensor(x, self.backend.torch_device)
+            codes, scale = self.backend.quantize_rows(t if t.dtype in DTYPE_CODES else t.float())
+            return self.backend.linear_q8(codes, scale, self.wq, self.scale, bias=bias, out_dtype=torch.float32)
         if self.qtype == "int8":
             return self.backend.gemv_w8(x, self.wq, self.scale, bias=bias)
         group = self.in_features if self.qtype == "int4" else 128
