@@ -1036,9 +1036,12 @@ int vnx_q8_dequantize(const int8_t* codes, int64_t ldc, const float* scale, int6
  * vnnn.py:779-807), no res.  y and res VNX_F32, VNX_BF16 or VNX_F16, rounded
  * once.  x and W on 16 bytes with pitches a multiple of 16 (below 2^22); bytes
  * of a row between K and its pitch are not used, whatever they hold.  y must not
- * share bytes with what is read but as said.  Codes may be -128.  force_shape
- * (tuning and tests): 1 + the index of a launch shape; 0: the plan's choice,
- * another value VNX_ERR_UNSUPPORTED. */
+ * share bytes with what is read but as said.  Codes may be -128.  One launch, or
+ * two when few tiles share a long k: the workspace (vnx_q8_linear_workspace(args)
+ * bytes, 16-byte aligned, no initialisation; it reads the sizes, types and
+ * epilogue only) then holds the partial sums.  force_shape (tuning and tests): 1
+ * + the index of a launch shape; 0: the plan's choice, another value
+ * VNX_ERR_UNSUPPORTED.  The result does not depend on the shape. */
 typedef struct vnx_q8_linear_args {
   const int8_t* x;
   const float* x_scale;
@@ -1052,7 +1055,8 @@ typedef struct vnx_q8_linear_args {
   int res_dtype, y_dtype, epilogue, force_shape;
 } vnx_q8_linear_args;
 
-int vnx_q8_linear(const vnx_q8_linear_args* args, void* stream);
+size_t vnx_q8_linear_workspace(const vnx_q8_linear_args* args);
+int vnx_q8_linear(const vnx_q8_linear_args* args, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -33,7 +33,7 @@ def linear(**over):
     for k, v in (dict(x=AT, x_scale=2 * AT, w=3 * AT, w_scale=4 * AT, bias=5 * AT, res=6 * AT, y=FAR, ldx=64, ldw=64,
                       ldr=32, ldy=32, M=4, N=32, K=64, res_dtype=_lib.VNX_BF16, y_dtype=_lib.VNX_F32) | over).items():
         setattr(a, k, v)
-    return _lib.lib().vnx_q8_linear(ctypes.byref(a), None)
+    return _lib.lib().vnx_q8_linear(ctypes.byref(a), None, 0, None)
 
 
 BAD = [
@@ -80,7 +80,8 @@ def test_no_rows(call):
 
 
 def test_null_block():
-    assert _lib.lib().vnx_q8_linear(None, None) == INVALID
+    assert _lib.lib().vnx_q8_linear(None, None, 0, None) == INVALID
+    assert _lib.lib().vnx_q8_linear_workspace(None) == 256
 
 
 def test_binding_leaves_calls_off_the_gpu():
@@ -92,6 +93,24 @@ def test_binding_leaves_calls_off_the_gpu():
         assert b.q8_rmsnorm(0, 0, n, s, 1e-6, None, None) is None
         assert b.q8_linear(0, 0, n, s, c, s, None, None, False, torch.float32, None) is None
     assert b.q8_quantize() is None and b.q8_linear(1, 2) is None and b.q8_rmsnorm(*range(7)) is None
-    for bad in ((), (1, 2, 3, 0), ("a", 1, 1, 1)):
+    for bad in ((), (1, 2, 3, 4, 0), ("a", 1, 1, 1, 1)):
         with pytest.raises((TypeError, ValueError)):
             b.init_q8(*bad)
+
+
+def test_workspace():
+    """Sums that are split over k need one; what the sizes alone refuse needs none."""
+    L, a = _lib.lib(), _lib.Q8LinearArgs()
+    for k, v in dict(ldx=8192, ldw=8192, ldy=64, M=64, N=64, K=8192, y_dtype=_lib.VNX_F32, force_shape=6).items():
+        setattr(a, k, v)
+    need = L.vnx_q8_linear_workspace(ctypes.byref(a))
+    assert need >= 2 * 64 * 64 * 4
+    a.x, a.x_scale, a.w, a.w_scale, a.y = AT, 2 * AT, 3 * AT, 4 * AT, FAR
+    for ws, n in ((None, need), (FAR * 2, need - 1), (FAR * 2 + 8, need)):
+        assert L.vnx_q8_linear(ctypes.byref(a), ws, n, None) == _lib.VNX_ERR_WORKSPACE
+    for over in (dict(M=0), dict(ldy=63), dict(force_shape=4), dict(K=0)):
+        for k, v in over.items():
+            old = getattr(a, k)
+            setattr(a, k, v)
+            assert L.vnx_q8_linear_workspace(ctypes.byref(a)) == 256
+            setattr(a, k, old)

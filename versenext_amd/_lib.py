@@ -232,7 +232,8 @@ SIGNATURES.update({
     "vnx_q8_rmsnorm": (_int, [_vp, _int, _c_i64, _vp, _int, _c_i64, _vp, _f32, _c_i64, _c_i64, _vp, _c_i64, _vp,
                               _c_i64, _vp, _vp]),
     "vnx_q8_dequantize": (_int, [_vp, _c_i64, _vp, _c_i64, _c_i64, _vp, _int, _c_i64, _vp]),
-    "vnx_q8_linear": (_int, [_vp, _vp]),
+    "vnx_q8_linear_workspace": (_c_sz, [_vp]),
+    "vnx_q8_linear": (_int, [_vp, _vp, _c_sz, _vp]),
     "vnx_kv_write": (_int, [_vp, _vp]),
     "vnx_kv_read": (_int, [_vp, _vp]),
     "vnx_tree_attn_q8_workspace": (_c_sz, [_vp]),
@@ -327,7 +328,7 @@ def bind():
             _vnx_bind.init(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
                 L.vnx_kv_write, L.vnx_kv_read, L.vnx_tree_attn_q8_workspace, L.vnx_tree_attn_q8)))
             _vnx_bind.init_q8(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
-                L.vnx_q8_quantize, L.vnx_q8_rmsnorm, L.vnx_q8_dequantize, L.vnx_q8_linear)))
+                L.vnx_q8_quantize, L.vnx_q8_rmsnorm, L.vnx_q8_dequantize, L.vnx_q8_linear_workspace, L.vnx_q8_linear)))
             _bind = _vnx_bind
     return _bind
 

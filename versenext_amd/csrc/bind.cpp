@@ -314,6 +314,7 @@ PyObject* tree_attn_q8(PyObject*, PyObject* const* a, Py_ssize_t n) {
 decltype(&vnx_q8_quantize) g_quantize;
 decltype(&vnx_q8_rmsnorm) g_rmsnorm;
 decltype(&vnx_q8_dequantize) g_dequantize;
+decltype(&vnx_q8_linear_workspace) g_linear_ws;
 decltype(&vnx_q8_linear) g_linear;
 
 // (rows, K) with unit last stride and rows that follow each other: its pitch in
@@ -488,7 +489,11 @@ PyObject* q8_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   p.x_scale = static_cast<const float*>(xs->data_ptr()), p.w_scale = static_cast<const float*>(ws->data_ptr());
   p.y = out->data_ptr(), p.y_dtype = code_of(out->scalar_type());
   p.epilogue = sw ? VNX_EPI_SWIGLU : VNX_EPI_NONE;
-  const int rc = g_linear(&p, st);
+  // a workspace of this call's own: a captured graph keeps it in its pool
+  const size_t need = g_linear_ws(&p);
+  at::Tensor buf;
+  if (need > 256) buf = at::empty({(int64_t)need}, x->options().dtype(at::kByte));
+  const int rc = g_linear(&p, need > 256 ? buf.data_ptr() : nullptr, need > 256 ? need : 0, st);
   if (rc != VNX_OK) return status(rc);
   if (a[10] != Py_None) {
     Py_INCREF(a[10]);
@@ -525,14 +530,15 @@ PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Py_RETURN_NONE;
 }
 
-// init_q8(address of vnx_q8_quantize, vnx_q8_rmsnorm, vnx_q8_dequantize, vnx_q8_linear)
+// init_q8(address of vnx_q8_quantize, vnx_q8_rmsnorm, vnx_q8_dequantize, vnx_q8_linear_workspace, vnx_q8_linear)
 PyObject* init_q8(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  void* f[4];
-  if (!addresses(a, n, 4, f)) return nullptr;
+  void* f[5];
+  if (!addresses(a, n, 5, f)) return nullptr;
   g_quantize = reinterpret_cast<decltype(g_quantize)>(f[0]);
   g_rmsnorm = reinterpret_cast<decltype(g_rmsnorm)>(f[1]);
   g_dequantize = reinterpret_cast<decltype(g_dequantize)>(f[2]);
-  g_linear = reinterpret_cast<decltype(g_linear)>(f[3]);
+  g_linear_ws = reinterpret_cast<decltype(g_linear_ws)>(f[3]);
+  g_linear = reinterpret_cast<decltype(g_linear)>(f[4]);
   Py_RETURN_NONE;
 }
 

@@ -33,6 +33,7 @@ struct Q8LinParams {
   int mt, nt;      // tiles
   int res_dtype, y_dtype;
   int y_vec;       // rows of y lie on 16 bytes
+  int per;         // slabs a split of k has (sums alone)
 };
 
 // Up to eight columns n.. of row m: y = v (already scaled, with bias or SwiGLU
@@ -217,7 +218,10 @@ int q8_direct(Q8LinParams p, hipStream_t st) {
 // comes into the buffer that slab g has left, so one barrier a slab does.
 //
 // W is the products' first operand: lane (r, g) then holds four columns of y of
-// row r, which it stores itself.
+// row r.
+//
+// TY int: the sums alone, of the p.per slabs of k that are blockIdx.y's, into the
+// 32-bit matrix [split][row][column] of whole tiles at p.y.
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t lds_addr(const void* p) {
   return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
@@ -324,7 +328,9 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void k_q8_tile(Q8LinParams p) {
     m0 = (blk * 8 + in - ni * h) * BM;
     o0 = ni * OC;
   }
-  const int nsl = (p.K + 2 * SLAB - 1) / (2 * SLAB) * 2;  // an even number: the last may be all zeros
+  constexpr bool SUMS = __is_same(TY, int);
+  const int k0 = SUMS ? (int)blockIdx.y * p.per * SLAB : 0, K = SUMS ? min(p.K - k0, p.per * SLAB) : p.K;
+  const int nsl = (K + 2 * SLAB - 1) / (2 * SLAB) * 2;  // an even number: the last may be all zeros
   const uint32_t lds0 = lds_addr(smem);
 
   // this wave's copies of a part: rows 16 (wave PW + q) + lane / 4 of [x tile; W tile]
@@ -335,26 +341,26 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void k_q8_tile(Q8LinParams p) {
   for (int q = 0; q < PW; ++q) {
     const int r0 = (wave * PW + q) * 16;
     if (r0 < BM) {
-      base[q] = p.x + (int64_t)m0 * p.ldx;
+      base[q] = p.x + (int64_t)m0 * p.ldx + k0;
       off[q] = (uint32_t)min(r0 + (lane >> 2), p.M - 1 - m0) * (uint32_t)p.ldx + piece * 16;
     } else {
       const int w0 = r0 - BM, up = SW ? w0 / 16 & 1 : 0, row = SW ? w0 / 32 * 16 : w0;
-      base[q] = p.w + (int64_t)(up ? p.cols + o0 : o0) * p.ldw;
+      base[q] = p.w + (int64_t)(up ? p.cols + o0 : o0) * p.ldw + k0;
       off[q] = (uint32_t)min(row + (lane >> 2), p.cols - 1 - o0) * (uint32_t)p.ldw + piece * 16;
     }
   }
   // copy j of slab c (a piece past the row's end: its first instead)
   auto copy = [&](int c, int j) {
     const int part = j / PW, q = j % PW, k = c * SLAB + part * 64;
-    const uint32_t back = k + piece * 16 < p.K ? 0u : piece * 16u;
+    const uint32_t back = k + piece * 16 < K ? 0u : piece * 16u;
     const uint32_t to = lds0 + c % NS * STAGE + part * PART + (wave * PW + q) * 1024;
-    copy_to_lds(__builtin_amdgcn_readfirstlane(to), off[q] - back, base[q] + (k < p.K ? k : 0));
+    copy_to_lds(__builtin_amdgcn_readfirstlane(to), off[q] - back, base[q] + (k < K ? k : 0));
   };
   // bytes of x at or past K count as 0, in the pieces of slab c that this lane copied
   auto clear = [&](int c) {
 #pragma unroll
     for (int j = 0; j < CW; ++j) {
-      const int part = j / PW, q = j % PW, in = p.K - c * SLAB - part * 64 - piece * 16;
+      const int part = j / PW, q = j % PW, in = K - c * SLAB - part * 64 - piece * 16;
       if ((wave * PW + q) * 16 >= BM || in >= 16) continue;
       u32x4* d = reinterpret_cast<u32x4*>(smem + c % NS * STAGE + part * PART + (wave * PW + q) * 1024 + lane * 16);
       u32x4 v = *d;
@@ -392,7 +398,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void k_q8_tile(Q8LinParams p) {
     static_assert(PROD % G == 0, "");
     if constexpr (!LAST) {
       wait_copies<decltype(left)::value * CW>();
-      if ((c + 2) * SLAB > p.K) clear(c + 1);     // uniform
+      if ((c + 2) * SLAB > K) clear(c + 1);     // uniform
       lds_barrier();
     }
     const char* b = smem + (c + 1) % NS * STAGE;
@@ -412,20 +418,22 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void k_q8_tile(Q8LinParams p) {
     }
   };
 
-  // the scales, 64 a copy
-  for (int u = wave; u < (BM + (p.bias ? 2 : 1) * BN) / 64; u += NW) {
-    const int j = u * 64 + lane;
-    const float* src;
-    if (u * 64 < BM) {
-      src = p.xs + m0 + min(j, p.M - 1 - m0);
-    } else {
-      const int w = j < BM + BN ? j - BM : j - BM - BN, up = SW ? w / 16 & 1 : 0, row = SW ? w / 32 * 16 + w % 16 : w;
-      src = (j < BM + BN ? p.ws : p.bias) + (int64_t)up * p.cols + min(o0 + row, p.cols - 1);
+  if constexpr (!SUMS) {
+    // the scales, 64 a copy
+    for (int u = wave; u < (BM + (p.bias ? 2 : 1) * BN) / 64; u += NW) {
+      const int j = u * 64 + lane;
+      const float* src;
+      if (u * 64 < BM) {
+        src = p.xs + m0 + min(j, p.M - 1 - m0);
+      } else {
+        const int w = j < BM + BN ? j - BM : j - BM - BN, up = SW ? w / 16 & 1 : 0, row = SW ? w / 32 * 16 + w % 16 : w;
+        src = (j < BM + BN ? p.ws : p.bias) + (int64_t)up * p.cols + min(o0 + row, p.cols - 1);
+      }
+      copy_to_lds(lds_addr(scales) + u * 256, src);
     }
-    copy_to_lds(lds_addr(scales) + u * 256, src);
+    if (!p.bias)
+      for (int i = tid; i < BN; i += 64 * NW) scales[BM + BN + i] = 0.0f;
   }
-  if (!p.bias)
-    for (int i = tid; i < BN; i += 64 * NW) scales[BM + BN + i] = 0.0f;
 #pragma unroll 1
   for (int c = 0; c < NS; ++c)                       // (of fewer slabs: the first again, not read)
 #pragma unroll
@@ -437,7 +445,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void k_q8_tile(Q8LinParams p) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[i][t][e] = 0;
   wait_copies<(NS - 1) * CW>();
-  if (SLAB > p.K) clear(0);
+  if (SLAB > K) clear(0);
   lds_barrier();
   Set a, b;
 #pragma unroll
@@ -460,6 +468,15 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void k_q8_tile(Q8LinParams p) {
   };
   each(tail, std::make_integer_sequence<int, NS>{});
   wait_copies<0>();
+  if constexpr (SUMS) {
+    const int64_t ld = (int64_t)p.nt * BN;
+    int* y = static_cast<int*>(p.y) + ((int64_t)blockIdx.y * p.mt * BM + m0 + wm * RT * 16 + r) * ld + o0 + wn * CT * 16 + 4 * g4;
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int t = 0; t < CT; ++t) *reinterpret_cast<i32x4*>(y + i * 16 * ld + t * 16) = acc[i][t];
+    return;
+  }
   lds_barrier();                                     // every wave has its operands: the ring is free
 
   // Sixteen rows of up to 128 bytes at a time leave through a part of LDS of the
@@ -543,8 +560,10 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void k_q8_tile(Q8LinParams p) {
       }
     }
   };
-  if (m0 + BM <= p.M && o0 + OC <= p.cols) leave(BoolC<false>{});
-  else leave(BoolC<true>{});
+  if constexpr (!SUMS) {
+    if (m0 + BM <= p.M && o0 + OC <= p.cols) leave(BoolC<false>{});
+    else leave(BoolC<true>{});
+  }
 }
 
 template <bool SW, int BM, int BN, int WM, int WN, int KS, int NS, int OCC>
@@ -586,17 +605,67 @@ int q8_tile(Q8LinParams p, hipStream_t st) {
 //   64 x 1,024 x 4,096       direct 5.5 / 5.7; 64^2 9.3 / 8.5
 //   1 x 248,320 x 1,024      direct 40 / 40; 64 x 128 29 / 47, which HBM holds up (51 in the estimate)
 // ---------------------------------------------------------------------------
-constexpr int kQ8Shapes = 5;
+constexpr int kQ8Direct = 4, kQ8Split = 5, kQ8Shapes = 6;
 struct Q8Shape { int bm, bn; double slab, alone, rest; };
 constexpr Q8Shape kQ8Tiles[4] = {
     {256, 256, 0.85, 0.68, 3.0}, {128, 128, 0.32, 0.27, 0.6}, {64, 128, 0.23, 0.17, 0.4}, {64, 64, 0.14, 0.11, 0.25}};
 
+// A split's sums joined: thread i has eight columns of a row.
 template <bool SW>
-int q8_plan(const Q8LinParams& p) {
+__global__ __launch_bounds__(256) void k_q8_join(Q8LinParams p, const int* part, int64_t split, int64_t ld, int splits) {
+  const int pieces = (p.cols + 7) / 8;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / pieces;
+  if (row >= p.M) return;
+  const int m = (int)row, n = (int)(i - row * pieces) * 8;
+  auto sum8 = [&](int col, int (&a)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) a[e] = 0;
+    const int* src = part + m * ld + col;
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s) {
+      i32x4 lo, hi;
+      __builtin_memcpy(&lo, src + s * split, 16);
+      __builtin_memcpy(&hi, src + s * split + 4, 16);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { a[e] += lo[e]; a[4 + e] += hi[e]; }
+    }
+  };
+  int a[8];
+  float v[8];
+  const float xs = p.xs[m];
+  sum8(n, a);
+  if constexpr (SW) {
+    float u[8];
+    q8_scale8(p, xs, n, p.cols, a, v);
+    sum8(p.cols + n, a);
+    q8_scale8(p, xs, p.cols + n, p.N, a, u);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = q8_swiglu(v[e], u[e]);
+  } else {
+    q8_scale8(p, xs, n, p.N, a, v);
+  }
+  q8_out8(p, m, n, v);
+}
+
+struct Q8Plan {
+  int shape, per, splits;  // kQ8Split: slabs of 128 a split, splits
+  size_t bytes;            // workspace
+};
+
+// The splits of k that 64 x 64 tiles in `want` of them have.
+Q8Plan q8_split(const Q8LinParams& p, int want) {
+  const int nsl = (p.K + 255) / 256 * 2, per = (nsl + 2 * want - 1) / (2 * want) * 2;
+  const int splits = (nsl + per - 1) / per;
+  const int64_t cells = (int64_t)((p.M + 63) / 64) * ((p.N + 63) / 64) * 4096;
+  return {kQ8Split, per, splits, (size_t)(cells * splits * 4 + 64)};  // (the join may read 28 bytes on)
+}
+
+template <bool SW>
+Q8Plan q8_plan(const Q8LinParams& p, int force) {
   const int64_t cus = device_cus();
   const double slabs = (p.K + 63) / 64;
   const double hbm = ((double)p.M * p.K + (double)p.N * p.K + (double)p.M * p.cols * elem_size(p.y_dtype)) / 5e6;
-  int best = 0;
+  Q8Plan best{0, 0, 0, 0};
   double least = 1e300;
   for (int i = 0; i < 4; ++i) {
     const Q8Shape& s = kQ8Tiles[i];
@@ -604,28 +673,76 @@ int q8_plan(const Q8LinParams& p) {
     const int64_t tiles = (int64_t)((p.M + s.bm - 1) / s.bm) * ((p.cols + oc - 1) / oc);
     const double t = (double)((tiles + cus - 1) / cus) * (slabs * (2 * tiles <= cus ? s.alone : s.slab) + s.rest);
     const double us = t > hbm ? t : hbm + 0.01 * t;
-    if (us < least) least = us, best = i;
+    if (us < least) least = us, best.shape = i;
   }
   if (!SW) {
     // 16 x 16 of y a workgroup; rows of x that are one and the same line cost less
     const int64_t wgs = (int64_t)((p.M + 15) / 16) * ((p.N + 15) / 16);
     const double us = (double)(wgs > cus ? wgs : cus) / cus * slabs * (p.M <= 4 ? 0.039 : 0.055);
-    if (us < least) best = 4;
+    if (us < least) least = us, best.shape = kQ8Direct;
   }
+  // Few tiles and a long k: a CU's 70 GB/s of copies to LDS bounds a tile, so k is
+  // shared by more of them, at the price of a second launch.  64 x 4,096 x 10,944
+  // 21.7 -> 13.1 us, 512 x 1,024 x 8,192 17.1 -> 13.8; 224 x 1,024 x 2,752 would
+  // take 7.8 (6.9 as it is).
+  const int64_t tiles = (int64_t)((p.M + 63) / 64) * ((p.N + 63) / 64);
+  if (force == kQ8Split + 1) least = 1e300;
+  for (int want = 2; want <= 32 && (want == 2 || tiles * want <= 2 * cus); want *= 2) {
+    const Q8Plan s = q8_split(p, want);
+    const int64_t wgs = tiles * s.splits;
+    const double us = 3.5 + (double)((wgs + cus - 1) / cus) * (s.per * 2 * (2 * wgs <= cus ? 0.11 : 0.14) + 0.25) +
+                      (double)s.bytes / 3e6;
+    if (us < 0.95 * least && s.bytes < (size_t)1 << 30) least = us, best = s;
+  }
+  if (force && force != kQ8Split + 1) best = {force - 1, 0, 0, 0};
   return best;
 }
 
 template <bool SW>
-int q8_linear(const Q8LinParams& p, int force, hipStream_t st) {
-  switch (force ? force - 1 : q8_plan<SW>(p)) {
+int q8_linear(const Q8LinParams& p, int force, void* workspace, size_t workspace_bytes, hipStream_t st) {
+  const Q8Plan plan = q8_plan<SW>(p, force);
+  switch (plan.shape) {
     case 0: return q8_tile<SW, 256, 256, 2, 4, 1, 4, 1>(p, st);
     case 1: return q8_tile<SW, 128, 128, 2, 2, 1, 4, 2>(p, st);
     case 2: return q8_tile<SW, 64, 128, 2, 2, 1, 4, 3>(p, st);
     case 3: return q8_tile<SW, 64, 64, 2, 2, 2, 4, 2>(p, st);
-    default:
+    case kQ8Direct:
       if constexpr (!SW) return q8_direct<4>(p, st);
       return VNX_ERR_UNSUPPORTED;
   }
+  if (!workspace || workspace_bytes < plan.bytes || !aligned16(workspace)) return VNX_ERR_WORKSPACE;
+  Q8LinParams q = p;
+  q.cols = p.N;  // (gate and up rows are columns like any)
+  q.y = workspace, q.per = plan.per;
+  q.mt = (p.M + 63) / 64, q.nt = (p.N + 63) / 64;
+  const int64_t tiles = ((int64_t)q.mt * q.nt + kQ8Xcds - 1) / kQ8Xcds * kQ8Xcds, rows = (int64_t)q.mt * 64;
+  const int64_t joins = ((int64_t)p.M * ((p.cols + 7) / 8) + 255) / 256;
+  if ((int64_t)q.mt * q.nt >= INT_MAX / 2 || (int64_t)8 * q.nt >= INT_MAX || !launch_fits(tiles * plan.splits, 256) ||
+      !launch_fits(joins, 256))
+    return VNX_ERR_UNSUPPORTED;
+  hipLaunchKernelGGL((k_q8_tile<int, false, false, 64, 64, 2, 2, 2, 4, 2>), dim3((unsigned)tiles, plan.splits), dim3(256), 0,
+                     st, q);
+  VNX_LAUNCH_CHECK();
+  hipLaunchKernelGGL((k_q8_join<SW>), dim3((unsigned)joins), dim3(256), 0, st, p, static_cast<const int*>(workspace),
+                     rows * q.nt * 64, (int64_t)q.nt * 64, plan.splits);
+  VNX_LAUNCH_CHECK();
+  return VNX_OK;
+}
+
+// The checks that need no pointer, and the sizes.
+int q8_sizes(const vnx_q8_linear_args* a, Q8LinParams* p) {
+  if (!a || a->M < 0 || a->N < 0 || a->K < 1 || a->ldx < a->K || a->ldw < a->K) return VNX_ERR_INVALID_ARG;
+  if (a->epilogue != VNX_EPI_NONE && a->epilogue != VNX_EPI_SWIGLU) return VNX_ERR_INVALID_ARG;
+  const bool sw = a->epilogue == VNX_EPI_SWIGLU;
+  const int64_t cols = sw ? a->N / 2 : a->N;
+  if ((sw && (a->N % 2 || a->res)) || a->ldy < cols || (a->res && a->ldr < cols)) return VNX_ERR_INVALID_ARG;
+  if (!q8_float(a->y_dtype) || (a->res && !q8_float(a->res_dtype))) return VNX_ERR_UNSUPPORTED;
+  // rows and columns are numbered to the end of their last tile in 32 bits
+  if (a->K > kQ8MaxK || a->M >= INT_MAX - 4096 || a->N >= INT_MAX - 4096) return VNX_ERR_UNSUPPORTED;
+  if (a->force_shape < 0 || a->force_shape > kQ8Shapes) return VNX_ERR_UNSUPPORTED;
+  p->M = (int)a->M; p->N = (int)a->N; p->K = (int)a->K; p->cols = (int)cols;
+  p->y_dtype = a->y_dtype; p->res_dtype = a->res_dtype;
+  return VNX_OK;
 }
 
 // Bytes from a on that rows `ld` apart take.
@@ -641,16 +758,18 @@ using namespace vnx;
 
 extern "C" {
 
-int vnx_q8_linear(const vnx_q8_linear_args* a, void* stream) {
-  if (!a || a->M < 0 || a->N < 0 || a->K < 1 || a->ldx < a->K || a->ldw < a->K) return VNX_ERR_INVALID_ARG;
-  if (a->epilogue != VNX_EPI_NONE && a->epilogue != VNX_EPI_SWIGLU) return VNX_ERR_INVALID_ARG;
+size_t vnx_q8_linear_workspace(const vnx_q8_linear_args* a) {
+  Q8LinParams p{};
+  if (q8_sizes(a, &p) != VNX_OK || a->M == 0 || a->N == 0) return 256;
+  const size_t n = (a->epilogue == VNX_EPI_SWIGLU ? q8_plan<true>(p, a->force_shape) : q8_plan<false>(p, a->force_shape)).bytes;
+  return n > 256 ? n : 256;
+}
+
+int vnx_q8_linear(const vnx_q8_linear_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+  Q8LinParams p{};
+  if (const int rc = q8_sizes(a, &p)) return rc;
   const bool sw = a->epilogue == VNX_EPI_SWIGLU;
-  const int64_t cols = sw ? a->N / 2 : a->N;
-  if ((sw && (a->N % 2 || a->res)) || a->ldy < cols || (a->res && a->ldr < cols)) return VNX_ERR_INVALID_ARG;
-  if (!q8_float(a->y_dtype) || (a->res && !q8_float(a->res_dtype))) return VNX_ERR_UNSUPPORTED;
-  // rows and columns are numbered to the end of their last tile in 32 bits
-  if (a->K > kQ8MaxK || a->M >= INT_MAX - 4096 || a->N >= INT_MAX - 4096) return VNX_ERR_UNSUPPORTED;
-  if (a->force_shape < 0 || a->force_shape > kQ8Shapes) return VNX_ERR_UNSUPPORTED;
+  const int64_t cols = p.cols;
   if (a->M == 0 || a->N == 0) return VNX_OK;
   if (!a->x || !a->x_scale || !a->w || !a->w_scale || !a->y) return VNX_ERR_INVALID_ARG;
   const int ey = elem_size(a->y_dtype), er = elem_size(a->res_dtype);
@@ -672,13 +791,11 @@ int vnx_q8_linear(const vnx_q8_linear_args* a, void* stream) {
     if (er != ey || a->ldr != a->ldy || a->res == a->y || Rows(cols, &a->ldy, {a->M}).meet(a->y, a->res, ey))
       return VNX_ERR_INVALID_ARG;
   }
-  Q8LinParams p{};
   p.x = a->x; p.w = a->w; p.xs = a->x_scale; p.ws = a->w_scale; p.bias = a->bias; p.res = a->res; p.y = a->y;
   p.ldx = a->ldx; p.ldw = a->ldw; p.ldr = a->ldr; p.ldy = a->ldy;
-  p.M = (int)a->M; p.N = (int)a->N; p.K = (int)a->K; p.cols = (int)cols;
-  p.res_dtype = a->res_dtype; p.y_dtype = a->y_dtype;
   const auto st = static_cast<hipStream_t>(stream);
-  return sw ? q8_linear<true>(p, a->force_shape, st) : q8_linear<false>(p, a->force_shape, st);
+  return sw ? q8_linear<true>(p, a->force_shape, workspace, workspace_bytes, st)
+            : q8_linear<false>(p, a->force_shape, workspace, workspace_bytes, st);
 }
 
 }  // extern "C"

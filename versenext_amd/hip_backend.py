@@ -1068,7 +1068,10 @@ class HipBackend(DeviceBackend):
             ldx, ldw, self._pitch(rt) if rt is not None else 0, self._pitch(y), M, N, K,
             _lib.DTYPE_CODES[rt.dtype] if rt is not None else _lib.VNX_F32, _lib.DTYPE_CODES[y.dtype],
             _lib.VNX_EPI_SWIGLU if swiglu else _lib.VNX_EPI_NONE, int(force_shape))
-        _lib.check(self._L.vnx_q8_linear(args, self._stream()), "linear_q8")
+        # a workspace of this call's own: a captured graph keeps it in its pool
+        need = self._L.vnx_q8_linear_workspace(args)
+        buf = torch.empty(need, dtype=torch.uint8, device=self._torch_device) if need > 256 else None
+        _lib.check(self._L.vnx_q8_linear(args, _ptr(buf), need if buf is not None else 0, self._stream()), "linear_q8")
         return out
 
     def attention(self, q, k, v, mask=None):
