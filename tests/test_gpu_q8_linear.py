@@ -4,6 +4,7 @@ import pytest
 import torch
 
 import q8_ref as R
+from versenext_amd import _lib
 
 pytestmark = pytest.mark.gpu
 
@@ -215,6 +216,61 @@ def test_captured_and_replayed(hip):
             assert all(torch.equal(p, q) for p, q in zip(out, w))
 
 
+def test_split_captured_and_replayed(hip):
+    """Two graphs of products whose k is split (each with partial sums of its own), replayed at once on two streams with
+    eager calls between, equal the eager result."""
+    dev = hip.torch_device
+    g = R.gen(21)
+    sets, graphs = [], []
+    for M, N, K, force, swiglu in ((200, 500, 16000, 0, False), (70, 260, 8192, 6, True)):
+        sets.append((R.codes(g, M, K).to(dev), R.scales(g, M).to(dev), R.codes(g, N, K).to(dev), R.scales(g, N).to(dev),
+                     None, None, swiglu, torch.float32, None, force))
+        p = _lib.pack_q8_linear(*[0] * 7, K, K, 0, N, M, N, K, 0, _lib.VNX_F32, _lib.VNX_EPI_SWIGLU if swiglu else _lib.VNX_EPI_NONE,
+                                force)
+        assert hip._L.vnx_q8_linear_workspace(p) > 256       # two launches
+    want = [hip.linear_q8(*a[:-1], force_shape=2) for a in sets]
+    streams = [torch.cuda.Stream(device=dev) for _ in sets]
+    for a, st in zip(sets, streams):
+        st.wait_stream(torch.cuda.current_stream(dev))
+        with torch.cuda.stream(st):
+            hip.linear_q8(*a)
+        torch.cuda.synchronize()
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr, stream=st):
+            out = hip.linear_q8(*a)
+        graphs.append((gr, out))
+    for k in range(4):
+        for a in sets:
+            a[1].uniform_(0.001, 0.1)
+        want = [hip.linear_q8(*a[:-1], force_shape=2) for a in sets]
+        for _, out in graphs:
+            out.fill_(7.0)
+        torch.cuda.synchronize()
+        for (gr, _), st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                gr.replay()
+        eager = [hip.linear_q8(*a) for a in sets]
+        torch.cuda.synchronize()
+        for (_, out), e, w in zip(graphs, eager, want):
+            assert torch.equal(out, w) and torch.equal(e, w)
+
+
+def test_one_row_of_a_wide_tensor(hip, monkeypatch):
+    """A single row has no pitch to refuse, however far its tensor's next one would be."""
+    dev = hip.torch_device
+    g = R.gen(3)
+    wide = torch.zeros(1, (1 << 22) + 64, dtype=torch.int8, device=dev)
+    c, w = R.codes(g, 1, 100).to(dev), R.codes(g, 5, 100).to(dev)
+    wide[:, :100] = c
+    cs, ws = R.scales(g, 1).to(dev), R.scales(g, 5).to(dev)
+    for bind in (_lib.bind(), _lib.NoBind):
+        monkeypatch.setattr(hip, "_bind", bind)
+        want = hip.linear_q8(c, cs, w, ws)
+        assert torch.equal(hip.linear_q8(wide[:, :100], cs, w, ws), want)
+        assert torch.equal(hip.linear_q8(w, ws, wide[:, :100], cs), hip.linear_q8(w, ws, c, cs))
+        assert torch.equal(hip.dequantize_rows(wide[:, :100], cs), hip.dequantize_rows(c, cs))
+
+
 def test_streams(hip):
     """Two streams at once give what one gives."""
     dev = hip.torch_device
@@ -234,7 +290,6 @@ def test_streams(hip):
 
 
 def test_binding_and_general_path_agree(hip, monkeypatch):
-    from versenext_amd import _lib
     dev = hip.torch_device
     g = R.gen(9)
     c, w = (R.pitched(R.codes(g, n, 100), 112, 9, dev) for n in (21, 34))

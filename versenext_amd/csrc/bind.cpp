@@ -321,7 +321,7 @@ decltype(&vnx_q8_linear) g_linear;
 // elements, 0 where it is not.
 int64_t pitch_of(const at::Tensor& t) {
   if (t.dim() != 2 || t.size(1) < 1 || (t.size(1) > 1 && t.stride(1) != 1)) return 0;
-  return t.size(0) <= 1 ? std::max(t.size(1), t.stride(0)) : t.stride(0) >= t.size(1) ? t.stride(0) : 0;
+  return t.size(0) <= 1 ? t.size(1) : t.stride(0) >= t.size(1) ? t.stride(0) : 0;
 }
 
 int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }

@@ -908,7 +908,7 @@ class HipBackend(DeviceBackend):
 
     @staticmethod
     def _pitch(t2: torch.Tensor) -> int:
-        return max(t2.shape[1], t2.stride(0))
+        return t2.stride(0) if t2.shape[0] > 1 else t2.shape[1]
 
     def _code_rows(self, x, what: str):
         """int8 rows as vnx_q8_linear reads them: on 16 bytes (padded where
