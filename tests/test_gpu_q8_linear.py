@@ -8,8 +8,8 @@ from versenext_amd import _lib
 
 pytestmark = pytest.mark.gpu
 
-SHAPES = range(0, 7)     # 0: the plan's choice
-TILES = [0, 1, 2, 3, 4, 6]      # those that take SwiGLU
+SHAPES = range(0, 8)     # 0: the plan's choice
+TILES = [0, 1, 2, 3, 4, 6, 7]      # those that take SwiGLU
 
 
 def check(hip, shape, M, N, K, out=torch.bfloat16, bias=False, residual=None, swiglu=False, low=-127, fill=77, seed=0):

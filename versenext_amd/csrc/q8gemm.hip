@@ -4,6 +4,7 @@
 //   y[m, n] = acc * x_scale[m] * w_scale[n] (+ bias[n]) (+ residual[m, n])
 // or, of gate rows and up rows, silu(gate) * up.  The sums are whole numbers, so
 // how K is split never changes a result.
+#include <algorithm>
 #include <climits>
 #include <utility>
 
@@ -306,10 +307,10 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void k_q8_tile(Q8LinParams p) {
   constexpr int NW = WM * WN, RT = BM / WM / 16, CT = BN / WN / 16;
   constexpr int SLAB = 64 * KS, PART = (BM + BN) * 64, STAGE = KS * PART, OC = SW ? BN / 2 : BN;
   constexpr int PW = (BM + BN) / 16 / NW, CW = PW * KS;  // a wave's copies of a part, and of a slab
-  static_assert((BM + BN) / 16 % NW == 0 && (NS - 1) * CW < 64 && NS % 2 == 0 && (!SW || CT % 2 == 0) && BM % 64 == 0 &&
-                    BN % 64 == 0, "");
+  static_assert((BM + BN) / 16 % NW == 0 && (NS - 1) * CW < 64 && NS % 2 == 0 && (!SW || CT % 2 == 0), "");
   __shared__ __attribute__((aligned(256))) char smem[NS * STAGE];
-  __shared__ __attribute__((aligned(256))) float scales[BM + 2 * BN];  // of x, of W, the bias
+  constexpr int SM = (BM + 63) / 64 * 64, SN = (BN + 63) / 64 * 64;
+  __shared__ __attribute__((aligned(256))) float scales[SM + 2 * SN];  // of x, of W, the bias
   // results: tiles of a row (CTO, ST in a strip), values in 16 bytes, lanes a row, pitch
   constexpr int CTO = SW ? CT / 2 : CT, VE = 16 / sizeof(TY), ST = CTO < 8 / (int)sizeof(TY) ? CTO : 8 / (int)sizeof(TY);
   constexpr int LR = ST * 16 / VE, SP = ST * 16 * (int)sizeof(TY) + 16;
@@ -420,19 +421,19 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void k_q8_tile(Q8LinParams p) {
 
   if constexpr (!SUMS) {
     // the scales, 64 a copy
-    for (int u = wave; u < (BM + (p.bias ? 2 : 1) * BN) / 64; u += NW) {
+    for (int u = wave; u < (SM + (p.bias ? 2 : 1) * SN) / 64; u += NW) {
       const int j = u * 64 + lane;
       const float* src;
-      if (u * 64 < BM) {
+      if (u * 64 < SM) {
         src = p.xs + m0 + min(j, p.M - 1 - m0);
       } else {
-        const int w = j < BM + BN ? j - BM : j - BM - BN, up = SW ? w / 16 & 1 : 0, row = SW ? w / 32 * 16 + w % 16 : w;
-        src = (j < BM + BN ? p.ws : p.bias) + (int64_t)up * p.cols + min(o0 + row, p.cols - 1);
+        const int w = j < SM + SN ? j - SM : j - SM - SN, up = SW ? w / 16 & 1 : 0, row = SW ? w / 32 * 16 + w % 16 : w;
+        src = (j < SM + SN ? p.ws : p.bias) + (int64_t)up * p.cols + min(o0 + row, p.cols - 1);
       }
       copy_to_lds(lds_addr(scales) + u * 256, src);
     }
     if (!p.bias)
-      for (int i = tid; i < BN; i += 64 * NW) scales[BM + BN + i] = 0.0f;
+      for (int i = tid; i < SN; i += 64 * NW) scales[SM + SN + i] = 0.0f;
   }
 #pragma unroll 1
   for (int c = 0; c < NS; ++c)                       // (of fewer slabs: the first again, not read)
@@ -486,7 +487,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void k_q8_tile(Q8LinParams p) {
   auto leave = [&](auto edge) {
     constexpr bool EDGE = decltype(edge)::value;
     constexpr bool LATE = RES && sizeof(TY) == 4;  // the residual is added behind LDS, which holds fp32
-    const float* sw = scales + BM + wn * CT * 16 + 4 * g4;  // of this lane's W rows (read again and again: registers are few)
+    const float* sw = scales + SM + wn * CT * 16 + 4 * g4;  // of this lane's W rows (read again and again: registers are few)
     const int n0 = o0 + wn * CTO * 16;
     char* mine = smem + wave * 16 * SP;
     const int lr = lane / LR, lc = lane % LR * VE; // row and first column of this lane's 16 bytes
@@ -501,7 +502,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void k_q8_tile(Q8LinParams p) {
           const int t = (q + u) * (SW ? 2 : 1);
           float v[4];
           auto val = [&](int at, float (&d)[4]) {
-            const f32x4 w = *reinterpret_cast<const f32x4*>(sw + at * 16), c = *reinterpret_cast<const f32x4*>(sw + BN + at * 16);
+            const f32x4 w = *reinterpret_cast<const f32x4*>(sw + at * 16), c = *reinterpret_cast<const f32x4*>(sw + SN + at * 16);
 #pragma unroll
             for (int e = 0; e < 4; ++e) d[e] = fmaf((float)acc[i][at][e] * sx, w[e], c[e]);
           };
@@ -594,21 +595,27 @@ int q8_tile(Q8LinParams p, hipStream_t st) {
 }
 
 // ---------------------------------------------------------------------------
-// Launch shapes, and the choice between them by an estimate of their time: n =
-// workgroups a CU, each of them `slab` us per 64 bytes of k (`alone` where less
-// than half of the CUs has one) and `rest` us besides.  Fitted to 60 sizes; us by
-// the estimate / measured (M x N x K; the shape taken first, then the others in
-// the order below):
-//   2,048 x 2,048 x 1,024    128^2 7.7 / 8.8; 256^2 16 / 16, 64 x 128 9.9 / 9.9, 64^2 12 / 11
-//   2,048 x 1,024 x 2,752    64 x 128 12 / 12.5; 256^2 34 / 33, 128^2 14 / 17, 64^2 15 / 14
-//   224 x 1,024 x 2,752      64^2 7.0 / 6.9; 128^2 14 / 14, 64 x 128 9.9 / 10, direct 11 / 8.6
-//   64 x 1,024 x 4,096       direct 5.5 / 5.7; 64^2 9.3 / 8.5
-//   1 x 248,320 x 1,024      direct 40 / 40; 64 x 128 29 / 47, which HBM holds up (51 in the estimate)
+// Launch shapes, and the choice between them by an estimate of their time: `once`
+// us a launch and, n the workgroups a CU, n times `slab` us per 64 bytes of k
+// (`alone` where less than half of the CUs has one; k to whole pairs of slabs, four
+// slabs at least) and `rest` us.  Fitted to 168 sizes (1 to 8,192 rows): the shape
+// taken is 1.1% slower than the fastest on average, 16% at most.  us by the estimate
+// / measured (M x N x K; the shape taken first):
+//   2,048 x 2,048 x 1,024    128^2 8.3 / 8.7; 64 x 128 9.5 / 9.8, 64^2 10.3 / 10.6, 256^2 15.4 / 16.2
+//   2,048 x 1,024 x 2,752    64 x 128 11.7 / 12.5; 64^2 13.1 / 14.2, 128^2 14.2 / 17.3
+//   400 x 2,048 x 2,048      64^2 6.1 / 6.0; 64 x 128 8.4 / 8.4, 32^2 9.2 / 8.7
+//   224 x 1,024 x 4,096      32^2 5.6 / 5.8; 64^2 9.2 / 9.6, direct 14.6 / 16.5
+//   32 x 4,096 x 1,024       32^2 2.9 / 2.8; direct 3.8 / 3.8, 64^2 3.9 / 3.9
+//   1 x 1,024 x 4,096        direct 4.6 / 4.1; 32^2 5.5 / 5.1
 // ---------------------------------------------------------------------------
-constexpr int kQ8Direct = 4, kQ8Split = 5, kQ8Shapes = 6;
-struct Q8Shape { int bm, bn; double slab, alone, rest; };
-constexpr Q8Shape kQ8Tiles[4] = {
-    {256, 256, 0.85, 0.68, 3.0}, {128, 128, 0.32, 0.27, 0.6}, {64, 128, 0.23, 0.17, 0.4}, {64, 64, 0.14, 0.11, 0.25}};
+constexpr int kQ8Direct = 4, kQ8Split = 5, kQ8Shapes = 7;
+struct Q8Shape { int shape, bm, bn, ks; double slab, alone, rest, once; };
+constexpr Q8Shape kQ8Tiles[5] = {{0, 256, 256, 1, 0.795, 0.562, 4.96, 1.49},
+                                 {1, 128, 128, 1, 0.295, 0.243, 1.04, 2.52},
+                                 {2, 64, 128, 1, 0.207, 0.183, 0.317, 2.2},
+                                 {3, 64, 64, 2, 0.124, 0.111, 0.071, 2.08},
+                                 {6, 32, 32, 4, 0.055, 0.053, 0.045, 2.02}};
+constexpr Q8Shape kQ8Pairs = {6, 32, 32, 4, 0.066, 0.091, 0, 2.31};  // of SwiGLU: two waves
 
 // A split's sums joined: thread i has eight columns of a row.
 template <bool SW>
@@ -663,34 +670,34 @@ Q8Plan q8_split(const Q8LinParams& p, int want) {
 template <bool SW>
 Q8Plan q8_plan(const Q8LinParams& p, int force) {
   const int64_t cus = device_cus();
-  const double slabs = (p.K + 63) / 64;
   const double hbm = ((double)p.M * p.K + (double)p.N * p.K + (double)p.M * p.cols * elem_size(p.y_dtype)) / 5e6;
   Q8Plan best{0, 0, 0, 0};
   double least = 1e300;
-  for (int i = 0; i < 4; ++i) {
-    const Q8Shape& s = kQ8Tiles[i];
-    const int oc = SW ? s.bn / 2 : s.bn;
-    const int64_t tiles = (int64_t)((p.M + s.bm - 1) / s.bm) * ((p.cols + oc - 1) / oc);
-    const double t = (double)((tiles + cus - 1) / cus) * (slabs * (2 * tiles <= cus ? s.alone : s.slab) + s.rest);
+  auto take = [&](double t, int shape) {
     const double us = t > hbm ? t : hbm + 0.01 * t;
-    if (us < least) least = us, best.shape = i;
+    if (us < least) least = us, best.shape = shape;
+  };
+  for (int i = 0; i < 5; ++i) {
+    const Q8Shape& s = SW && i == 4 ? kQ8Pairs : kQ8Tiles[i];
+    const int oc = SW ? s.bn / 2 : s.bn, slabs = 2 * s.ks * std::max(2, (p.K + 128 * s.ks - 1) / (128 * s.ks));
+    const int64_t tiles = (int64_t)((p.M + s.bm - 1) / s.bm) * ((p.cols + oc - 1) / oc);
+    take(s.once + (double)((tiles + cus - 1) / cus) * (slabs * (2 * tiles <= cus ? s.alone : s.slab) + s.rest), s.shape);
   }
   if (!SW) {
     // 16 x 16 of y a workgroup; rows of x that are one and the same line cost less
     const int64_t wgs = (int64_t)((p.M + 15) / 16) * ((p.N + 15) / 16);
-    const double us = (double)(wgs > cus ? wgs : cus) / cus * slabs * (p.M <= 4 ? 0.039 : 0.055);
-    if (us < least) least = us, best.shape = kQ8Direct;
+    take(1.98 + (double)(wgs > cus ? wgs : cus) / cus * ((p.K + 63) / 64) * (p.M <= 4 ? 0.0403 : 0.0557), kQ8Direct);
   }
   // Few tiles and a long k: a CU's 70 GB/s of copies to LDS bounds a tile, so k is
-  // shared by more of them, at the price of a second launch.  64 x 4,096 x 10,944
-  // 21.7 -> 13.1 us, 512 x 1,024 x 8,192 17.1 -> 13.8; 224 x 1,024 x 2,752 would
-  // take 7.8 (6.9 as it is).
+  // shared by more of them, at the price of a second launch.  32 x 256 x 16,384 14.8
+  // -> 9.6 us, 16 x 1,024 x 11,008 11.6 -> 8.7; 224 x 1,024 x 4,096 would take 9.0
+  // (5.8 as it is).
   const int64_t tiles = (int64_t)((p.M + 63) / 64) * ((p.N + 63) / 64);
   if (force == kQ8Split + 1) least = 1e300;
   for (int want = 2; want <= 32 && (want == 2 || tiles * want <= 2 * cus); want *= 2) {
     const Q8Plan s = q8_split(p, want);
     const int64_t wgs = tiles * s.splits;
-    const double us = 3.5 + (double)((wgs + cus - 1) / cus) * (s.per * 2 * (2 * wgs <= cus ? 0.11 : 0.14) + 0.25) +
+    const double us = 4.4 + (double)((wgs + cus - 1) / cus) * (s.per * 2 * (2 * wgs <= cus ? 0.091 : 0.131) + 1.13) +
                       (double)s.bytes / 3e6;
     if (us < 0.95 * least && s.bytes < (size_t)1 << 30) least = us, best = s;
   }
@@ -706,6 +713,7 @@ int q8_linear(const Q8LinParams& p, int force, void* workspace, size_t workspace
     case 1: return q8_tile<SW, 128, 128, 2, 2, 1, 4, 2>(p, st);
     case 2: return q8_tile<SW, 64, 128, 2, 2, 1, 4, 3>(p, st);
     case 3: return q8_tile<SW, 64, 64, 2, 2, 2, 4, 2>(p, st);
+    case 6: return q8_tile<SW, 32, 32, 2, SW ? 1 : 2, 4, 4, 2>(p, st);
     case kQ8Direct:
       if constexpr (!SW) return q8_direct<4>(p, st);
       return VNX_ERR_UNSUPPORTED;
