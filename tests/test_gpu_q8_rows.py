@@ -8,8 +8,8 @@ import q8_ref as R
 pytestmark = pytest.mark.gpu
 
 # every launch shape and its border, rows that 8 does not divide, fewer than 8 values, more than a workgroup holds
-WIDTHS = [1, 3, 7, 8, 9, 64, 511, 512, 513, 1000, 1024, 1025, 2047, 2048, 2056, 4096, 4101, 8192, 8200, 32768, 32777,
-          70001]
+WIDTHS = [1, 3, 7, 8, 9, 64, 511, 512, 513, 1000, 1024, 1025, 2047, 2048, 2056, 4096, 4101, 8192, 8200, 12288, 12289,
+          16384, 16385, 32768, 32777, 70001]
 
 
 def rows(seed, M, K, dtype):
@@ -18,9 +18,10 @@ def rows(seed, M, K, dtype):
 
 
 def scale_steps(K):
-    """Roundings of a norm's scale: the sum of squares (at most 48 in a row's threads and their tree, K / 256 + 16 where a
-    thread walks the row), halved by the root; the mean, eps, the root, a / 127 and the quotient."""
-    return (48 if 8 <= K <= 32768 else K / 256 + 16) / 2 + 6
+    """Roundings of a norm's scale: the sum of squares (at most 33 in a thread of 32 values, 6 in a wave, 15 over sixteen
+    waves: 54; K / 256 + 16 where a thread walks the row), halved by the root; the mean, eps, the root, a / 127 and the
+    quotient."""
+    return (54 if 8 <= K <= 32768 else K / 256 + 16) / 2 + 6
 
 
 @pytest.mark.parametrize("K", WIDTHS)

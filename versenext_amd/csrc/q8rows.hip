@@ -13,6 +13,11 @@
 // load to the store.  The last vector of a row that 8 does not divide starts at
 // K - 8 and so repeats values of the one before it: they are left out of the
 // sum, and stored twice alike.
+//
+// HBM bounds it, or a few rows the launch.  us and TB/s of bytes in and out, from
+// a graph: quantize 4,096 x 8,200 fp32 28.7 (5.8), 4,096 x 10,944 bf16 22.6 (6.0),
+// 1 x 10,944 2.2; norm with a bf16 residual 4,096 x 10,944 bf16 47.7 (6.6; partly
+// the last-level cache's), 2,048 x 4,096 fp32 15.5 (5.9).  A large copy: 5.1 TB/s.
 #include <climits>
 
 #include "q8.h"
@@ -194,7 +199,9 @@ __global__ __launch_bounds__(256) void k_q8_rows_any(Q8RowParams p) {
 template <typename TX, typename TR, bool NORM>
 int q8_rows(const Q8RowParams& p, hipStream_t st) {
   // A wave a row up to 2,048 values (no barrier, and a token's row is short),
-  // then a workgroup of 4 or of 16 waves.
+  // then a workgroup of 4 to 16 waves, with no more values a thread than it needs:
+  // registers and idle lanes are bytes not in flight (4,096 rows of 8,200 fp32
+  // by 16 waves of 32 values: quantize 36.2 us, norm 107; by 8 of 24, 28.7 and 70.3).
   auto go = [&](auto tc, auto nc) -> int {
     constexpr int T = decltype(tc)::value, NV = decltype(nc)::value, NT = T < 256 ? 256 : T;
     const int64_t wgs = (p.M + NT / T - 1) / (NT / T);
@@ -209,6 +216,8 @@ int q8_rows(const Q8RowParams& p, hipStream_t st) {
     if (p.K <= 2048) return go(IntC<64>{}, IntC<4>{});
     if (p.K <= 4096) return go(IntC<256>{}, IntC<2>{});
     if (p.K <= 8192) return go(IntC<256>{}, IntC<4>{});
+    if (p.K <= 12288) return go(IntC<512>{}, IntC<3>{});
+    if (p.K <= 16384) return go(IntC<1024>{}, IntC<2>{});
     if (p.K <= 32768) return go(IntC<1024>{}, IntC<4>{});
   }
   if (!launch_fits(p.M, 256)) return VNX_ERR_UNSUPPORTED;
