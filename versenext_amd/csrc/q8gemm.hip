@@ -14,7 +14,6 @@ namespace vnx {
 namespace {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
-typedef int i32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kQ8Chunk = 128;   // bytes of k a chunk: a cache line of a row
 constexpr int kQ8Xcds = 8;
@@ -107,6 +106,11 @@ __device__ __forceinline__ i32x4 q8_mma(u32x4 a, u32x4 b, i32x4 c) {
 // is free as long as both operands have the same, so a lane loads two 16-byte
 // pieces side by side of its row (lane (r, g): row r, bytes 32 g .. + 32), whole
 // lines over the wave.
+//
+// Memory's latency bounds it, then the copies of x and W that every workgroup reads
+// for itself.  us, from a graph (32 x 32 tiles): 1 x 2,048 x 1,024 2.5 (2.7), 1 x
+// 1,024 x 4,096 4.1 (5.1), 64 x 1,024 x 2,752 4.0 (5.2), 32 x 4,096 x 1,024 3.8
+// (2.8).  Eight or sixteen waves, or loads of the next chunks ahead, took longer.
 // ---------------------------------------------------------------------------
 template <int KW>
 __global__ __launch_bounds__(64 * KW) void k_q8_direct(Q8LinParams p) {
@@ -220,6 +224,21 @@ int q8_direct(Q8LinParams p, hipStream_t st) {
 //
 // W is the products' first operand: lane (r, g) then holds four columns of y of
 // row r.
+//
+// What bounds it, by shape:
+//   256 x 256, eight waves   the chip's power: 8,192^3 takes 442-458 us (2,400-2,490
+//                            TOP/s) at about 1.55 GHz with the matrix cores busy two
+//                            thirds of the time, 326 with codes of zero; copies gone
+//                            348, LDS reads gone 381, stores gone 408.  Products of
+//                            32 x 32 x 32: 474; four waves of 128 x 128: 566.
+//   128^2, 64 x 128, 64^2    copies into a CU's LDS, about 70 GB/s of them, and the
+//                            last round of workgroups.
+//   32 x 32                  the chain of a slab: wait, barrier, LDS read, product (0.2
+//                            us per 256 bytes of k, 0.13 per 128, so slabs are long;
+//                            of 512 they gain 6% at a k of 4,096 and lose half at
+//                            1,024; eight buffers instead of four gain nothing).
+// One workgroup a CU that fetches its next tile's slabs during the results: 1-6%
+// slower at every size.
 //
 // TY int: the sums alone, of the p.per slabs of k that are blockIdx.y's, into the
 // 32-bit matrix [split][row][column] of whole tiles at p.y.
