@@ -284,16 +284,15 @@ enum { Q8_CHAIN = 0, Q8_TREE = 1, Q8_ALL = 2 };
 template <int CT>
 struct Q8Mask {
   int node[CT];
+  uint64_t word[CT];  // a tree's: the columns' ancestors
   int tp, window, rows, full_lo, full_hi;
-  const uint64_t* words;
 };
 
 // Bit e set: key k0 + 16 (e / 4) + g4 + e % 4 is hidden from the column.
 template <int KIND>
-__device__ __forceinline__ uint32_t q8_hidden(int tp, int window, int rows, const uint64_t* words, int node, int k0,
+__device__ __forceinline__ uint32_t q8_hidden(int tp, int window, int rows, uint64_t w, int node, int k0,
                                               int g4) {
   int lo, hi;
-  uint64_t w = 0;
   if constexpr (KIND == Q8_ALL) {
     lo = 0;
     hi = rows;
@@ -301,7 +300,6 @@ __device__ __forceinline__ uint32_t q8_hidden(int tp, int window, int rows, cons
     lo = tp + node - window + 1;
     hi = tp + node + 1;
   } else {
-    w = words[node];
     lo = tp + __popcll(w) - window;
     hi = rows;
   }
@@ -464,7 +462,7 @@ __device__ __forceinline__ bool q8_steps(const Q8Src& src, int first, int s0, in
       }
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) {
-        const uint32_t hide = q8_hidden<KIND>(mk.tp, mk.window, mk.rows, mk.words, mk.node[ct], k0, g4);
+        const uint32_t hide = q8_hidden<KIND>(mk.tp, mk.window, mk.rows, mk.word[ct], mk.node[ct], k0, g4);
 #pragma unroll
         for (int e = 0; e < 8; ++e)
           x[ct][e] = hide >> e & 1 ? kNegInf : bad >> e & 1 ? __builtin_nanf("") : x[ct][e];
@@ -568,7 +566,7 @@ struct Q8Tile {
   int first, steps;   // steps of 32 keys from key first on
   Q8Src src2;
 
-  // E: bytes of the cache's elements
+  template <int KIND>
   __device__ __forceinline__ void init(const Q8Params& p, const Q8Words& tw, int bh, int c0, int lane) {
     const int m = lane & 15, g = lane >> 4;
     b = bh / p.Hkv;
@@ -581,7 +579,6 @@ struct Q8Tile {
     mask.tp = tp;
     mask.rows = rows;
     mask.window = W;
-    mask.words = p.tree == 2 ? p.anc + b * p.anc_sb : tw.w;
     int lo_min, hi_max;
     if (p.tree) {
       lo_min = p.window > 0 ? max(0, tp - 1 - W + 1) : 0;             // an empty word sits at tp - 1
@@ -606,6 +603,22 @@ struct Q8Tile {
       for (int i = 0; i < D / 32; ++i)
         qf[ct][i] = *reinterpret_cast<const bf16x8*>(q + D / 4 * g + 8 * i);
       mask.node[ct] = node;
+      mask.word[ct] = 0;
+      if constexpr (KIND == Q8_TREE) {
+        // Words among the arguments are read by the scalar unit, one node after the
+        // other: a lane's own load from the arguments' memory has returned wrong
+        // words for single lanes (in 18-22 of 40 calls of 2 x 40 nodes over 300 rows
+        // in 32 splits; in none where the same code read them from device memory).
+        if (p.tree == 2) {
+          mask.word[ct] = p.anc[b * p.anc_sb + node];
+        } else {
+          const int last = uni(min(c0 + 16 * ct + 15, p.cols - 1) / p.rep);
+          for (int i = uni(min(c0 + 16 * ct, p.cols - 1) / p.rep); i <= last; ++i) {
+            const uint64_t w = tw.w[i];
+            if (node == i) mask.word[ct] = w;
+          }
+        }
+      }
     }
     const int64_t kv = b * p.c_sb + kvh * p.c_sh, ss = b * p.s_sb + kvh * p.s_sh;
     src.k = p.kc + kv;
@@ -625,10 +638,9 @@ struct Q8Tile {
   __device__ __forceinline__ Q8Mask<CT> mask2(int T2) const {
     Q8Mask<CT> k;
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) k.node[ct] = 0;
+    for (int ct = 0; ct < CT; ++ct) k.node[ct] = 0, k.word[ct] = 0;
     k.tp = k.window = k.full_lo = 0;
     k.rows = k.full_hi = T2;
-    k.words = nullptr;
     return k;
   }
 };
@@ -691,7 +703,7 @@ __global__ __launch_bounds__((KW * CW + (SEG2 && KW >= 4)) * 64,
   const int bh = blockIdx.x % BH, rest = blockIdx.x / BH;
   const int grp = p.groups - 1 - rest % p.groups, split = rest / p.groups;
   Q8Tile<D, CT> t;
-  t.init(p, tw, bh, min((grp * CW + cw) * COLS, (p.cols - 1) / COLS * COLS), lane);  // (a tile past the last: the last again)
+  t.template init<KIND>(p, tw, bh, min((grp * CW + cw) * COLS, (p.cols - 1) / COLS * COLS), lane);  // (a tile past the last: the last again)
   Q8State<CT, D> st;
   // where this thread stands in the merge
   const int mc = threadIdx.x / TPC, dd = threadIdx.x % TPC * DP;   // column (of 16 CW), first dim
