@@ -1015,7 +1015,8 @@ int vnx_tree_attn_q8(const vnx_attn_q8_args* args, void* workspace, size_t works
  * range has scale NaN.
  *
  * vnx_q8_dequantize: out (M, K) in out_dtype = code * scale.
- * No output may share bytes with an input but as said (VNX_ERR_INVALID_ARG).
+ * No output may share bytes with an input, or with another output, but as said
+ * (VNX_ERR_INVALID_ARG).
  * ------------------------------------------------------------------------- */
 int vnx_q8_quantize(const void* x, int dtype, int64_t ldx, int64_t M, int64_t K, int8_t* codes, int64_t ldc,
                     float* scale, void* stream);

@@ -274,6 +274,14 @@ bool spoils(const void* out, int64_t ldo, int eo, const void* in, int64_t ldi, i
   return Rows(K, &ldo, {M}).meet(out, in, eo);
 }
 
+// Whether one of M rows of K elements from p on shares a byte with the n bytes at s.
+bool rows_meet(const void* p, int64_t ld, int e, int64_t M, int64_t K, const void* s, __int128 n) {
+  const __int128 at = (__int128)reinterpret_cast<uintptr_t>(s) - (__int128)reinterpret_cast<uintptr_t>(p);
+  const __int128 row = (__int128)K * e, pitch = (__int128)ld * e;
+  const __int128 m = at < row ? 0 : (at - row) / pitch + 1;  // the first row that ends behind s
+  return m < M && m * pitch < at + n;
+}
+
 }  // namespace
 }  // namespace vnx
 
@@ -288,7 +296,10 @@ int vnx_q8_quantize(const void* x, int dtype, int64_t ldx, int64_t M, int64_t K,
   if (M == 0) return VNX_OK;
   const int e = elem_size(dtype);
   if (!x || !codes || !scale || !aligned_to(x, e) || !aligned_to(scale, 4)) return VNX_ERR_INVALID_ARG;
-  if (spans_meet(codes, ldc, 1, x, ldx, e, M, K)) return VNX_ERR_INVALID_ARG;
+  const __int128 ns = (__int128)M * 4;
+  if (spans_meet(codes, ldc, 1, x, ldx, e, M, K) || rows_meet(x, ldx, e, M, K, scale, ns) ||
+      rows_meet(codes, ldc, 1, M, K, scale, ns))
+    return VNX_ERR_INVALID_ARG;
   Q8RowParams p{};
   p.x = x; p.ldx = ldx; p.codes = codes; p.ldc = ldc; p.scale = scale; p.M = M; p.K = (int)K;
   return q8_by_type(dtype, [&](auto tx) {
@@ -311,6 +322,13 @@ int vnx_q8_rmsnorm(const void* x, int dtype, int64_t ldx, const void* res, int r
       (sum && (spans_meet(codes, ldc, 1, sum, lds, e, M, K) || spoils(sum, lds, e, x, ldx, e, M, K) ||
                (res && spoils(sum, lds, e, res, ldr, er, M, K)))))
     return VNX_ERR_INVALID_ARG;
+  // the weight is read by every row's workgroup, whichever others have ended
+  const __int128 ns = (__int128)M * 4, nw = (__int128)K * 4;
+  if (rows_meet(codes, ldc, 1, M, K, w, nw) || (sum && rows_meet(sum, lds, e, M, K, w, nw)) ||
+      rows_meet(w, K, 4, 1, K, scale, ns) || rows_meet(x, ldx, e, M, K, scale, ns) ||
+      (res && rows_meet(res, ldr, er, M, K, scale, ns)) || (sum && rows_meet(sum, lds, e, M, K, scale, ns)) ||
+      rows_meet(codes, ldc, 1, M, K, scale, ns))
+    return VNX_ERR_INVALID_ARG;
   Q8RowParams p{};
   p.x = x; p.ldx = ldx; p.res = res; p.ldr = ldr; p.w = w; p.eps = eps; p.sum = sum; p.lds = lds;
   p.codes = codes; p.ldc = ldc; p.scale = scale; p.M = M; p.K = (int)K;
@@ -329,7 +347,8 @@ int vnx_q8_dequantize(const int8_t* codes, int64_t ldc, const float* scale, int6
   if (M == 0) return VNX_OK;
   const int e = elem_size(out_dtype);
   if (!codes || !scale || !out || !aligned_to(out, e) || !aligned_to(scale, 4)) return VNX_ERR_INVALID_ARG;
-  if (spans_meet(codes, ldc, 1, out, ldo, e, M, K)) return VNX_ERR_INVALID_ARG;
+  if (spans_meet(codes, ldc, 1, out, ldo, e, M, K) || rows_meet(out, ldo, e, M, K, scale, (__int128)M * 4))
+    return VNX_ERR_INVALID_ARG;
   Q8ValParams p{codes, scale, out, ldc, ldo, M, (int)K, 1};
   auto go = [&](auto to, auto lc) -> int {
     constexpr int L = decltype(lc)::value;
