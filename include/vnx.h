@@ -1012,7 +1012,8 @@ int vnx_tree_attn_q8(const vnx_attn_q8_args* args, void* workspace, size_t works
  *   scale = RN(a / 127) / sqrt(mean(s^2) + eps),  a = max|t|:
  * RMSNorm (packages/verse_torch/verse_torch/vnnn.py:593-615) of the residual
  * stream, its factor in the scale alone.  A row whose squares sum past fp32's
- * range has scale NaN.
+ * range has scale NaN; squares below it are summed of scaled values, so a small
+ * row's norm is as exact as another's (eps may be 0).
  *
  * vnx_q8_dequantize: out (M, K) in out_dtype = code * scale.
  * No output may share bytes with an input, or with another output, but as said

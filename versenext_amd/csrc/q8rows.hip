@@ -26,6 +26,7 @@ namespace vnx {
 namespace {
 
 constexpr float kQ8Tiny = 7.8886090522101181e-31f;  // 2^-100: 127 / a stays finite above it
+constexpr float kQ8Up = 0x1p100f;
 
 struct Q8RowParams {
   const void* x;
@@ -40,9 +41,10 @@ struct Q8RowParams {
 };
 
 // The row's scale and the factor of its codes (0: codes of 0) from the bits of
-// max|t| (NaN above infinity above every number) and, of a norm, the sum of s^2.
+// max|t| (NaN above infinity above every number) and, of a norm, the sum of s^2
+// (tiny: of (2^100 s)^2).
 template <bool NORM>
-__device__ __forceinline__ float q8_scale(uint32_t am, float ss, const Q8RowParams& p, float* r) {
+__device__ __forceinline__ float q8_scale(uint32_t am, float ss, bool tiny, const Q8RowParams& p, float* r) {
   const float a = __uint_as_float(am);
   *r = 0.0f;
   if (am >= 0x7F800000u) return __uint_as_float(0x7FC00000u);
@@ -52,7 +54,21 @@ __device__ __forceinline__ float q8_scale(uint32_t am, float ss, const Q8RowPara
   if constexpr (!NORM) return s;
   // a sum of squares past fp32's range: no scale rather than one of 0
   if (!(ss < __builtin_inff())) return __uint_as_float(0x7FC00000u);
+  if (tiny) {
+    const float root = sqrtf(ss / (float)p.K + p.eps * kQ8Up * kQ8Up);
+    return s < 1.0f ? s * kQ8Up / root : s / root * kQ8Up;  // (s may be far from the rows' size: weights)
+  }
   return s / sqrtf(ss / (float)p.K + p.eps);
+}
+
+// Whether a row's mean square and eps lie where fp32 loses the squares' bits, or
+// the squares: they are then summed again, of values 2^100 as large (exact; below
+// 2^-110 times K the new sum stays below 2^121).  Above, a square's rounding to a
+// multiple of 2^-149 is 2^-40 of the mean.  The same in all threads of a row.
+// Kernels of their own (EPS0) for an eps below 2^-110, the only ones that can
+// meet such a row: the branch costs registers (4,096 x 16,000 bf16 85 -> 93 us).
+__device__ __forceinline__ bool q8_tiny(float am, float ss, const Q8RowParams& p) {
+  return am >= kQ8Tiny && ss / (float)p.K + p.eps < 0x1p-110f;
 }
 
 // Eight codes of v * r, |v * r| <= 127: adding 1.5 * 2^23 rounds to a whole
@@ -74,7 +90,7 @@ __device__ __forceinline__ float max_bits(float a, float b) {
 
 // T threads a row (a wave, or a workgroup), NV vectors of 8 values a thread:
 // 8 <= K <= 8 T NV.  TR void: no residual.
-template <typename TX, typename TR, bool NORM, int T, int NV>
+template <typename TX, typename TR, bool NORM, bool EPS0, int T, int NV>
 __global__ __launch_bounds__(T < 256 ? 256 : T) void k_q8_rows(Q8RowParams p) {
   constexpr int RPW = T < 256 ? 256 / T : 1;
   constexpr bool RES = !__is_void(TR);
@@ -118,8 +134,8 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void k_q8_rows(Q8RowParams p) {
   }
   am = wave_reduce(am, max_bits);
   if constexpr (NORM) ss = wave_reduce(ss, [](float a, float b) { return a + b; });
+  __shared__ float la[T / 64], ls[T / 64];
   if constexpr (T > 64) {
-    __shared__ float la[T / 64], ls[T / 64];
     if ((t & 63) == 0) {
       la[t >> 6] = am;
       ls[t >> 6] = ss;
@@ -132,10 +148,33 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void k_q8_rows(Q8RowParams p) {
       ss += ls[i];
     }
   }
+  bool tiny = false;
+  if constexpr (EPS0) {
+    tiny = q8_tiny(am, ss, p);
+    if (tiny) {
+      ss = 0.0f;
+#pragma unroll 1
+      for (int i = t; i < p.K; i += T) {
+        float u = q8_ld1(x + i);
+        if constexpr (RES) u = q8_round<TX>(u + q8_ld1(static_cast<const TR*>(p.res) + row * p.ldr + i));
+        u *= kQ8Up;
+        ss += u * u;
+      }
+      ss = wave_reduce(ss, [](float a, float b) { return a + b; });
+      if constexpr (T > 64) {
+        __syncthreads();
+        if ((t & 63) == 0) ls[t >> 6] = ss;
+        __syncthreads();
+        ss = ls[0];
+#pragma unroll
+        for (int i = 1; i < T / 64; ++i) ss += ls[i];
+      }
+    }
+  }
   // (stores from here on: every load of the row is done, so the sum may be
   // written over x or the residual)
   float r;
-  const float sc = q8_scale<NORM>(__float_as_uint(am), ss, p, &r);
+  const float sc = q8_scale<NORM>(__float_as_uint(am), ss, tiny, p, &r);
   if (t == 0) p.scale[row] = sc;
   int8_t* codes = p.codes + row * p.ldc;
   TX* sum = static_cast<TX*>(p.sum) + row * p.lds;
@@ -151,7 +190,7 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void k_q8_rows(Q8RowParams p) {
 
 // Rows of any length (fewer than 8 values, or more than a workgroup holds): one
 // workgroup a row, which reads it twice.
-template <typename TX, typename TR, bool NORM>
+template <typename TX, typename TR, bool NORM, bool EPS0>
 __global__ __launch_bounds__(256) void k_q8_rows_any(Q8RowParams p) {
   constexpr bool RES = !__is_void(TR);
   const int t = threadIdx.x;
@@ -186,8 +225,24 @@ __global__ __launch_bounds__(256) void k_q8_rows_any(Q8RowParams p) {
   __syncthreads();
   am = max_bits(max_bits(la[0], la[1]), max_bits(la[2], la[3]));
   ss = ls[0] + ls[1] + ls[2] + ls[3];
+  bool tiny = false;
+  if constexpr (EPS0) {
+    tiny = q8_tiny(am, ss, p);
+    if (tiny) {
+      ss = 0.0f;
+      for (int64_t i = t; i < p.K; i += 256) {
+        const float u = (sum ? q8_ld1(sum + i) : at((int)i)) * kQ8Up;  // (the sum: this thread's own store)
+        ss += u * u;
+      }
+      ss = wave_reduce(ss, [](float a, float b) { return a + b; });
+      __syncthreads();
+      if ((t & 63) == 0) ls[t >> 6] = ss;
+      __syncthreads();
+      ss = ls[0] + ls[1] + ls[2] + ls[3];
+    }
+  }
   float r;
-  const float sc = q8_scale<NORM>(__float_as_uint(am), ss, p, &r);
+  const float sc = q8_scale<NORM>(__float_as_uint(am), ss, tiny, p, &r);
   if (t == 0) p.scale[row] = sc;
   for (int64_t i = t; i < p.K; i += 256) {
     float u = NORM && sum ? q8_ld1(sum + i) : at((int)i);
@@ -196,8 +251,10 @@ __global__ __launch_bounds__(256) void k_q8_rows_any(Q8RowParams p) {
   }
 }
 
-template <typename TX, typename TR, bool NORM>
+template <typename TX, typename TR, bool NORM, bool EPS0 = false>
 int q8_rows(const Q8RowParams& p, hipStream_t st) {
+  if constexpr (NORM && !EPS0)
+    if (p.eps < 0x1p-110f) return q8_rows<TX, TR, true, true>(p, st);
   // A wave a row up to 2,048 values (no barrier, and a token's row is short),
   // then a workgroup of 4 to 16 waves, with no more values a thread than it needs:
   // registers and idle lanes are bytes not in flight (4,096 rows of 8,200 fp32
@@ -206,7 +263,7 @@ int q8_rows(const Q8RowParams& p, hipStream_t st) {
     constexpr int T = decltype(tc)::value, NV = decltype(nc)::value, NT = T < 256 ? 256 : T;
     const int64_t wgs = (p.M + NT / T - 1) / (NT / T);
     if (!launch_fits(wgs, NT)) return VNX_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL((k_q8_rows<TX, TR, NORM, T, NV>), dim3((unsigned)wgs), dim3(NT), 0, st, p);
+    hipLaunchKernelGGL((k_q8_rows<TX, TR, NORM, EPS0, T, NV>), dim3((unsigned)wgs), dim3(NT), 0, st, p);
     VNX_LAUNCH_CHECK();
     return VNX_OK;
   };
@@ -221,7 +278,7 @@ int q8_rows(const Q8RowParams& p, hipStream_t st) {
     if (p.K <= 32768) return go(IntC<1024>{}, IntC<4>{});
   }
   if (!launch_fits(p.M, 256)) return VNX_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL((k_q8_rows_any<TX, TR, NORM>), dim3((unsigned)p.M), dim3(256), 0, st, p);
+  hipLaunchKernelGGL((k_q8_rows_any<TX, TR, NORM, EPS0>), dim3((unsigned)p.M), dim3(256), 0, st, p);
   VNX_LAUNCH_CHECK();
   return VNX_OK;
 }
