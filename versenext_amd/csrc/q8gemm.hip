@@ -252,12 +252,12 @@ __device__ __forceinline__ void copy_to_lds(uint32_t to, uint32_t off, const int
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                :
                : "s"(to), "v"(off), "s"(base)
-               : "memory");
+               : "memory", "m0");
 }
 
 // Lane l's value at p to LDS at `to` + 4 l.
 __device__ __forceinline__ void copy_to_lds(uint32_t to, const float* p) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" : : "s"(to), "v"(p) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" : : "s"(to), "v"(p) : "memory", "m0");
 }
 
 // Waits until at most N of this wave's copies are under way.
