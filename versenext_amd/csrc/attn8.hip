@@ -81,6 +81,9 @@ struct Q8Params {
 
 __device__ __forceinline__ float q8_ex2(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ uint64_t uni64(uint64_t x) {
+  return (uint64_t)(uint32_t)uni((int)(x >> 32)) << 32 | (uint32_t)uni((int)x);
+}
 
 // Maximum / sum over the four lanes lane % 16 + {0, 16, 32, 48}: v_permlane
 // swaps pair the halves without LDS.
@@ -605,17 +608,20 @@ struct Q8Tile {
       mask.node[ct] = node;
       mask.word[ct] = 0;
       if constexpr (KIND == Q8_TREE) {
-        // Words among the arguments are read by the scalar unit, one node after the
-        // other: a lane's own load from the arguments' memory has returned wrong
-        // words for single lanes (in 18-22 of 40 calls of 2 x 40 nodes over 300 rows
-        // in 32 splits; in none where the same code read them from device memory).
+        // Words among the arguments are read by the scalar unit, as every other
+        // argument, four at a time.  (uni() holds them there: a plain load the
+        // compiler moves under the comparison, and each lane loads its own.)
         if (p.tree == 2) {
           mask.word[ct] = p.anc[b * p.anc_sb + node];
         } else {
           const int last = uni(min(c0 + 16 * ct + 15, p.cols - 1) / p.rep);
-          for (int i = uni(min(c0 + 16 * ct, p.cols - 1) / p.rep); i <= last; ++i) {
-            const uint64_t w = tw.w[i];
-            if (node == i) mask.word[ct] = w;
+          for (int i = uni(min(c0 + 16 * ct, p.cols - 1) / p.rep); i <= last; i += 4) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int n = min(i + j, last);
+              const uint64_t w = uni64(tw.w[n]);
+              if (node == n) mask.word[ct] = w;
+            }
           }
         }
       }
