@@ -642,8 +642,7 @@ class CometSparkGPU:
     def __init__(self, cfg: ModelConfig, weights: Dict[str, torch.Tensor], hip, batch: int, capacity: int,
                  dtype=torch.bfloat16, int4: bool = False, kv_dtype: Optional[torch.dtype] = None,
                  w8a8: bool = False):
-        if w8a8 and (int4 or dtype != torch.bfloat16):
-            raise ValueError("w8a8 needs dtype bfloat16 and int4 False")
+        self._check_w8a8(w8a8, int4, dtype)
         self.w8a8 = bool(w8a8)
         if kv_dtype is not None:
             if kv_dtype not in (torch.int8, torch.float8_e4m3fn):
@@ -774,8 +773,13 @@ class CometSparkGPU:
         # first, the form it is tested against)
         self.embed_fold = True
 
+    @staticmethod
+    def _check_w8a8(w8a8: bool, int4: bool, dtype) -> None:
+        if w8a8 and (int4 or dtype != torch.bfloat16):
+            raise ValueError("w8a8 needs dtype bfloat16 and int4 False")
+
     @classmethod
-    def from_vn(cls, path: str, hip, batch: int, capacity: int, dtype=torch.bfloat16, int4: bool = True,
+    def from_vn(cls, path: str, hip, batch: int, capacity: int, dtype=torch.bfloat16, int4: Optional[bool] = None,
                 chunk_bytes: int = 64 << 20, cfg: Optional[ModelConfig] = None,
                 kv_dtype: Optional[torch.dtype] = None, w8a8: bool = False) -> "CometSparkGPU":
         """The model saved in a .vn file (CometSparkNexLM.save_vn /
@@ -787,7 +791,11 @@ class CometSparkGPU:
         held in full precision.  A tied model's state_dict holds the
         embedding twice (as 'head.weight' too): that copy is skipped.  With
         tie_weights false in the config (cometspark.py:396-398) the stored
-        'head.weight' is the LM head."""
+        'head.weight' is the LM head.  int4 None: True, False with w8a8, whose
+        codes come from the weights as stored."""
+        if int4 is None:
+            int4 = not w8a8
+        cls._check_w8a8(w8a8, int4, dtype)                 # (before the file is read)
         from .vn import VNReader, config_from_vn, int4_matrix, load_vn_weights
         with VNReader(path) as r:
             r.read_meta()
