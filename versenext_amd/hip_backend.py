@@ -16,6 +16,7 @@ zero-initialised workspace that the kernels leave zeroed after every call.
 from __future__ import annotations
 
 import ctypes
+import math
 import threading
 
 import numpy as np
@@ -939,8 +940,12 @@ class HipBackend(DeviceBackend):
                 or out.dtype not in dtypes:
             raise ValueError(f"{what} must be a {shape} tensor of {', '.join(str(d) for d in dtypes)} on "
                              f"{self._torch_device}")
-        K = shape[-1]
-        o = out if out.dim() == 2 else out.view(-1, K)
+        K, o = shape[-1], out
+        if out.dim() != 2:
+            try:
+                o = out.view(math.prod(shape[:-1]), K)
+            except RuntimeError:
+                raise ValueError(f"{what} needs rows at one distance from each other") from None
         if (K > 1 and o.stride(1) != 1) or (o.shape[0] > 1 and o.stride(0) < K) or o.is_neg():
             raise ValueError(f"{what} needs unit last stride and rows that do not overlap")
         return o
