@@ -1,8 +1,9 @@
 // Python binding of the 8-bit KV cache's entries and of the products in 8-bit
 // integers: _vnx_bind.kv_write, kv_read, tree_attn_q8, q8_quantize, q8_rmsnorm,
 // q8_dequantize and q8_linear take tensors, check them, allocate the results and
-// call the C entries of vnx.h, in 1-2 us of host time a call beside the launch's
-// 3.5, where the same checks in Python take 7-13 (a decode step's kernels take 3-9 us).
+// call the C entries of vnx.h, in 1-3 us of host time a call beside the launch's
+// 3.5 (3: q8_rmsnorm's, with three results), where the same checks in Python take
+// 7-13 (a decode step's kernels take 3-9 us).
 //
 // Each function serves the call whose arguments the kernels read as they are.
 // It returns None for every other one (a tensor elsewhere, another type, strides

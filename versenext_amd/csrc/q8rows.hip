@@ -189,7 +189,8 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void k_q8_rows(Q8RowParams p) {
 }
 
 // Rows of any length (fewer than 8 values, or more than a workgroup holds): one
-// workgroup a row, which reads it twice.
+// workgroup a row, which reads it twice, a value a load.  That load bounds it: norm
+// of 2,048 x 40,000 bf16 with a residual 325 us, 1.8 TB/s (32,000 by k_q8_rows 102).
 template <typename TX, typename TR, bool NORM, bool EPS0>
 __global__ __launch_bounds__(256) void k_q8_rows_any(Q8RowParams p) {
   constexpr bool RES = !__is_void(TR);

@@ -282,7 +282,8 @@ __global__ __launch_bounds__(NW * 64, (PF == 2 && D == 64 && NW == 4) ? 2 : 1) v
   // Ancestor words of this lane's query columns.
   // (Two loads of two address spaces under a uniform branch: one load through
   // a selected pointer would be a flat one, which also counts against the LDS
-  // counter; it cost the verify calls 1 us.)
+  // counter; it cost the verify calls 1 us.  Words among the arguments: one
+  // load a lane, the same words call after call by test.)
   auto word = [&](int node) -> uint64_t {
     typedef const __attribute__((address_space(1))) uint64_t* gptr;
     if (p.anc) return *(gptr)(p.anc + b * p.anc_sb + node);
