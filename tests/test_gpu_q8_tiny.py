@@ -55,3 +55,18 @@ def test_weights_that_lift_the_row(hip, K):
     big = torch.ones(K)
     big[0] = 2.0 ** 120               # (one value carries the maximum: 2^-70 * 2^120)
     check(hip, torch.full((2, K), 2.0 ** -70), big, 0.0)
+
+
+@pytest.mark.parametrize("K", WIDTHS)
+@pytest.mark.parametrize("over", [0, 1])
+def test_sum_in_place(hip, K, over):
+    """The sum over x, or over the residual, of rows that are summed twice: the bits of the call that writes elsewhere."""
+    g, dev = R.gen(K), hip.torch_device
+    x, r = ((torch.randn(70, K, generator=g) * 2.0 ** -80).to(dev) for _ in range(2))
+    x[::3] *= 2.0 ** 80
+    w = torch.ones(K, device=dev)
+    want = hip.rmsnorm_q8(x, w, eps=0.0, residual=r)
+    pair = [x.clone(), r.clone()]
+    got = hip.rmsnorm_q8(pair[0], w, eps=0.0, residual=pair[1], sum_out=pair[over])
+    assert got[2] is pair[over] and all(torch.equal(a, b) for a, b in zip(got, want))
+    assert torch.isfinite(got[1]).all() and (got[1] > 0).all()
